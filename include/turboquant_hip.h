@@ -466,6 +466,161 @@ int tq_decode_concurrent_units(int k_bits, int k_qjl, int v_bits, int num_q_head
 int tq_decode_workgroup_waves(int k_bits, int k_qjl, int v_bits, int num_q_heads, int num_kv_heads,
                               int norm_row_bytes, int share_codebook, int* waves);
 
+/* ---- 8-bit paged cache ----------------------------------------------------------- */
+
+/*
+ * A K or V cache of 8 bits a value: one tile per (physical block, KV head) at
+ * cache + block*stride_block + head*stride_head (bytes), tq_kv8_tile_bytes(block_size) bytes:
+ * block_size * 128 codes, the tile's fp32 scale, 12 unused bytes.  A code stands for code * scale;
+ * encoding TQ_E4M3 (OCP fp8 e4m3: 4 exponent bits, 3 of mantissa, largest value 448, one NaN) or
+ * TQ_INT8 (two's complement, -127..127).  The scale is the smallest power of two 2^e, e >= -126, with
+ * (largest finite |x| of the tile) <= 448 * 2^e (127 * 2^e); 0 in a tile that was never written.
+ * Order of the codes: keys row-major [block_size][128]; values in groups of four tokens with the dims
+ * outside, byte 512 g + 4 d + r = dim d of token 4 g + r (TQ_TILE_KEYS / TQ_TILE_VALUES for 8 bits).
+ */
+#define TQ_E4M3 0
+#define TQ_INT8 1
+int64_t tq_kv8_tile_bytes(int block_size);
+
+/*
+ * K and V rows x[t, h, :] of num_tokens tokens into their slots, one launch.  Token t goes to block
+ * slot / block_size, row slot % block_size; negative slots and slots >= num_blocks * block_size are
+ * skipped.  code = x / scale rounded to nearest even; infinities become the largest code, NaN stays NaN
+ * (TQ_E4M3) or becomes 0 (TQ_INT8), and neither counts in the scale.
+ * The scale of a block that is written from row 0 on is that of the new rows alone, and what its other
+ * rows hold is no longer meaningful: a block starts anew with its first row.  Otherwise the
+ * scale never falls: where it grows from 2^e to 2^f the block's other rows are requantised in place,
+ * code -> code * 2^(e - f) rounded to nearest even (exact for e4m3 codes that stay normal).
+ * The tokens of one call that go to one block must be consecutive tokens with consecutive slots (as
+ * a sequence's new tokens are); otherwise, and where a slot is named twice, that block's contents
+ * are unspecified (no access leaves its tile).
+ * Rows: element strides, rows of 128 contiguous elements, pointers 16-byte aligned and strides multiples
+ * of 8 elements; caches 16-byte aligned with strides that are multiples of 16.  block_size: a positive
+ * multiple of 16.
+ */
+typedef struct tq_kv8_update_args {
+    const void* k;
+    const void* v;
+    int64_t k_stride_token, k_stride_head, v_stride_token, v_stride_head;
+    void* k_cache;
+    void* v_cache;
+    int64_t k_stride_block, k_cache_stride_head, v_stride_block, v_cache_stride_head;
+    const void* slot_mapping;
+    int64_t num_tokens, num_blocks;
+    int32_t x_dtype, slot_dtype; /* TQ_F32 / TQ_F16 / TQ_BF16; TQ_I32 / TQ_I64 */
+    int32_t encoding, num_heads, head_dim, block_size;
+} tq_kv8_update_args;
+int tq_kv8_update(const tq_kv8_update_args* a, tq_stream_t stream);
+
+/*
+ * Attention over the 8-bit caches.  tq_kv8_decode: one query token per sequence, q and out
+ * [num_seqs, num_q_heads, 128].  tq_kv8_prefill: sequence s has the query rows cu_seqlens_q[s] ..
+ * cu_seqlens_q[s+1] - 1 of q [T, num_q_heads, 128], its last tokens; with TQ_PREFILL_CAUSAL in flags
+ * query i of n sees the tokens t <= seq_lens[s] - n + i, without it all of them.
+ *   out = sum_t softmax_t(sm_scale * q . k_t) v_t,  k_t, v_t = code * scale
+ * with fp32 (or exact) sums.  q is scaled by a power of two per row to fp16 range and K is exact in
+ * fp16; the probabilities are rounded to fp16 before the product with V.  With q or out of type TQ_F32
+ * q and the probabilities are taken as the sum of two fp16 numbers instead.
+ * A row that sees no token gives 0, as do rows of sequences of length 0.  Block-table entries outside
+ * [0, num_blocks) mask their tokens.  Query rows outside every sequence are not written.  Sequences
+ * longer than the block table (decode: than max_seq_len) are cut there.  max_q_len >= every n.
+ * workspace: tq_kv8_decode_workspace_bytes / tq_kv8_prefill_workspace_bytes of the same sizes, 256-byte
+ * aligned, no initial contents; calls that overlap in time must not share one.  How the keys are cut
+ * over the device follows from all lengths of the call: the same call gives the same bits, the same
+ * row in another batch may differ by rounding.
+ * q and out: rows of 128 contiguous elements, 16-byte aligned, strides multiples of 8 elements;
+ * caches as for tq_kv8_update.  group = num_q_heads / num_kv_heads: 1..16 for decode, any for prefill.
+ */
+typedef struct tq_kv8_attn_args {
+    const void* q;
+    void* out;
+    const void* k_cache;
+    const void* v_cache;
+    const int32_t* block_tables; /* [num_seqs, block_table_stride], max_blocks_per_seq entries each */
+    const int32_t* seq_lens;     /* [num_seqs], tokens in the cache, the new ones included */
+    const int32_t* cu_seqlens_q; /* [num_seqs + 1] (prefill only) */
+    void* workspace;
+    int64_t workspace_bytes;
+    int64_t q_stride_token, q_stride_head, out_stride_token, out_stride_head;
+    int64_t k_stride_block, k_stride_head, v_stride_block, v_stride_head;
+    int64_t num_blocks, block_table_stride;
+    int32_t q_dtype, out_dtype, encoding, num_seqs, num_q_heads, num_kv_heads, head_dim, block_size;
+    int32_t max_blocks_per_seq, max_seq_len, max_q_len, flags;
+    float sm_scale;
+    int32_t reserved; /* 0 */
+} tq_kv8_attn_args;
+int tq_kv8_decode(const tq_kv8_attn_args* a, tq_stream_t stream);
+int tq_kv8_prefill(const tq_kv8_attn_args* a, tq_stream_t stream);
+int64_t tq_kv8_decode_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads);
+int64_t tq_kv8_prefill_workspace_bytes(int num_seqs, int max_q_len, int num_q_heads, int num_kv_heads);
+
+/* ---- rotary positions -------------------------------------------------------------- */
+
+/*
+ * Rotates the pairs of the first rotary_dim elements of every row: with angle a = 2 pi * position *
+ * turns[i], (x, y) -> magnitude * (x cos a - y sin a, y cos a + x sin a); the other elements are copied.
+ * Pair i is (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with interleaved.  The angle's turns are
+ * computed and reduced in 64 bits, so far positions keep their precision; arithmetic in fp32, one rounding.
+ * q [num_tokens, q_heads, 128] and k [num_tokens, k_heads, 128] of one dtype (k_heads 0: q alone);
+ * outputs of the same dtype and shape, which may be the inputs (in place: the same pointer and strides).
+ * positions: int32 or int64 [num_tokens], any sign; turns: fp64 [rotary_dim / 2] on the device.
+ * rotary_dim: even, 2..128.  Element strides; rows of 128 contiguous elements.
+ */
+typedef struct tq_rope_args {
+    const void* q;
+    const void* k;
+    void* q_out;
+    void* k_out;
+    int64_t q_stride_token, q_stride_head, k_stride_token, k_stride_head;
+    int64_t q_out_stride_token, q_out_stride_head, k_out_stride_token, k_out_stride_head;
+    const void* positions;
+    const double* turns;
+    int64_t num_tokens;
+    int32_t dtype, position_dtype, q_heads, k_heads, head_dim, rotary_dim, interleaved;
+    float magnitude;
+} tq_rope_args;
+int tq_rope(const tq_rope_args* a, tq_stream_t stream);
+
+/* ---- step planning -------------------------------------------------------------------- */
+
+/*
+ * What the layers of one engine step need, from the requests' lengths alone, without the host.
+ * Request s holds past[s] cached tokens in the blocks tables[s, 0 .. ceil(past/block_size)) and gets
+ * new_tokens[s] more, or gives up -new_tokens[s] (all of them when it ends; lengths stay >= 0).
+ * Free blocks: a ring of num_blocks ids, pool_in = {first, count}: entries ring[(first + i) %
+ * num_blocks], i < count.  In request order, blocks for new tokens are taken from the ring's front
+ * and written to the table; given-up blocks are read from the table (entries stay) and put at its
+ * end.  Blocks given up in a call are not handed out in it.  A request whose blocks the ring no
+ * longer holds (those of the requests before it counted) or whose table is too narrow
+ * is not extended: its length stays past[s] and its new tokens get slot -1.
+ *   seq_lens[s]          the new length
+ *   query_start_loc[s]   new tokens of the requests before s (num_seqs + 1 entries)
+ *   positions[t], slot_mapping[t] of every new token, t < num_tokens; behind the last one 0 and -1
+ *   pool_out             {first, count} afterwards; may be pool_in
+ * past and seq_lens may be one array.  workspace: tq_plan_step_workspace_bytes(num_seqs) bytes, 16-byte
+ * aligned, no initial contents; calls that overlap must not share it.  num_seqs <= 2^20, max_blocks *
+ * block_size < 2^31.
+ */
+typedef struct tq_plan_args {
+    const int32_t* past;
+    const int32_t* new_tokens;
+    int32_t* tables;
+    int64_t table_stride;
+    int32_t* ring;
+    const int32_t* pool_in;
+    int32_t* pool_out;
+    int32_t* seq_lens;
+    int32_t* query_start_loc;
+    int32_t* positions;
+    int64_t* slot_mapping;
+    void* workspace;
+    int64_t workspace_bytes;
+    int64_t num_tokens;
+    int32_t num_seqs, max_blocks, num_blocks, block_size;
+} tq_plan_args;
+int tq_plan_step(const tq_plan_args* a, tq_stream_t stream);
+int64_t tq_plan_step_workspace_bytes(int num_seqs);
+
 /* ---- packing helpers ----------------------------------------------------------- */
 
 /* Reorder sign rows [n_rows, 16] natural -> stride-4 permuted (out bit 32c+k = in bit 4k+c).

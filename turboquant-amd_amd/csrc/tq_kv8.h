@@ -1,0 +1,185 @@
+// Shared device helpers of the 8-bit paged cache (tq_kv8_*.hip): the tile, its codes and their values.
+//
+// A tile holds block_size tokens of one (physical block, KV head): block_size * 128 codes and one fp32
+// scale, a power of two.  Every conversion between the two is then exact but for the one rounding to the
+// code: x / scale, code * scale and a change of scale are changes of exponent (the rounding shows only where an
+// e4m3 code becomes subnormal, and for int8), results do not depend on how a division rounds, and
+// appending rows one at a time requantises a block at most once per doubling of its largest value.
+#pragma once
+
+#include "tq_common.h"
+
+constexpr int kKv8ScaleBytes = 16;  // fp32 scale and padding behind a tile's codes
+
+typedef _Float16 kv8_half2 __attribute__((ext_vector_type(2)));
+
+template <int ENC>
+struct Kv8Code;
+
+template <>
+struct Kv8Code<TQ_E4M3> {
+    // smallest e with top <= 448 * 2^e: 448 = 1.75 * 2^8, so one is carried where top's mantissa is over 0.75
+    static __device__ __forceinline__ int exponent(uint32_t top_bits) { return (int)((top_bits + 0x1fffffu) >> 23) - 127 - 8; }
+    // four codes of scaled values, the first in the low byte
+    static __device__ __forceinline__ uint32_t pack(float a, float b, float c, float d) {
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(clamp(a), clamp(b), 0, false);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(clamp(c), clamp(d), w, true);
+    }
+    // (only infinities are outside; NaN stays)
+    static __device__ __forceinline__ float clamp(float x) {
+        const float y = __builtin_amdgcn_fmed3f(x, -448.f, 448.f);
+        return x == x ? y : x;
+    }
+    static __device__ __forceinline__ float value(uint32_t w, int i) {
+        return i == 0   ? __builtin_amdgcn_cvt_f32_fp8((int)w, 0)
+               : i == 1 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 1)
+               : i == 2 ? __builtin_amdgcn_cvt_f32_fp8((int)w, 2)
+                        : __builtin_amdgcn_cvt_f32_fp8((int)w, 3);
+    }
+    // fp16 of codes 2h and 2h + 1 of w, times s (a power of two)
+    static __device__ __forceinline__ kv8_half2 half2(uint32_t w, int h, float s) {
+        return h == 0 ? __builtin_bit_cast(kv8_half2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, false))
+                      : __builtin_bit_cast(kv8_half2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, true));
+    }
+};
+
+template <>
+struct Kv8Code<TQ_INT8> {
+    // 127 = 1.984375 * 2^6
+    static __device__ __forceinline__ int exponent(uint32_t top_bits) { return (int)((top_bits + 0x1ffffu) >> 23) - 127 - 6; }
+    static __device__ __forceinline__ uint32_t code(float x) {
+        const float y = __builtin_amdgcn_fmed3f(__builtin_rintf(x == x ? x : 0.f), -127.f, 127.f);
+        return (uint32_t)(int)y & 0xffu;
+    }
+    static __device__ __forceinline__ uint32_t pack(float a, float b, float c, float d) {
+        return code(a) | code(b) << 8 | code(c) << 16 | code(d) << 24;
+    }
+    static __device__ __forceinline__ float value(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
+    // The byte b = code + 128 under the exponent byte 0x64 is the fp16 number 1024 + b; s * (that) - 1152 s is
+    // exact in one fused step (1152 s is a 4-bit multiple of a power of two).
+    static __device__ __forceinline__ kv8_half2 half2(uint32_t w, int h, float s) {
+        const uint32_t x = __builtin_amdgcn_perm(0x64646464u, w ^ 0x80808080u, h == 0 ? 0x04010400u : 0x04030402u);
+        const _Float16 hs = (_Float16)s, hb = (_Float16)(-1152.f * s);
+        return __builtin_elementwise_fma(__builtin_bit_cast(kv8_half2, x), kv8_half2{hs, hs}, kv8_half2{hb, hb});
+    }
+};
+
+// 2^e as fp32, -126 <= e <= 127
+__device__ __forceinline__ float kv8_exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// ---- attention over the tiles: what the decode and prefill kernels share ----
+constexpr float kKv8NegInf = -__builtin_huge_valf();
+constexpr float kKv8None = -1e30f;  // exponent base of a row that has seen no token
+constexpr float kKv8Log2e = 1.4426950408889634f;
+
+struct Kv8Attn {
+    tq_kv8_attn_args a;
+    tq_udiv tpb_div;  // 16-token tiles per block
+    tq_udiv group_div;
+    int tpb, group, cap;  // cap: tokens a block table can hold
+    int workers;          // at most
+    float* ws_acc;        // [slot][row][128]
+    float* ws_ml;         // [slot][row][2]: exponent base (log2), sum
+};
+
+// The factor +-2^k that brings a query row with the largest |x| m to [1, 4), and 2^-k.  Rows that are all zero or
+// not finite keep k = 0.
+__device__ __forceinline__ float kv8_query_factor(float m, bool negate, float& back) {
+    const uint32_t b = __float_as_uint(m) >> 23;
+    int k = 127 - (int)b;
+    if (b == 0 || b == 255) k = 0;
+    k = k > 126 ? 126 : k < -126 ? -126 : k;
+    back = kv8_exp2i(-k);
+    return negate ? -kv8_exp2i(k) : kv8_exp2i(k);
+}
+// x * f as fp16; with FINE, lo gets what the rounding left
+template <bool FINE>
+__device__ __forceinline__ void kv8_query_half(const float (&x)[32], float f, tq_half8 (&hi)[4], tq_half8 (&lo)[4]) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const float y = x[i] * f;
+        hi[i >> 3][i & 7] = (_Float16)y;
+        if (FINE) lo[i >> 3][i & 7] = (_Float16)(y - (float)hi[i >> 3][i & 7]);
+    }
+}
+
+// 32 elements from element off on (16-byte aligned)
+__device__ __forceinline__ void kv8_load32(const void* base, int64_t off, int dt, float (&x)[32]) {
+    if (dt == TQ_F32) {
+        const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(base) + off);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float4 v = s[i];
+            x[4 * i] = v.x;
+            x[4 * i + 1] = v.y;
+            x[4 * i + 2] = v.z;
+            x[4 * i + 3] = v.w;
+        }
+    } else {
+        const tq_u32x4* s = reinterpret_cast<const tq_u32x4*>(static_cast<const uint16_t*>(base) + off);
+        tq_u32x4 raw[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw[i] = s[i];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const uint32_t b = (raw[i >> 3][(i >> 1) & 3] >> (16 * (i & 1))) & 0xffffu;
+            x[i] = dt == TQ_BF16 ? tq_bf16_to_f32(b) : tq_f16_to_f32(b);
+        }
+    }
+}
+
+// N (a multiple of 4) consecutive elements to element off (8-byte aligned for 16-bit types, N = 4)
+template <int N>
+__device__ __forceinline__ void kv8_store(void* base, int64_t off, int dt, const float* o) {
+    if (dt == TQ_F32) {
+        float4* d = reinterpret_cast<float4*>(static_cast<float*>(base) + off);
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) d[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        return;
+    }
+    uint32_t w[N / 2];
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i)
+        w[i] = dt == TQ_BF16 ? (tq_f32_to_bf16_bits(o[2 * i]) | tq_f32_to_bf16_bits(o[2 * i + 1]) << 16)
+                             : tq_pack_half2(o[2 * i], o[2 * i + 1]);
+    uint16_t* d = static_cast<uint16_t*>(base) + off;
+    if constexpr (N % 8 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 8; ++i)
+            reinterpret_cast<tq_u32x4*>(d)[i] = tq_u32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+    } else {
+        *reinterpret_cast<tq_u32x2*>(d) = tq_u32x2{w[0], w[1]};
+    }
+}
+
+// fp16 pairs of p; with FINE, lo gets the remainders
+template <bool FINE>
+__device__ __forceinline__ void kv8_prob8(const float (&p)[8], tq_half8& hi, tq_half8& lo) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        hi[i] = (_Float16)p[i];
+        if (FINE) lo[i] = (_Float16)(p[i] - (float)hi[i]);
+    }
+}
+
+// A tile's V scale relative to the largest (a power of two); below the smallest fp16 number it counts as zero
+__device__ __forceinline__ float kv8_relative(float s, float inv) {
+    const float r = s * inv;
+    return r < 5.9604645e-8f ? 0.f : r;
+}
+
+// Eight fp16 of two code words, four values each, times sa and sb
+template <int ENC>
+__device__ __forceinline__ tq_half8 kv8_half8(uint32_t a, uint32_t b, float sa, float sb) {
+    const kv8_half2 x0 = Kv8Code<ENC>::half2(a, 0, sa), x1 = Kv8Code<ENC>::half2(a, 1, sa);
+    const kv8_half2 x2 = Kv8Code<ENC>::half2(b, 0, sb), x3 = Kv8Code<ENC>::half2(b, 1, sb);
+    return tq_half8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+}
+
+// The word's bytes of the first n of its four tokens
+__device__ __forceinline__ uint32_t kv8_keep(int n) { return n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u; }
+
+// host: checks that decode and prefill share, and the derived fields
+int tq_kv8_attn_setup(const tq_kv8_attn_args* a, Kv8Attn* p);
+// host: compute units of the current device (0: unknown)
+int tq_kv8_cus();

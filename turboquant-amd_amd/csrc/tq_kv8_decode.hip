@@ -1,0 +1,485 @@
+// Decode attention over the 8-bit paged caches: one query token per sequence (tiles: tq_kv8.h).
+//
+// Work is the stream of 32-token steps of the (sequence, KV head) segments, sequences in order and a
+// sequence's KV heads after each other.  Of P steps in all, wave w of R takes steps [floor(w P / R),
+// floor((w + 1) P / R)): found on the device from seq_lens, so no length is needed on the host.  A
+// segment inside one wave is written directly; the pieces of a cut one go to workspace slot w + (segment
+// number), which never repeats since along the waves the segments never decrease, and
+// kv8_decode_merge_kernel joins them.  Each wave works alone: no LDS, no barriers.
+//
+// MFMA layout, lane l, n = l % 16, g = l / 16, tiles A and B of 16 tokens per step:
+//   S^T [16 tokens x 16 heads] = K . Q^T   4 x mfma_f32_16x16x32_f16 per tile; slice cc covers dims 32g + 8cc + (0..7),
+//                                          so the lane's operand is 32 bytes of token n
+//   O^T [dim 8m + a][head] += V^T . P^T    8 x mfma_f32_16x16x32_f16 per step, k = 8g + i being tokens 4g..4g+3 of A, then
+//                                          of B: what S^T leaves in the lane, and a word of the values layout each
+// One pass with the running maximum and sum of the softmax.  The tile's K scale goes into the score's
+// factor; V's scale, relative to the largest met so far, into the conversion to fp16, which is
+// exact (and the accumulators are rescaled when a larger one is met).
+//
+// Bound: HBM reads, 256 bytes per token and KV head.
+#include "tq_kv8.h"
+
+#include <atomic>
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kWavesPerCu = 12;  // resident: 3 per SIMD at up to 168 registers
+constexpr int kMaxWorkers = 256 * kWavesPerCu;
+constexpr int kMinSteps = 2;     // steps a wave takes at least
+
+__device__ __forceinline__ int steps_of(const Kv8Attn& p, int s) {
+    int L = p.a.seq_lens[s];
+    L = L < p.cap ? L : p.cap;
+    return L > 0 ? (L + 31) >> 5 : 0;
+}
+// steps of all sequences (one KV head), every lane
+__device__ __forceinline__ int64_t total_steps(const Kv8Attn& p) {
+    int64_t t = 0;
+    for (int s = threadIdx.x & 63; s < p.a.num_seqs; s += 64) t += steps_of(p, s);
+    for (int m = 32; m >= 1; m >>= 1) t += __shfl_xor(t, m, 64);
+    return t;
+}
+__device__ __forceinline__ int64_t workers_of(const Kv8Attn& p, int64_t P) {
+    const int64_t m = P / kMinSteps;
+    return m < 1 ? 1 : m < p.workers ? m : p.workers;
+}
+
+template <int ENC, bool FINE>
+__global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
+    using Code = Kv8Code<ENC>;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t w = (int64_t)blockIdx.x * kWaves + wave;
+    const int hkv = p.a.num_kv_heads;
+    const int64_t P = total_steps(p) * hkv;
+    const int64_t R = workers_of(p, P);
+    if (P == 0 || w >= R) return;
+    int64_t pos = w * P / R;
+    const int64_t end = (w + 1) * P / R;
+
+    // ---- the sequence that holds step pos ----
+    int s = 0;
+    int64_t seq0 = 0;  // its first step
+    for (int s0 = 0; s0 < p.a.num_seqs; s0 += 64) {
+        const int64_t u = s0 + lane < p.a.num_seqs ? (int64_t)steps_of(p, s0 + lane) * hkv : 0;
+        int64_t in = u;
+        for (int d = 1; d < 64; d <<= 1) {
+            const int64_t x = __shfl_up(in, d, 64);
+            if (lane >= d) in += x;
+        }
+        in += seq0;
+        const uint64_t over = __builtin_amdgcn_ballot_w64(in > pos);
+        if (over) {
+            const int l = __builtin_ctzll(over);
+            s = s0 + l;
+            seq0 = __shfl(in - u, l, 64);
+            break;
+        }
+        seq0 = __shfl(in, 63, 64);
+    }
+    s = __builtin_amdgcn_readfirstlane(s);
+    int np = steps_of(p, s);
+    int kh = (int)((pos - seq0) / np);
+    int64_t seg0 = seq0 + (int64_t)kh * np;
+
+    while (pos < end) {
+        int L = p.a.seq_lens[s];
+        L = __builtin_amdgcn_readfirstlane(L < p.cap ? L : p.cap);
+        const int j0 = __builtin_amdgcn_readfirstlane((int)(pos - seg0));
+        const int j1 = __builtin_amdgcn_readfirstlane((int)(end - seg0 < np ? end - seg0 : np));
+        const uint8_t* kb = static_cast<const uint8_t*>(p.a.k_cache) + kh * p.a.k_stride_head;
+        const uint8_t* vb = static_cast<const uint8_t*>(p.a.v_cache) + kh * p.a.v_stride_head;
+        const int32_t* bt = p.a.block_tables + s * p.a.block_table_stride;
+        const int last_tile = (L - 1) >> 4;
+        const uint32_t scale_at = (uint32_t)p.a.block_size * TQ_HEAD_DIM;
+
+        // ---- 64 tiles' blocks and scales at a time, one per lane ----
+        // block (tiles past the last and bad entries: a valid block and zero tokens), rows in use, scales
+        struct Tiles {
+            int blk, nv;
+            float ks, vs;
+        };
+        auto tiles_from = [&](int t0) -> Tiles {
+            Tiles t;
+            const int ti = t0 + lane;
+            const int tc = ti < last_tile ? ti : last_tile;
+            t.blk = bt[tq_udiv_apply((uint32_t)tc, p.tpb_div)];
+            const int nv = L - 16 * ti;
+            t.nv = nv < 16 ? (nv > 0 ? nv : 0) : 16;
+            if ((uint32_t)t.blk >= (uint64_t)p.a.num_blocks) {
+                t.blk = 0;
+                t.nv = 0;
+            }
+            t.ks = *reinterpret_cast<const float*>(kb + t.blk * p.a.k_stride_block + scale_at);
+            t.vs = *reinterpret_cast<const float*>(vb + t.blk * p.a.v_stride_block + scale_at);
+            return t;
+        };
+        int t0 = 2 * j0;  // first tile of the group at hand
+        Tiles cur = tiles_from(t0), nxt = cur;
+        if (t0 + 64 < 2 * j1) nxt = tiles_from(t0 + 64);
+
+        // ---- the query: heads kh * group + n ----
+        tq_half8 qh[4], ql[4];
+        float c1;
+        {
+            float x[32];
+            const int64_t off = s * p.a.q_stride_token + (int64_t)(kh * p.group + (n < p.group ? n : 0)) * p.a.q_stride_head + 32 * g;
+            kv8_load32(p.a.q, off, p.a.q_dtype, x);
+            float m = 0.f, back;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) m = fmaxf(m, __builtin_fabsf(x[i]));
+            const float f = kv8_query_factor(tq_max_over_groups(m), p.a.sm_scale < 0.f, back);
+            kv8_query_half<FINE>(x, f, qh, ql);
+            c1 = __builtin_fabsf(p.a.sm_scale) * kKv8Log2e * back;
+        }
+
+        uint32_t kw[2][8], vw[2][8];
+        auto load = [&](const uint8_t* tile, uint32_t at, uint32_t (&x)[8]) {
+            const tq_u32x4* src = reinterpret_cast<const tq_u32x4*>(tile + at);
+            const tq_u32x4 a = src[0], b = src[1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[i] = a[i];
+                x[4 + i] = b[i];
+            }
+        };
+        // the tile's codes: block and row within it
+        auto tile_at = [&](int ti, int blk, int64_t stride) -> int64_t {
+            const int tc = ti < last_tile ? ti : last_tile;
+            return blk * stride + (int64_t)(tc - p.tpb * (int)tq_udiv_apply((uint32_t)tc, p.tpb_div)) * (16 * TQ_HEAD_DIM);
+        };
+        const uint32_t k_off = 128 * n + 32 * g, v_off = 512 * g + 32 * n;
+        auto load_keys = [&](const Tiles& t, int i, int ti) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                load(kb + tile_at(ti + h, __builtin_amdgcn_readlane(t.blk, i + h), p.a.k_stride_block), k_off, kw[h]);
+        };
+        auto load_values = [&](const Tiles& t, int i, int ti) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                load(vb + tile_at(ti + h, __builtin_amdgcn_readlane(t.blk, i + h), p.a.v_stride_block), v_off, vw[h]);
+        };
+        load_keys(cur, 0, t0);
+        load_values(cur, 0, t0);
+
+        float M = kKv8None, lsum = 0.f, vref = 0.f;
+        tq_floatx4 acc[8];
+#pragma unroll
+        for (int a = 0; a < 8; ++a) acc[a] = tq_floatx4{0.f, 0.f, 0.f, 0.f};
+
+        for (int j = j0; j < j1; ++j) {
+            const int i = 2 * j - t0;  // lane of tile A in cur
+            const bool more = j + 1 < j1;
+            float ks[2], vs[2];
+            int nv[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                ks[h] = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(cur.ks), i + h));
+                vs[h] = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(cur.vs), i + h));
+                nv[h] = __builtin_amdgcn_readlane(cur.nv, i + h);
+            }
+            // ---- scores of both tiles in log2 units: tokens 4g + r of head n ----
+            float sv[8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                tq_floatx4 sc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int cc = 0; cc < 4; ++cc) {
+                    const tq_half8 a = kv8_half8<ENC>(kw[h][2 * cc], kw[h][2 * cc + 1], 1.f, 1.f);
+                    sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[cc], sc, 0, 0, 0);
+                    if (FINE) sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[cc], sc, 0, 0, 0);
+                }
+                const float f = c1 * ks[h];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sv[4 * h + r] = sc[r] * f;
+            }
+            // the group of 64 tiles used up: the next one takes its place
+            Tiles from = cur;
+            int fi = i + 2;
+            if (more && fi == 64) {
+                from = nxt;
+                fi = 0;
+            }
+            if (more) load_keys(from, fi, 2 * j + 2);
+            if (nv[0] + nv[1] != 32) {
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (4 * g + (r & 3) >= nv[r >> 2]) sv[r] = kKv8NegInf;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t keep = kv8_keep(nv[h] - 4 * g);
+#pragma unroll
+                    for (int a = 0; a < 8; ++a) vw[h][a] &= keep;
+                    if (nv[h] == 0) vs[h] = 0.f;
+                }
+            }
+            // ---- online softmax ----
+            float mx = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
+            if (__builtin_amdgcn_ballot_w64(mx > M)) {
+                const float Mn = fmaxf(M, tq_max_over_groups(mx));
+                const float alpha = __builtin_amdgcn_exp2f(M - Mn);
+                lsum *= alpha;
+#pragma unroll
+                for (int a = 0; a < 8; ++a) acc[a] *= alpha;
+                M = Mn;
+            }
+            float pr[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) pr[r] = __builtin_amdgcn_exp2f(sv[r] - M);
+            lsum += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
+            tq_half8 ph, pl;
+            kv8_prob8<FINE>(pr, ph, pl);
+            const float vmax = fmaxf(vs[0], vs[1]);
+            if (vmax > vref) {  // wave-uniform
+                const float f = vref / vmax;
+#pragma unroll
+                for (int a = 0; a < 8; ++a) acc[a] *= f;
+                vref = vmax;
+            }
+            const float rv = vref > 0.f ? 1.f / vref : 0.f;
+            const float va = kv8_relative(vs[0], rv), vbs = kv8_relative(vs[1], rv);
+#pragma unroll
+            for (int a = 0; a < 8; ++a) {
+                const tq_half8 v = kv8_half8<ENC>(vw[0][a], vw[1][a], va, vbs);
+                acc[a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, acc[a], 0, 0, 0);
+                if (FINE) acc[a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, acc[a], 0, 0, 0);
+            }
+            if (more) load_values(from, fi, 2 * j + 2);
+            if (more && i + 2 == 64) {
+                t0 += 64;
+                cur = nxt;
+                if (t0 + 64 < 2 * j1) nxt = tiles_from(t0 + 64);
+            }
+        }
+
+        // ---- acc[a][r] is dim 32g + 8r + a of head n ----
+        const float l = tq_sum_over_groups(lsum);
+        if (n < p.group) {
+            float o[32];
+            const bool complete = j0 == 0 && j1 == np;
+            const float f = complete ? (l == 0.f ? 0.f : vref / l) : vref;
+#pragma unroll
+            for (int a = 0; a < 8; ++a)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[8 * r + a] = acc[a][r] * f;
+            if (complete) {
+                kv8_store<32>(p.a.out, s * p.a.out_stride_token + (int64_t)(kh * p.group + n) * p.a.out_stride_head + 32 * g,
+                              p.a.out_dtype, o);
+            } else {
+                const int64_t row = (w + (int64_t)s * hkv + kh) * p.group + n;
+                kv8_store<32>(p.ws_acc, row * TQ_HEAD_DIM + 32 * g, TQ_F32, o);
+                if (g == 0) {
+                    p.ws_ml[2 * row] = M;
+                    p.ws_ml[2 * row + 1] = l;
+                }
+            }
+        }
+        // ---- next segment ----
+        pos = seg0 + j1;
+        if (j1 == np) {
+            seg0 += np;
+            if (++kh == hkv) {
+                kh = 0;
+                do {
+                    if (++s >= p.a.num_seqs) return;
+                    np = steps_of(p, s);
+                } while (np == 0);
+            }
+        }
+    }
+}
+
+// Workgroup (s, kh): out = sum_i 2^(M_i - M) acc_i / sum_i 2^(M_i - M) l_i over the pieces of the segment; nothing
+// to do where one wave held it all, zeros where the sequence is empty.  32 lanes a row, 4 dims each; the
+// workgroup's 8 half-waves share the rows, or, with fewer than 8 rows, the pieces of a row.
+__global__ __launch_bounds__(256) void kv8_decode_merge_kernel(Kv8Attn p) {
+    __shared__ int64_t s_sum[2][4];
+    __shared__ float s_part[8][32][6];
+    const int hkv = p.a.num_kv_heads;
+    const int s = (int)(blockIdx.x / (uint32_t)hkv), kh = (int)(blockIdx.x % (uint32_t)hkv);
+    int64_t before = 0, all = 0;
+    for (int i = threadIdx.x; i < p.a.num_seqs; i += 256) {
+        const int u = steps_of(p, i);
+        all += u;
+        if (i < s) before += u;
+    }
+    for (int m = 32; m >= 1; m >>= 1) {
+        before += __shfl_xor(before, m, 64);
+        all += __shfl_xor(all, m, 64);
+    }
+    if ((threadIdx.x & 63) == 0) {
+        s_sum[0][threadIdx.x >> 6] = before;
+        s_sum[1][threadIdx.x >> 6] = all;
+    }
+    __syncthreads();
+    before = s_sum[0][0] + s_sum[0][1] + s_sum[0][2] + s_sum[0][3];
+    const int64_t P = (s_sum[1][0] + s_sum[1][1] + s_sum[1][2] + s_sum[1][3]) * hkv;
+    const int np = steps_of(p, s);
+    int64_t w0 = 0, w1 = -1;
+    if (np > 0) {
+        const int64_t R = workers_of(p, P);
+        const int64_t a = before * hkv + (int64_t)kh * np;
+        // the wave of step x: the largest w with floor(w P / R) <= x
+        w0 = ((a + 1) * R - 1) / P;
+        w1 = ((a + np) * R - 1) / P;
+        if (w0 == w1) return;
+    }
+    const int half = threadIdx.x >> 5, l32 = threadIdx.x & 31;
+    const int64_t seg = (int64_t)s * hkv + kh;
+    int share = 1;  // half-waves of a row
+    while (2 * share * p.group <= 8) share *= 2;
+    const int rows = 8 / share;  // rows at a time
+    for (int r0 = 0; r0 < p.group; r0 += rows) {
+        const int r = r0 + half / share;
+        float M = kKv8NegInf, l = 0.f;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < p.group) {
+            for (int64_t wb = w0 + half % share; wb <= w1; wb += 4 * share) {
+                float mp[4], lp[4];
+                float4 v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int64_t wk = wb + k * share;
+                    mp[k] = kKv8NegInf;
+                    lp[k] = 0.f;
+                    v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (wk <= w1) {
+                        const int64_t row = (wk + seg) * p.group + r;
+                        mp[k] = fmaxf(p.ws_ml[2 * row], kKv8None);  // (also where M is NaN)
+                        lp[k] = p.ws_ml[2 * row + 1];
+                        v[k] = *reinterpret_cast<const float4*>(p.ws_acc + row * TQ_HEAD_DIM + 4 * l32);
+                    }
+                }
+                const float Mn = fmaxf(M, fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])));
+                const float f = M == kKv8NegInf ? 0.f : __builtin_amdgcn_exp2f(M - Mn);
+                l *= f;
+                a.x *= f;
+                a.y *= f;
+                a.z *= f;
+                a.w *= f;
+                M = Mn;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float e = mp[k] == kKv8NegInf ? 0.f : __builtin_amdgcn_exp2f(mp[k] - M);
+                    l = __builtin_fmaf(e, lp[k], l);
+                    a.x = __builtin_fmaf(e, v[k].x, a.x);
+                    a.y = __builtin_fmaf(e, v[k].y, a.y);
+                    a.z = __builtin_fmaf(e, v[k].z, a.z);
+                    a.w = __builtin_fmaf(e, v[k].w, a.w);
+                }
+            }
+        }
+        if (share > 1) {  // workgroup-uniform
+            float* mine = s_part[half][l32];
+            mine[0] = M;
+            mine[1] = l;
+            mine[2] = a.x;
+            mine[3] = a.y;
+            mine[4] = a.z;
+            mine[5] = a.w;
+            __syncthreads();
+            if (half % share == 0 && r < p.group) {
+                for (int k = 1; k < share; ++k) {
+                    const float* o = s_part[half + k][l32];
+                    const float Mn = fmaxf(M, o[0]);
+                    const float f = M == kKv8NegInf ? 0.f : __builtin_amdgcn_exp2f(M - Mn);
+                    const float e = o[0] == kKv8NegInf ? 0.f : __builtin_amdgcn_exp2f(o[0] - Mn);
+                    l = l * f + o[1] * e;
+                    a.x = a.x * f + o[2] * e;
+                    a.y = a.y * f + o[3] * e;
+                    a.z = a.z * f + o[4] * e;
+                    a.w = a.w * f + o[5] * e;
+                    M = Mn;
+                }
+            }
+            __syncthreads();
+        }
+        if (half % share == 0 && r < p.group) {
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const float o[4] = {a.x * inv, a.y * inv, a.z * inv, a.w * inv};
+            kv8_store<4>(p.a.out, s * p.a.out_stride_token + (int64_t)(kh * p.group + r) * p.a.out_stride_head + 4 * l32,
+                         p.a.out_dtype, o);
+        }
+    }
+}
+
+std::atomic<int> g_cus[64];
+
+}  // namespace
+
+int tq_kv8_cus() {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0) return 0;
+    int cus = dev < 64 ? g_cus[dev].load(std::memory_order_relaxed) : 0;
+    if (cus > 0) return cus;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) return 0;
+    if (dev < 64) g_cus[dev].store(cus, std::memory_order_relaxed);
+    return cus;
+}
+
+int tq_kv8_attn_setup(const tq_kv8_attn_args* a, Kv8Attn* p) {
+    if (a->head_dim != TQ_HEAD_DIM) return TQ_ERR_HEAD_DIM;
+    if (a->block_size <= 0 || a->block_size % 16 || a->block_size > 65536) return TQ_ERR_BLOCK_SIZE;
+    for (const int dt : {a->q_dtype, a->out_dtype})
+        if (dt != TQ_F32 && dt != TQ_F16 && dt != TQ_BF16) return TQ_ERR_DTYPE;
+    if (a->encoding != TQ_E4M3 && a->encoding != TQ_INT8) return TQ_ERR_DTYPE;
+    if (a->num_seqs < 0 || a->num_kv_heads <= 0 || a->num_q_heads <= 0 || a->num_blocks <= 0 || a->max_blocks_per_seq < 0 ||
+        a->block_table_stride < a->max_blocks_per_seq || a->num_blocks > INT32_MAX)
+        return TQ_ERR_INVALID_ARGUMENT;
+    if (a->num_q_heads % a->num_kv_heads) return TQ_ERR_GQA;
+    if (!(__builtin_fabsf(a->sm_scale) < __builtin_huge_valf())) return TQ_ERR_INVALID_ARGUMENT;
+    const uintptr_t ptrs = (uintptr_t)a->q | (uintptr_t)a->out | (uintptr_t)a->k_cache | (uintptr_t)a->v_cache;
+    const int64_t el = a->q_stride_token | a->q_stride_head | a->out_stride_token | a->out_stride_head;
+    const int64_t by = a->k_stride_block | a->k_stride_head | a->v_stride_block | a->v_stride_head;
+    if (ptrs % 16 || el % 8 || by % 16) return TQ_ERR_ALIGNMENT;
+    p->a = *a;
+    p->tpb = a->block_size / 16;
+    p->tpb_div = tq_make_udiv((uint32_t)p->tpb);
+    p->group = a->num_q_heads / a->num_kv_heads;
+    p->group_div = tq_make_udiv((uint32_t)p->group);
+    // (positions stay below 2^31 with room for a tile)
+    const int64_t cap = (int64_t)a->max_blocks_per_seq * a->block_size;
+    p->cap = (int)(cap < 0x7fffff00 ? cap : 0x7fffff00);
+    return TQ_OK;
+}
+
+extern "C" int64_t tq_kv8_decode_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads) {
+    if (num_seqs < 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads) return 0;
+    const int64_t slots = kMaxWorkers + (int64_t)num_seqs * num_kv_heads;
+    return slots * (num_q_heads / num_kv_heads) * (TQ_HEAD_DIM + 2) * 4;
+}
+
+extern "C" int tq_kv8_decode(const tq_kv8_attn_args* a, tq_stream_t stream) {
+    if (!a) return TQ_ERR_INVALID_ARGUMENT;
+    Kv8Attn p = {};
+    const int rc = tq_kv8_attn_setup(a, &p);
+    if (rc != TQ_OK) return rc;
+    if (p.group > 16) return TQ_ERR_GQA;
+    if (a->num_seqs == 0) return TQ_OK;
+    if (a->max_seq_len < 0 || (int64_t)a->num_seqs * a->num_kv_heads > INT32_MAX) return TQ_ERR_INVALID_ARGUMENT;
+    if (!a->q || !a->out || !a->k_cache || !a->v_cache || !a->block_tables || !a->seq_lens) return TQ_ERR_INVALID_ARGUMENT;
+    const int64_t need = tq_kv8_decode_workspace_bytes(a->num_seqs, a->num_q_heads, a->num_kv_heads);
+    if (!a->workspace || (uintptr_t)a->workspace % 256 || a->workspace_bytes < need) return TQ_ERR_WORKSPACE;
+    const int cus = tq_kv8_cus();
+    if (cus <= 0) return (int)hipErrorNoDevice;
+    p.cap = p.cap < a->max_seq_len ? p.cap : a->max_seq_len;
+    const int64_t slots = kMaxWorkers + (int64_t)a->num_seqs * a->num_kv_heads;
+    p.ws_acc = static_cast<float*>(a->workspace);
+    p.ws_ml = p.ws_acc + slots * p.group * TQ_HEAD_DIM;
+    // no more waves than the lengths can ask for
+    const int64_t most = (int64_t)a->num_seqs * a->num_kv_heads * ((p.cap + 31) / 32) / kMinSteps;
+    int64_t workers = (int64_t)cus * kWavesPerCu;
+    workers = workers < kMaxWorkers ? workers : kMaxWorkers;
+    workers = workers < most ? workers : most;
+    p.workers = (int)(workers < 1 ? 1 : workers);
+    const bool fine = a->q_dtype == TQ_F32 || a->out_dtype == TQ_F32;
+    const void* kern = a->encoding == TQ_E4M3 ? (fine ? (const void*)kv8_decode_kernel<TQ_E4M3, true> : (const void*)kv8_decode_kernel<TQ_E4M3, false>)
+                                              : (fine ? (const void*)kv8_decode_kernel<TQ_INT8, true> : (const void*)kv8_decode_kernel<TQ_INT8, false>);
+    void* args[] = {&p};
+    hipError_t e = hipLaunchKernel(kern, dim3((unsigned)((p.workers + kWaves - 1) / kWaves)), dim3(64 * kWaves), args, 0, stream);
+    if (e == hipSuccess)
+        e = hipLaunchKernel((const void*)kv8_decode_merge_kernel, dim3((unsigned)(a->num_seqs * a->num_kv_heads)), dim3(256), args, 0, stream);
+    if (e == hipSuccess) e = hipGetLastError();
+    return e == hipSuccess ? TQ_OK : (int)e;
+}

@@ -158,6 +158,16 @@ SIGNATURES = {
         _i32, [_vp, _i32, _i64, _i64, _i32, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
     "tq_compress_packed": (
         _i32, [_vp, _i32, _i64, _i64, _i32, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "tq_kv8_tile_bytes": (_i64, [_i32]),
+    # the argument structs go over as packed bytes (struct.Struct: a call costs a third of its fields as arguments)
+    "tq_kv8_update": (_i32, [ctypes.c_char_p, _vp]),
+    "tq_kv8_decode": (_i32, [ctypes.c_char_p, _vp]),
+    "tq_kv8_prefill": (_i32, [ctypes.c_char_p, _vp]),
+    "tq_kv8_decode_workspace_bytes": (_i64, [_i32, _i32, _i32]),
+    "tq_kv8_prefill_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "tq_rope": (_i32, [ctypes.c_char_p, _vp]),
+    "tq_plan_step": (_i32, [ctypes.c_char_p, _vp]),
+    "tq_plan_step_workspace_bytes": (_i64, [_i32]),
     "tq_permute_signs": (_i32, [_vp, _vp, _i64, _i32, _vp]),
     "tq_unpack_bits": (_i32, [_vp, _vp, _i64, _i32, _i32, _vp]),
 }
@@ -245,6 +255,23 @@ def stream_handle(device: torch.device) -> int:
         return torch.cuda.current_stream(device).cuda_stream
     idx = device.index if device.index is not None else torch.cuda.current_device()
     return _RAW_STREAM(idx)
+
+
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def launch(name: str, device: torch.device, args: bytes) -> None:
+    """Call entry point `name` with its packed argument struct on `device`'s current stream, with `device`
+    current for the call (kernels launch on the current device's code objects)."""
+    fn = getattr(lib(), name)
+    stream = stream_handle(device)
+    if device.index == _CURRENT_DEVICE():
+        rc = fn(args, stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(args, stream)
+    if rc != 0:
+        check(rc, name)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

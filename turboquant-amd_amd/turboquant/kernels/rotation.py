@@ -1,14 +1,18 @@
-"""Stand-alone Walsh-Hadamard rotation of 128-element rows on the GPU.
+"""Stand-alone rotations of 128-element query / key rows on the GPU: Walsh-Hadamard and rotary positions.
 
 wht_rows(x) = x @ make_wht_matrix(128) (the matrix is symmetric and its own inverse), computed
 with fp32 butterflies by tq_wht_rows.  It is the operation of the reference backend's
 TurboQuantFP8State.rotate_query / rotate_output (integration/vllm_backend.py:158-177) for
 callers that rotate outside the decode call; decode_paged(..., rotate=True) fuses both
 rotations into the decode kernels instead.
+
+apply_rope turns the pairs of every row by its token's position (the step before the cache write and, for
+queries, before attention); the frequencies come from turboquant.core.rope.
 """
 
 from __future__ import annotations
 
+import struct
 from typing import Optional
 
 import torch
@@ -53,3 +57,80 @@ def wht_rows(x: torch.Tensor, out: Optional[torch.Tensor] = None) -> torch.Tenso
     if target is not out:
         out.copy_(target)
     return out
+
+
+_ROPE = struct.Struct("@4Q8q2Qq7if")
+_STYLES = {"half": 0, "interleaved": 1}
+
+
+def apply_rope(
+    q: torch.Tensor,
+    k: Optional[torch.Tensor],
+    positions: torch.Tensor,
+    turns: torch.Tensor,
+    style: str = "half",
+    magnitude: float = 1.0,
+    q_out: Optional[torch.Tensor] = None,
+    k_out: Optional[torch.Tensor] = None,
+):
+    """Rotary positions on q [T, Hq, 128] and k [T, Hk, 128] (one dtype of f32 / f16 / bf16); k may be None.
+
+    turns: fp64 [rotary_dim / 2] on the device, the turns of each pair per position (core.rope.rope_turns);
+    positions: int32 or int64 [T], negative ones turn back.  With angle a = 2 pi * position * turns[i] pair
+    i of a row goes to magnitude * (x cos a - y sin a, y cos a + x sin a); angles are reduced in 64 bits.
+    style: "half" pairs element i with i + rotary_dim / 2, "interleaved" 2i with 2i + 1.  Elements from
+    rotary_dim on are copied.  q_out / k_out: destinations of the same shape and dtype, which may be the
+    inputs themselves.  Returns (q_out, k_out).
+    """
+    dev = _lib.require_gpu("apply_rope", q, k, positions, turns, q_out, k_out)
+    if style not in _STYLES:
+        raise ValueError(f"style must be one of {sorted(_STYLES)}, got {style!r}")
+    if turns.dtype != torch.float64 or turns.dim() != 1 or not 1 <= turns.shape[0] <= 64:
+        raise ValueError("turns must be float64 [rotary_dim / 2] with rotary_dim <= 128")
+    if q.dim() != 3 or q.shape[2] != 128:
+        raise ValueError(f"q must be [T, Hq, 128], got {tuple(q.shape)}")
+    T = q.shape[0]
+    if k is not None and (k.dim() != 3 or k.shape[0] != T or k.shape[2] != 128):
+        raise ValueError(f"k must be [{T}, Hk, 128], got {tuple(k.shape)}")
+    if k is not None and k.dtype != q.dtype:
+        raise TypeError("q and k must share a dtype")
+    if positions.dim() != 1 or positions.shape[0] != T:
+        raise ValueError("positions must be [T]")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError("positions must be int32 or int64")
+    if k is None and k_out is not None:
+        raise ValueError("k_out needs k")
+    turns, positions = turns.contiguous(), positions.contiguous()
+
+    def pair(x, out):
+        """(source, destination, copy the destination back to): what the kernel reads and writes."""
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        elif out.shape != x.shape or out.dtype != x.dtype:
+            raise ValueError("destinations must have their input's shape and dtype")
+        dst = out
+        if out.stride(2) != 1 or (out.data_ptr() == x.data_ptr() and out.stride() != x.stride()):
+            dst = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        if x.stride(2) != 1:
+            x = x.contiguous()
+        return x, dst, out
+
+    q, qd, q_out = pair(q, q_out)
+    kd, hk = None, 0
+    if k is not None:
+        k, kd, k_out = pair(k, k_out)
+        hk = k.shape[1]
+    if T:
+        qt, qh, _ = q.stride()
+        qot, qoh, _ = qd.stride()
+        kt, kh, _ = k.stride() if hk else (0, 0, 1)
+        kot, koh, _ = kd.stride() if hk else (0, 0, 1)
+        args = _ROPE.pack(q.data_ptr(), k.data_ptr() if hk else 0, qd.data_ptr(), kd.data_ptr() if hk else 0, qt, qh, kt, kh,
+                          qot, qoh, kot, koh, positions.data_ptr(), turns.data_ptr(), T, _lib.dtype_code(q),
+                          _lib.dtype_code(positions), q.shape[1], hk, 128, 2 * turns.shape[0], _STYLES[style], float(magnitude))
+        _lib.launch("tq_rope", dev, args)
+    if qd is not q_out:
+        q_out.copy_(qd)
+    if kd is not k_out:
+        k_out.copy_(kd)
+    return q_out, k_out
