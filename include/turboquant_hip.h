@@ -552,7 +552,8 @@ typedef struct tq_kv8_attn_args {
 int tq_kv8_decode(const tq_kv8_attn_args* a, tq_stream_t stream);
 int tq_kv8_prefill(const tq_kv8_attn_args* a, tq_stream_t stream);
 int64_t tq_kv8_decode_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads);
-int64_t tq_kv8_prefill_workspace_bytes(int num_seqs, int max_q_len, int num_q_heads, int num_kv_heads);
+int64_t tq_kv8_prefill_workspace_bytes(int num_seqs, int max_q_len, int num_q_heads, int num_kv_heads,
+                                       int max_blocks_per_seq, int block_size);
 
 /* ---- rotary positions -------------------------------------------------------------- */
 

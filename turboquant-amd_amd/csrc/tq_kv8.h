@@ -162,6 +162,18 @@ __device__ __forceinline__ void kv8_prob8(const float (&p)[8], tq_half8& hi, tq_
     }
 }
 
+// Their sum in fp32: of the numbers that the product with V sees, so that the rounding of a probability that
+// dominates its row cancels.
+template <bool FINE>
+__device__ __forceinline__ float kv8_sum8(const float (&p)[8], const tq_half8& hi) {
+    if (FINE) return ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+    const kv8_half2 one = {(_Float16)1.f, (_Float16)1.f};
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sum = __builtin_amdgcn_fdot2(kv8_half2{hi[2 * k], hi[2 * k + 1]}, one, sum, false);
+    return sum;
+}
+
 // A tile's V scale relative to the largest (a power of two); below the smallest fp16 number it counts as zero
 __device__ __forceinline__ float kv8_relative(float s, float inv) {
     const float r = s * inv;

@@ -115,9 +115,7 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
             t.vs = *reinterpret_cast<const float*>(vb + t.blk * p.a.v_stride_block + scale_at);
             return t;
         };
-        int t0 = 2 * j0;  // first tile of the group at hand
-        Tiles cur = tiles_from(t0), nxt = cur;
-        if (t0 + 64 < 2 * j1) nxt = tiles_from(t0 + 64);
+        Tiles nxt = tiles_from(2 * j0);
 
         // ---- the query: heads kh * group + n ----
         tq_half8 qh[4], ql[4];
@@ -150,27 +148,39 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
             return blk * stride + (int64_t)(tc - p.tpb * (int)tq_udiv_apply((uint32_t)tc, p.tpb_div)) * (16 * TQ_HEAD_DIM);
         };
         const uint32_t k_off = 128 * n + 32 * g, v_off = 512 * g + 32 * n;
-        auto load_keys = [&](const Tiles& t, int i, int ti) {
+        auto load_keys = [&](int b0, int b1, int ti) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                load(kb + tile_at(ti + h, __builtin_amdgcn_readlane(t.blk, i + h), p.a.k_stride_block), k_off, kw[h]);
+            for (int h = 0; h < 2; ++h) load(kb + tile_at(ti + h, h ? b1 : b0, p.a.k_stride_block), k_off, kw[h]);
         };
-        auto load_values = [&](const Tiles& t, int i, int ti) {
+        auto load_values = [&](int b0, int b1, int ti) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                load(vb + tile_at(ti + h, __builtin_amdgcn_readlane(t.blk, i + h), p.a.v_stride_block), v_off, vw[h]);
+            for (int h = 0; h < 2; ++h) load(vb + tile_at(ti + h, h ? b1 : b0, p.a.v_stride_block), v_off, vw[h]);
         };
-        load_keys(cur, 0, t0);
-        load_values(cur, 0, t0);
+        // (the loads of step j + 1 go out during step j without a condition, the last step repeats its own: where the
+        // compiler cannot count what is under way, it waits for all of it)
+        {
+            const int b0 = __builtin_amdgcn_readlane(nxt.blk, 0), b1 = __builtin_amdgcn_readlane(nxt.blk, 1);
+            load_keys(b0, b1, 2 * j0);
+            load_values(b0, b1, 2 * j0);
+        }
 
         float M = kKv8None, lsum = 0.f, vref = 0.f;
         tq_floatx4 acc[8];
 #pragma unroll
         for (int a = 0; a < 8; ++a) acc[a] = tq_floatx4{0.f, 0.f, 0.f, 0.f};
 
-        for (int j = j0; j < j1; ++j) {
+        for (int jg = j0; jg < j1; jg += 32) {  // 32 steps: 64 tiles
+        const int t0 = 2 * jg, je = jg + 32 < j1 ? jg + 32 : j1;
+        const Tiles cur = nxt;
+        if (t0 + 64 < 2 * j1) nxt = tiles_from(t0 + 64);
+        for (int j = jg; j < je; ++j) {
             const int i = 2 * j - t0;  // lane of tile A in cur
             const bool more = j + 1 < j1;
+            // the next step's tiles
+            const int jn = more ? j + 1 : j, fi = (more ? i + 2 : i) & 63;
+            const bool over = more && i == 62;
+            const int nb0 = over ? __builtin_amdgcn_readlane(nxt.blk, 0) : __builtin_amdgcn_readlane(cur.blk, fi);
+            const int nb1 = over ? __builtin_amdgcn_readlane(nxt.blk, 1) : __builtin_amdgcn_readlane(cur.blk, fi + 1);
             float ks[2], vs[2];
             int nv[2];
 #pragma unroll
@@ -194,14 +204,7 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) sv[4 * h + r] = sc[r] * f;
             }
-            // the group of 64 tiles used up: the next one takes its place
-            Tiles from = cur;
-            int fi = i + 2;
-            if (more && fi == 64) {
-                from = nxt;
-                fi = 0;
-            }
-            if (more) load_keys(from, fi, 2 * j + 2);
+            load_keys(nb0, nb1, 2 * jn);
             if (nv[0] + nv[1] != 32) {
 #pragma unroll
                 for (int r = 0; r < 8; ++r)
@@ -227,9 +230,9 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
             float pr[8];
 #pragma unroll
             for (int r = 0; r < 8; ++r) pr[r] = __builtin_amdgcn_exp2f(sv[r] - M);
-            lsum += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
             tq_half8 ph, pl;
             kv8_prob8<FINE>(pr, ph, pl);
+            lsum += kv8_sum8<FINE>(pr, ph);
             const float vmax = fmaxf(vs[0], vs[1]);
             if (vmax > vref) {  // wave-uniform
                 const float f = vref / vmax;
@@ -245,12 +248,8 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
                 acc[a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, acc[a], 0, 0, 0);
                 if (FINE) acc[a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, acc[a], 0, 0, 0);
             }
-            if (more) load_values(from, fi, 2 * j + 2);
-            if (more && i + 2 == 64) {
-                t0 += 64;
-                cur = nxt;
-                if (t0 + 64 < 2 * j1) nxt = tiles_from(t0 + 64);
-            }
+            load_values(nb0, nb1, 2 * jn);
+        }
         }
 
         // ---- acc[a][r] is dim 32g + 8r + a of head n ----

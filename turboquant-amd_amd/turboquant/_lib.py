@@ -164,7 +164,7 @@ SIGNATURES = {
     "tq_kv8_decode": (_i32, [ctypes.c_char_p, _vp]),
     "tq_kv8_prefill": (_i32, [ctypes.c_char_p, _vp]),
     "tq_kv8_decode_workspace_bytes": (_i64, [_i32, _i32, _i32]),
-    "tq_kv8_prefill_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32]),
+    "tq_kv8_prefill_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
     "tq_rope": (_i32, [ctypes.c_char_p, _vp]),
     "tq_plan_step": (_i32, [ctypes.c_char_p, _vp]),
     "tq_plan_step_workspace_bytes": (_i64, [_i32]),

@@ -188,7 +188,7 @@ def _attention(name, q, k_cache, k_fmt, v_cache, v_fmt, block_tables, seq_lens, 
     if cu_seqlens_q is None:
         need = _lib.lib().tq_kv8_decode_workspace_bytes(S, hq, hkv)
     else:
-        need = _lib.lib().tq_kv8_prefill_workspace_bytes(S, max_q_len, hq, hkv)
+        need = _lib.lib().tq_kv8_prefill_workspace_bytes(S, max_q_len, hq, hkv, block_tables.shape[1], k_fmt.block_size)
     if workspace is None:
         # (a buffer of this call: of the current stream, and of the graph under capture)
         workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
