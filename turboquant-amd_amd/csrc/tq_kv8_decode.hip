@@ -26,7 +26,7 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kWavesPerCu = 12;  // resident: 3 per SIMD at up to 168 registers
 constexpr int kMaxWorkers = 256 * kWavesPerCu;
-constexpr int kMinSteps = 2;     // steps a wave takes at least
+constexpr int kMinSteps = 2;     // steps a wave takes at least (1 x 4099 tokens: 1 18.2 us, 2 16.9, 4 16.9, 8 18.9)
 
 __device__ __forceinline__ int steps_of(const Kv8Attn& p, int s) {
     int L = p.a.seq_lens[s];
@@ -289,14 +289,16 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
     }
 }
 
-// Workgroup (s, kh): out = sum_i 2^(M_i - M) acc_i / sum_i 2^(M_i - M) l_i over the pieces of the segment; nothing
-// to do where one wave held it all, zeros where the sequence is empty.  32 lanes a row, 4 dims each; the
-// workgroup's 8 half-waves share the rows, or, with fewer than 8 rows, the pieces of a row.
+// Workgroup (s, head): out = sum_i 2^(M_i - M) acc_i / sum_i 2^(M_i - M) l_i over the pieces of the head's segment; nothing
+// to do where one wave held it all, zeros where the sequence is empty.  The workgroup's 8 half-waves share the
+// pieces, a lane has 4 dims.  (With a workgroup per KV head, one sequence of 4099 tokens: merge 13.6 -> 6.6 us.)
 __global__ __launch_bounds__(256) void kv8_decode_merge_kernel(Kv8Attn p) {
     __shared__ int64_t s_sum[2][4];
-    __shared__ float s_part[8][32][6];
+    __shared__ float4 s_acc[8][32];
+    __shared__ float2 s_ml[8];
     const int hkv = p.a.num_kv_heads;
-    const int s = (int)(blockIdx.x / (uint32_t)hkv), kh = (int)(blockIdx.x % (uint32_t)hkv);
+    const int s = (int)(blockIdx.x / (uint32_t)p.a.num_q_heads), head = (int)(blockIdx.x % (uint32_t)p.a.num_q_heads);
+    const int kh = head / p.group, r = head - kh * p.group;
     int64_t before = 0, all = 0;
     for (int i = threadIdx.x; i < p.a.num_seqs; i += 256) {
         const int u = steps_of(p, i);
@@ -326,81 +328,65 @@ __global__ __launch_bounds__(256) void kv8_decode_merge_kernel(Kv8Attn p) {
     }
     const int half = threadIdx.x >> 5, l32 = threadIdx.x & 31;
     const int64_t seg = (int64_t)s * hkv + kh;
-    int share = 1;  // half-waves of a row
-    while (2 * share * p.group <= 8) share *= 2;
-    const int rows = 8 / share;  // rows at a time
-    for (int r0 = 0; r0 < p.group; r0 += rows) {
-        const int r = r0 + half / share;
-        float M = kKv8NegInf, l = 0.f;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (r < p.group) {
-            for (int64_t wb = w0 + half % share; wb <= w1; wb += 4 * share) {
-                float mp[4], lp[4];
-                float4 v[4];
+    float M = kKv8NegInf, l = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int64_t wb = w0 + half; wb <= w1; wb += 4 * 8) {
+        float mp[4], lp[4];
+        float4 v[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int64_t wk = wb + k * share;
-                    mp[k] = kKv8NegInf;
-                    lp[k] = 0.f;
-                    v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (wk <= w1) {
-                        const int64_t row = (wk + seg) * p.group + r;
-                        mp[k] = fmaxf(p.ws_ml[2 * row], kKv8None);  // (also where M is NaN)
-                        lp[k] = p.ws_ml[2 * row + 1];
-                        v[k] = *reinterpret_cast<const float4*>(p.ws_acc + row * TQ_HEAD_DIM + 4 * l32);
-                    }
-                }
-                const float Mn = fmaxf(M, fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])));
-                const float f = M == kKv8NegInf ? 0.f : __builtin_amdgcn_exp2f(M - Mn);
-                l *= f;
-                a.x *= f;
-                a.y *= f;
-                a.z *= f;
-                a.w *= f;
-                M = Mn;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float e = mp[k] == kKv8NegInf ? 0.f : __builtin_amdgcn_exp2f(mp[k] - M);
-                    l = __builtin_fmaf(e, lp[k], l);
-                    a.x = __builtin_fmaf(e, v[k].x, a.x);
-                    a.y = __builtin_fmaf(e, v[k].y, a.y);
-                    a.z = __builtin_fmaf(e, v[k].z, a.z);
-                    a.w = __builtin_fmaf(e, v[k].w, a.w);
-                }
+        for (int k = 0; k < 4; ++k) {
+            const int64_t wk = wb + k * 8;
+            mp[k] = kKv8NegInf;
+            lp[k] = 0.f;
+            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (wk <= w1) {
+                const int64_t row = (wk + seg) * p.group + r;
+                mp[k] = fmaxf(p.ws_ml[2 * row], kKv8None);  // (also where M is NaN)
+                lp[k] = p.ws_ml[2 * row + 1];
+                v[k] = *reinterpret_cast<const float4*>(p.ws_acc + row * TQ_HEAD_DIM + 4 * l32);
             }
         }
-        if (share > 1) {  // workgroup-uniform
-            float* mine = s_part[half][l32];
-            mine[0] = M;
-            mine[1] = l;
-            mine[2] = a.x;
-            mine[3] = a.y;
-            mine[4] = a.z;
-            mine[5] = a.w;
-            __syncthreads();
-            if (half % share == 0 && r < p.group) {
-                for (int k = 1; k < share; ++k) {
-                    const float* o = s_part[half + k][l32];
-                    const float Mn = fmaxf(M, o[0]);
-                    const float f = M == kKv8NegInf ? 0.f : __builtin_amdgcn_exp2f(M - Mn);
-                    const float e = o[0] == kKv8NegInf ? 0.f : __builtin_amdgcn_exp2f(o[0] - Mn);
-                    l = l * f + o[1] * e;
-                    a.x = a.x * f + o[2] * e;
-                    a.y = a.y * f + o[3] * e;
-                    a.z = a.z * f + o[4] * e;
-                    a.w = a.w * f + o[5] * e;
-                    M = Mn;
-                }
-            }
-            __syncthreads();
-        }
-        if (half % share == 0 && r < p.group) {
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            const float o[4] = {a.x * inv, a.y * inv, a.z * inv, a.w * inv};
-            kv8_store<4>(p.a.out, s * p.a.out_stride_token + (int64_t)(kh * p.group + r) * p.a.out_stride_head + 4 * l32,
-                         p.a.out_dtype, o);
+        const float Mn = fmaxf(M, fmaxf(fmaxf(mp[0], mp[1]), fmaxf(mp[2], mp[3])));
+        const float f = M == kKv8NegInf ? 0.f : __builtin_amdgcn_exp2f(M - Mn);
+        l *= f;
+        a.x *= f;
+        a.y *= f;
+        a.z *= f;
+        a.w *= f;
+        M = Mn;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float e = mp[k] == kKv8NegInf ? 0.f : __builtin_amdgcn_exp2f(mp[k] - M);
+            l = __builtin_fmaf(e, lp[k], l);
+            a.x = __builtin_fmaf(e, v[k].x, a.x);
+            a.y = __builtin_fmaf(e, v[k].y, a.y);
+            a.z = __builtin_fmaf(e, v[k].z, a.z);
+            a.w = __builtin_fmaf(e, v[k].w, a.w);
         }
     }
+    s_acc[half][l32] = a;
+    if (l32 == 0) s_ml[half] = make_float2(M, l);
+    __syncthreads();
+    if (half) return;
+    float Mn = kKv8NegInf;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) Mn = fmaxf(Mn, s_ml[k].x);
+    l = 0.f;
+    a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float2 ml = s_ml[k];
+        const float4 v = s_acc[k][l32];
+        const float e = ml.x == kKv8NegInf ? 0.f : __builtin_amdgcn_exp2f(ml.x - Mn);
+        l = __builtin_fmaf(e, ml.y, l);
+        a.x = __builtin_fmaf(e, v.x, a.x);
+        a.y = __builtin_fmaf(e, v.y, a.y);
+        a.z = __builtin_fmaf(e, v.z, a.z);
+        a.w = __builtin_fmaf(e, v.w, a.w);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float o[4] = {a.x * inv, a.y * inv, a.z * inv, a.w * inv};
+    kv8_store<4>(p.a.out, s * p.a.out_stride_token + (int64_t)head * p.a.out_stride_head + 4 * l32, p.a.out_dtype, o);
 }
 
 std::atomic<int> g_cus[64];
@@ -456,7 +442,7 @@ extern "C" int tq_kv8_decode(const tq_kv8_attn_args* a, tq_stream_t stream) {
     if (rc != TQ_OK) return rc;
     if (p.group > 16) return TQ_ERR_GQA;
     if (a->num_seqs == 0) return TQ_OK;
-    if (a->max_seq_len < 0 || (int64_t)a->num_seqs * a->num_kv_heads > INT32_MAX) return TQ_ERR_INVALID_ARGUMENT;
+    if (a->max_seq_len < 0 || (int64_t)a->num_seqs * a->num_q_heads > INT32_MAX) return TQ_ERR_INVALID_ARGUMENT;
     if (!a->q || !a->out || !a->k_cache || !a->v_cache || !a->block_tables || !a->seq_lens) return TQ_ERR_INVALID_ARGUMENT;
     const int64_t need = tq_kv8_decode_workspace_bytes(a->num_seqs, a->num_q_heads, a->num_kv_heads);
     if (!a->workspace || (uintptr_t)a->workspace % 256 || a->workspace_bytes < need) return TQ_ERR_WORKSPACE;
@@ -478,7 +464,7 @@ extern "C" int tq_kv8_decode(const tq_kv8_attn_args* a, tq_stream_t stream) {
     void* args[] = {&p};
     hipError_t e = hipLaunchKernel(kern, dim3((unsigned)((p.workers + kWaves - 1) / kWaves)), dim3(64 * kWaves), args, 0, stream);
     if (e == hipSuccess)
-        e = hipLaunchKernel((const void*)kv8_decode_merge_kernel, dim3((unsigned)(a->num_seqs * a->num_kv_heads)), dim3(256), args, 0, stream);
+        e = hipLaunchKernel((const void*)kv8_decode_merge_kernel, dim3((unsigned)(a->num_seqs * a->num_q_heads)), dim3(256), args, 0, stream);
     if (e == hipSuccess) e = hipGetLastError();
     return e == hipSuccess ? TQ_OK : (int)e;
 }

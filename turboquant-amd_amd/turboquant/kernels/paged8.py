@@ -34,7 +34,9 @@ SCALE_BYTES = 16
 
 @dataclass(frozen=True)
 class Paged8Format:
-    """Geometry of one 8-bit paged cache.  layout: "keys" for a K cache, "values" for a V cache."""
+    """Geometry of one 8-bit paged cache.  layout: "keys" for a K cache, "values" for a V cache.
+
+    code_bytes and tile_bytes: bytes of a tile's codes and of the whole tile."""
 
     encoding: str = "e4m3"
     block_size: int = 16
@@ -50,6 +52,10 @@ class Paged8Format:
             raise ValueError(f"layout must be 'keys' or 'values', got {self.layout!r}")
         if self.head_dim != 128:
             raise ValueError("head_dim must be 128")
+        # (worked out once: every call reads them)
+        object.__setattr__(self, "code_bytes", self.block_size * self.head_dim)
+        object.__setattr__(self, "tile_bytes", self.code_bytes + SCALE_BYTES)
+        object.__setattr__(self, "encoding_code", _ENCODINGS[self.encoding])
 
     @classmethod
     def for_keys(cls, encoding: str = "e4m3", block_size: int = 16) -> "Paged8Format":
@@ -58,14 +64,6 @@ class Paged8Format:
     @classmethod
     def for_values(cls, encoding: str = "e4m3", block_size: int = 16) -> "Paged8Format":
         return cls(encoding, block_size, "values")
-
-    @property
-    def code_bytes(self) -> int:
-        return self.block_size * self.head_dim
-
-    @property
-    def tile_bytes(self) -> int:
-        return self.code_bytes + SCALE_BYTES
 
 
 def dequantize_paged8(cache: torch.Tensor, fmt: Paged8Format) -> torch.Tensor:
@@ -79,7 +77,8 @@ def dequantize_paged8(cache: torch.Tensor, fmt: Paged8Format) -> torch.Tensor:
     return x * cache[..., n:n + 4].contiguous().view(torch.float32)[..., None]
 
 
-def _check_cache(cache: torch.Tensor, fmt: Paged8Format, what: str) -> None:
+def _check_cache(cache: torch.Tensor, fmt: Paged8Format, what: str) -> tuple[int, int]:
+    """The cache's block and head strides."""
     if cache.dtype != torch.uint8 or cache.dim() != 3:
         raise ValueError(f"{what}: cache must be uint8 [num_blocks, num_kv_heads, tile_bytes]")
     sb, sh, s1 = cache.stride()
@@ -87,17 +86,21 @@ def _check_cache(cache: torch.Tensor, fmt: Paged8Format, what: str) -> None:
         raise ValueError(f"{what}: cache tiles must hold {fmt.tile_bytes} contiguous bytes")
     if (sb | sh | cache.data_ptr()) % 16:
         raise ValueError(f"{what}: cache tiles must be 16-byte aligned")
+    return sb, sh
 
 
-def _check_pair(k_cache, k_fmt, v_cache, v_fmt, what: str) -> None:
-    _check_cache(k_cache, k_fmt, what + " (K)")
-    _check_cache(v_cache, v_fmt, what + " (V)")
+def _check_pair(k_cache, k_fmt, v_cache, v_fmt, what: str) -> tuple[int, int, int, int, int, int]:
+    """(blocks, heads, K block stride, K head stride, V block stride, V head stride)."""
+    kb, kh = _check_cache(k_cache, k_fmt, what)
+    vb, vh = _check_cache(v_cache, v_fmt, what)
     if k_fmt.layout != "keys" or v_fmt.layout != "values":
         raise ValueError(f"{what}: the K cache takes layout='keys', the V cache layout='values'")
     if k_fmt.block_size != v_fmt.block_size or k_fmt.encoding != v_fmt.encoding:
         raise ValueError(f"{what}: K and V caches must share block_size and encoding")
-    if k_cache.shape[:2] != v_cache.shape[:2]:
+    nb, heads, _ = k_cache.shape
+    if v_cache.shape[0] != nb or v_cache.shape[1] != heads:
         raise ValueError(f"{what}: K and V caches must have the same [num_blocks, num_kv_heads]")
+    return nb, heads, kb, kh, vb, vh
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -132,9 +135,9 @@ def quantize_paged8_kv(
     if k.dtype != v.dtype:
         raise TypeError("k and v must share a dtype")
     T, H, _ = k.shape
-    _check_pair(k_cache, k_fmt, v_cache, v_fmt, "quantize_paged8_kv")
-    if k_cache.shape[1] != H:
-        raise ValueError(f"caches have {k_cache.shape[1]} heads, k and v {H}")
+    nb, heads, kb, kc, vb, vc = _check_pair(k_cache, k_fmt, v_cache, v_fmt, "quantize_paged8_kv")
+    if heads != H:
+        raise ValueError(f"caches have {heads} heads, k and v {H}")
     if slot_mapping.dim() != 1 or slot_mapping.shape[0] != T:
         raise ValueError("slot_mapping must be [T]")
     if slot_mapping.dtype not in (torch.int32, torch.int64):
@@ -142,69 +145,64 @@ def quantize_paged8_kv(
     k, v, slot_mapping = _rows(k), _rows(v), slot_mapping.contiguous()
     kt, kh, _ = k.stride()
     vt, vh, _ = v.stride()
-    kb, kc, _ = k_cache.stride()
-    vb, vc, _ = v_cache.stride()
     args = _UPDATE.pack(k.data_ptr(), v.data_ptr(), kt, kh, vt, vh, k_cache.data_ptr(), v_cache.data_ptr(), kb, kc, vb, vc,
-                        slot_mapping.data_ptr(), T, k_cache.shape[0], _lib.dtype_code(k), _lib.dtype_code(slot_mapping),
-                        _ENCODINGS[k_fmt.encoding], H, 128, k_fmt.block_size)
+                        slot_mapping.data_ptr(), T, nb, _lib.dtype_code(k), _lib.dtype_code(slot_mapping),
+                        k_fmt.encoding_code, H, 128, k_fmt.block_size)
     _lib.launch("tq_kv8_update", dev, args)
     return k_cache, v_cache
 
 
 _ATTN = struct.Struct("@8Q11q12ifi")
+_SCALE = 1.0 / math.sqrt(128)
 
 
-def _attention(name, q, k_cache, k_fmt, v_cache, v_fmt, block_tables, seq_lens, cu_seqlens_q, sm_scale, max_seq_len, max_q_len,
-               flags, out, workspace, dev):
+def _attention(name, dev, q, caches, k_cache, v_cache, k_fmt, block_tables, seq_lens, cu_seqlens_q, sm_scale, max_seq_len,
+               max_q_len, flags, out, workspace):
     rows, hq, _ = q.shape
-    S = seq_lens.shape[0]
-    hkv = k_cache.shape[1]
-    if not hkv or hq % hkv:
-        raise ValueError(f"num_q_heads {hq} must be a multiple of num_kv_heads {hkv}")
+    nb, hkv, kb, kh, vb, vh = caches
+    S, mb = block_tables.shape if block_tables.dim() == 2 else (-1, 0)
+    if S != seq_lens.shape[0] or (mb > 1 and block_tables.stride(1) != 1):
+        raise ValueError("block_tables must be [num_seqs, max_blocks] with unit inner stride")
     if block_tables.dtype != torch.int32 or seq_lens.dtype != torch.int32:
         raise TypeError("block_tables and seq_lens must be int32")
-    if block_tables.dim() != 2 or block_tables.shape[0] != S or (block_tables.stride(1) != 1 and block_tables.shape[1] > 1):
-        raise ValueError("block_tables must be [num_seqs, max_blocks] with unit inner stride")
-    if not k_cache.shape[0]:
+    if not hkv or hq % hkv:
+        raise ValueError(f"num_q_heads {hq} must be a multiple of num_kv_heads {hkv}")
+    if not nb:
         raise ValueError("the caches hold no blocks")
+    if out is not None and (out.shape != q.shape or out.device != q.device):
+        raise ValueError("out must have q's shape and device")
+    scale = _SCALE if sm_scale is None else float(sm_scale)
+    if not math.isfinite(scale):
+        raise ValueError("sm_scale must be finite")
     seq_lens = seq_lens.contiguous()
     q = _rows(q)
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.device != q.device:
-        raise ValueError("out must have q's shape and device")
-    scale = 1.0 / math.sqrt(128) if sm_scale is None else float(sm_scale)
-    if not math.isfinite(scale):
-        raise ValueError("sm_scale must be finite")
     if not rows or not hq:
         return out
-    st, sh, s1 = out.stride()
-    # (a destination that takes no vector stores gets a copy of the result)
-    target = out if s1 == 1 and not (st | sh) % 8 and not out.data_ptr() % 16 else torch.empty_like(
-        out, memory_format=torch.contiguous_format)
-    if target is not out and cu_seqlens_q is not None:
-        target.copy_(out)  # rows of no sequence stay as they were
-    ot, oh, _ = target.stride()
+    target = out
+    ot, oh, o1 = out.stride()
+    if o1 != 1 or (ot | oh) % 8 or out.data_ptr() % 16:
+        # a destination that takes no vector stores gets a copy of the result (rows of no sequence stay as they were)
+        target = out.clone(memory_format=torch.contiguous_format)
+        ot, oh, _ = target.stride()
+    L = _lib.lib()
     if cu_seqlens_q is None:
-        need = _lib.lib().tq_kv8_decode_workspace_bytes(S, hq, hkv)
+        need = L.tq_kv8_decode_workspace_bytes(S, hq, hkv)
     else:
-        need = _lib.lib().tq_kv8_prefill_workspace_bytes(S, max_q_len, hq, hkv, block_tables.shape[1], k_fmt.block_size)
+        need = L.tq_kv8_prefill_workspace_bytes(S, max_q_len, hq, hkv, mb, k_fmt.block_size)
     if workspace is None:
         # (a buffer of this call: of the current stream, and of the graph under capture)
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
     elif workspace.get_device() != dev.index or workspace.numel() * workspace.element_size() < need or \
             workspace.data_ptr() % 256 or not workspace.is_contiguous():
         raise ValueError(f"workspace must be {need} contiguous bytes on {dev}, 256-byte aligned")
     qt, qh, _ = q.stride()
-    kb, kh, _ = k_cache.stride()
-    vb, vh, _ = v_cache.stride()
-    mb = block_tables.shape[1]
     args = _ATTN.pack(q.data_ptr(), target.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
-                      seq_lens.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(),
-                      0 if workspace is None else workspace.data_ptr(), need, qt, qh, ot, oh, kb, kh, vb, vh,
-                      k_cache.shape[0], block_tables.stride(0) if S > 1 else mb, _lib.dtype_code(q), _lib.dtype_code(target),
-                      _ENCODINGS[k_fmt.encoding], S, hq, hkv, 128, k_fmt.block_size, mb, max_seq_len, max_q_len, flags,
-                      scale, 0)
+                      seq_lens.data_ptr(), 0 if cu_seqlens_q is None else cu_seqlens_q.data_ptr(), workspace.data_ptr(), need,
+                      qt, qh, ot, oh, kb, kh, vb, vh, nb, block_tables.stride(0) if S > 1 else mb, _lib.dtype_code(q),
+                      _lib.dtype_code(target), k_fmt.encoding_code, S, hq, hkv, 128, k_fmt.block_size, mb, max_seq_len,
+                      max_q_len, flags, scale, 0)
     _lib.launch(name, dev, args)
     if target is not out:
         out.copy_(target)
@@ -237,13 +235,13 @@ def decode_paged8(
         raise ValueError("q must be [S, Hq, 128]")
     if seq_lens.dim() != 1 or seq_lens.shape[0] != q.shape[0]:
         raise ValueError("seq_lens must be [S]")
-    _check_pair(k_cache, k_fmt, v_cache, v_fmt, "decode_paged8")
-    if k_cache.shape[1] and q.shape[1] > 16 * k_cache.shape[1]:
+    caches = _check_pair(k_cache, k_fmt, v_cache, v_fmt, "decode_paged8")
+    if caches[1] and q.shape[1] > 16 * caches[1]:
         raise ValueError("decode_paged8 takes up to 16 query heads per KV head")
-    cap = min(block_tables.shape[-1] * k_fmt.block_size, 0x7fffff00)
+    cap = min(block_tables.shape[-1] * k_fmt.block_size, 0x7fffff00) if block_tables.dim() else 0
     msl = cap if max_seq_len is None else max(0, min(int(max_seq_len), cap))
-    return _attention("tq_kv8_decode", q, k_cache, k_fmt, v_cache, v_fmt, block_tables, seq_lens, None, sm_scale, msl, 1, 0,
-                      out, workspace, dev)
+    return _attention("tq_kv8_decode", dev, q, caches, k_cache, v_cache, k_fmt, block_tables, seq_lens, None, sm_scale, msl, 1,
+                      0, out, workspace)
 
 
 def prefill_paged8(
@@ -276,8 +274,8 @@ def prefill_paged8(
         raise ValueError("seq_lens must be [num_seqs] and cu_seqlens_q [num_seqs + 1]")
     if cu_seqlens_q.dtype != torch.int32:
         raise TypeError("cu_seqlens_q must be int32")
-    _check_pair(k_cache, k_fmt, v_cache, v_fmt, "prefill_paged8")
+    caches = _check_pair(k_cache, k_fmt, v_cache, v_fmt, "prefill_paged8")
     T = q.shape[0]
     mq = T if max_q_len is None else max(0, min(int(max_q_len), T))
-    return _attention("tq_kv8_prefill", q, k_cache, k_fmt, v_cache, v_fmt, block_tables, seq_lens, cu_seqlens_q.contiguous(),
-                      sm_scale, 0, mq, PREFILL_CAUSAL if causal else 0, out, workspace, dev)
+    return _attention("tq_kv8_prefill", dev, q, caches, k_cache, v_cache, k_fmt, block_tables, seq_lens,
+                      cu_seqlens_q.contiguous(), sm_scale, 0, mq, PREFILL_CAUSAL if causal else 0, out, workspace)

@@ -61,10 +61,8 @@ def plan_step(
     itself).  out: a StepPlan whose arrays are written instead of new ones; its seq_lens may be past_lens.
     """
     dev = _lib.require_gpu("plan_step", past_lens, new_lens, block_tables, ring, pool, pool_out)
-    for t, name in ((past_lens, "past_lens"), (new_lens, "new_lens"), (block_tables, "block_tables"), (ring, "ring"),
-                    (pool, "pool")):
-        if t.dtype != torch.int32:
-            raise TypeError(f"{name} must be int32")
+    if not (past_lens.dtype == new_lens.dtype == block_tables.dtype == ring.dtype == pool.dtype == torch.int32):
+        raise TypeError("past_lens, new_lens, block_tables, ring and pool must be int32")
     if past_lens.dim() != 1 or new_lens.shape != past_lens.shape:
         raise ValueError("past_lens and new_lens must be [S]")
     S = past_lens.shape[0]
@@ -73,30 +71,32 @@ def plan_step(
     if ring.dim() != 1 or not ring.numel() or not ring.is_contiguous():
         raise ValueError("ring must be [num_blocks], contiguous")
     pool_out = pool if pool_out is None else pool_out
-    for t in (pool, pool_out):
-        if t.shape != (2,) or t.dtype != torch.int32 or not t.is_contiguous():
-            raise ValueError("pool and pool_out must be int32 [2], contiguous")
+    if pool.shape != (2,) or pool_out.shape != (2,) or pool_out.dtype != torch.int32 or not pool.is_contiguous() or \
+            not pool_out.is_contiguous():
+        raise ValueError("pool and pool_out must be int32 [2], contiguous")
     num_tokens = int(num_tokens)
     if num_tokens < 0:
         raise ValueError("num_tokens must not be negative")
     past_lens, new_lens = past_lens.contiguous(), new_lens.contiguous()
+    L = _lib.lib()
+    need = L.tq_plan_step_workspace_bytes(S)
     if out is None:
-        out = StepPlan(torch.empty(S + 1, dtype=torch.int32, device=dev), torch.empty(S, dtype=torch.int32, device=dev),
-                       torch.empty(num_tokens, dtype=torch.int32, device=dev),
-                       torch.empty(num_tokens, dtype=torch.int64, device=dev), pool_out)
+        # one allocation for the workspace and the 32-bit arrays behind it
+        w = need // 4
+        buf = torch.empty(w + 2 * S + 1 + num_tokens, dtype=torch.int32, device=dev)
+        _, start, lens, positions = buf.split((w, S + 1, S, num_tokens))
+        out = StepPlan(start, lens, positions, torch.empty(num_tokens, dtype=torch.int64, device=dev), pool_out)
     else:
+        buf = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
         for t, shape, dt in ((out.query_start_loc, (S + 1,), torch.int32), (out.seq_lens, (S,), torch.int32),
                              (out.positions, (num_tokens,), torch.int32), (out.slot_mapping, (num_tokens,), torch.int64)):
             if t.shape != shape or t.dtype != dt or not t.is_contiguous() or t.device != dev:
                 raise ValueError("out does not match the step's sizes, types or device")
         out.pool = pool_out
-    L = _lib.lib()
-    need = L.tq_plan_step_workspace_bytes(S)
-    workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
     args = _PLAN.pack(past_lens.data_ptr(), new_lens.data_ptr(), block_tables.data_ptr(),
                       block_tables.stride(0) if S > 1 else block_tables.shape[1], ring.data_ptr(), pool.data_ptr(),
                       pool_out.data_ptr(), out.seq_lens.data_ptr(), out.query_start_loc.data_ptr(), out.positions.data_ptr(),
-                      out.slot_mapping.data_ptr(), workspace.data_ptr(), workspace.numel(), num_tokens, S,
-                      block_tables.shape[1], ring.shape[0], int(block_size))
+                      out.slot_mapping.data_ptr(), buf.data_ptr(), need, num_tokens, S, block_tables.shape[1], ring.shape[0],
+                      int(block_size))
     _lib.launch("tq_plan_step", dev, args)
     return out

@@ -63,6 +63,24 @@ _ROPE = struct.Struct("@4Q8q2Qq7if")
 _STYLES = {"half": 0, "interleaved": 1}
 
 
+def _rope_pair(x: torch.Tensor, out: Optional[torch.Tensor]):
+    """(source, what the kernel writes, the destination, their token and head strides)."""
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    elif out.shape != x.shape or out.dtype != x.dtype:
+        raise ValueError("destinations must have their input's shape and dtype")
+    xt, xh, x1 = x.stride()
+    ot, oh, o1 = out.stride()
+    dst = out
+    if o1 != 1 or (out.data_ptr() == x.data_ptr() and (ot != xt or oh != xh)):
+        dst = torch.empty_like(x, memory_format=torch.contiguous_format)
+        ot, oh, _ = dst.stride()
+    if x1 != 1:
+        x = x.contiguous()
+        xt, xh, _ = x.stride()
+    return x, dst, out, (xt, xh, ot, oh)
+
+
 def apply_rope(
     q: torch.Tensor,
     k: Optional[torch.Tensor],
@@ -102,32 +120,15 @@ def apply_rope(
         raise ValueError("k_out needs k")
     turns, positions = turns.contiguous(), positions.contiguous()
 
-    def pair(x, out):
-        """(source, destination, copy the destination back to): what the kernel reads and writes."""
-        if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        elif out.shape != x.shape or out.dtype != x.dtype:
-            raise ValueError("destinations must have their input's shape and dtype")
-        dst = out
-        if out.stride(2) != 1 or (out.data_ptr() == x.data_ptr() and out.stride() != x.stride()):
-            dst = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        if x.stride(2) != 1:
-            x = x.contiguous()
-        return x, dst, out
-
-    q, qd, q_out = pair(q, q_out)
-    kd, hk = None, 0
+    q, qd, q_out, qs = _rope_pair(q, q_out)
+    kd, kp, kdp, hk, ks = None, 0, 0, 0, (0, 0, 0, 0)
     if k is not None:
-        k, kd, k_out = pair(k, k_out)
-        hk = k.shape[1]
+        k, kd, k_out, ks = _rope_pair(k, k_out)
+        kp, kdp, hk = k.data_ptr(), kd.data_ptr(), k.shape[1]
     if T:
-        qt, qh, _ = q.stride()
-        qot, qoh, _ = qd.stride()
-        kt, kh, _ = k.stride() if hk else (0, 0, 1)
-        kot, koh, _ = kd.stride() if hk else (0, 0, 1)
-        args = _ROPE.pack(q.data_ptr(), k.data_ptr() if hk else 0, qd.data_ptr(), kd.data_ptr() if hk else 0, qt, qh, kt, kh,
-                          qot, qoh, kot, koh, positions.data_ptr(), turns.data_ptr(), T, _lib.dtype_code(q),
-                          _lib.dtype_code(positions), q.shape[1], hk, 128, 2 * turns.shape[0], _STYLES[style], float(magnitude))
+        args = _ROPE.pack(q.data_ptr(), kp, qd.data_ptr(), kdp, qs[0], qs[1], ks[0], ks[1], qs[2], qs[3], ks[2], ks[3],
+                          positions.data_ptr(), turns.data_ptr(), T, _lib.dtype_code(q), _lib.dtype_code(positions), q.shape[1],
+                          hk, 128, 2 * turns.shape[0], _STYLES[style], float(magnitude))
         _lib.launch("tq_rope", dev, args)
     if qd is not q_out:
         q_out.copy_(qd)
