@@ -491,9 +491,9 @@ int64_t tq_kv8_tile_bytes(int block_size);
  * rows hold is no longer meaningful: a block starts anew with its first row.  Otherwise the
  * scale never falls: where it grows from 2^e to 2^f the block's other rows are requantised in place,
  * code -> code * 2^(e - f) rounded to nearest even (exact for e4m3 codes that stay normal).
- * The tokens of one call that go to one block must be consecutive tokens with consecutive slots (as
- * a sequence's new tokens are); otherwise, and where a slot is named twice, that block's contents
- * are unspecified (no access leaves its tile).
+ * The tokens of one call that go to one block must follow each other with consecutive slots (as a
+ * sequence's new tokens do), up to 63 skipped tokens between two of them; otherwise, and where a slot
+ * is named twice, that block's contents are unspecified (no access leaves its tile).
  * Rows: element strides, rows of 128 contiguous elements, pointers 16-byte aligned and strides multiples
  * of 8 elements; caches 16-byte aligned with strides that are multiples of 16.  block_size: a positive
  * multiple of 16.

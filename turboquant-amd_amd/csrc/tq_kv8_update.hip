@@ -1,8 +1,8 @@
 // Quantisation of K and V rows into the 8-bit paged caches (tiles: tq_kv8.h).
 //
-// A run is a maximal stretch of consecutive tokens with consecutive slots inside one block; one wave
-// takes one run of one head of K or of V, so a block's scale, its requantisation and its rows have one
-// owner and need no atomics.  Pass 1 finds the largest finite |x| of the run, pass 2 writes the codes; where
+// A run is a maximal stretch of tokens with consecutive slots inside one block, skipped tokens between them (at most
+// 63 at a time) passed over; one wave takes one run of one head of K or of V, so a block's scale, its
+// requantisation and its rows have one owner and need no atomics.  Pass 1 finds the largest finite |x| of the run, pass 2 writes the codes; where
 // the run lies in one 16-row sub-tile the rows stay in registers between the two.  Lane (c, g), c = lane % 16,
 // g = lane / 16, holds dims 8c..8c+7 of rows 4g..4g+3 of a sub-tile: a wave's load is four whole rows, the
 // keys' store four whole rows, and the values' store (whose words are four rows of one dim) 2 KB in one
@@ -49,8 +49,28 @@ __device__ __forceinline__ Raw<DT> load_raw(const void* base, int64_t off) {
     return r;
 }
 
+// The next rows of a run from token `at` on: the tokens of up to 16 of them to s_tok, and the token behind the last.
+__device__ __forceinline__ int64_t next_tokens(const Kv8Update& p, int64_t at, int rows, int64_t slots, int* s_tok, int64_t t0) {
+    const int lane = threadIdx.x & 63;
+    for (int got = 0; got < rows;) {
+        const int64_t u = at + lane;
+        const int64_t s = u < p.a.num_tokens ? slot_at(p, u) : -1;
+        const bool valid = s >= 0 && s < slots;
+        const uint64_t mask = __builtin_amdgcn_ballot_w64(valid);
+        const int rank = got + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
+        if (valid && rank < rows) s_tok[rank] = (int)(u - t0);
+        const uint64_t last = __builtin_amdgcn_ballot_w64(valid && rank == rows - 1);
+        if (last) return at + __builtin_ctzll(last) + 1;
+        if (!mask) break;  // (a run's rows are there: not reached)
+        got += __builtin_popcountll(mask);
+        at += 64;
+    }
+    return at;
+}
+
+// gaps: tokens are skipped inside the run
 template <int ENC, int DT, bool VALUES>
-__device__ __forceinline__ void write_run(const Kv8Update& p, int64_t t0, int n, int64_t block, int row0, int head) {
+__device__ __forceinline__ void write_run(const Kv8Update& p, int64_t t0, int n, bool gaps, int* s_tok, int64_t block, int row0, int head) {
     using Code = Kv8Code<ENC>;
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const void* x = VALUES ? p.a.v : p.a.k;
@@ -66,12 +86,19 @@ __device__ __forceinline__ void write_run(const Kv8Update& p, int64_t t0, int n,
     const int64_t xbase = head * xsh + 8 * c;
 
     Raw<DT> raw[4];
+    int64_t at_token = t0;  // of the next sub-tile's first row
     auto load = [&](int sub) {
+        const int from = 16 * sub > row0 ? 16 * sub : row0, to = 16 * sub + 16 < end ? 16 * sub + 16 : end;
+        if (gaps) {
+            if (sub == sub0) at_token = t0;
+            at_token = next_tokens(p, at_token, to - from, p.a.num_blocks * p.a.block_size, s_tok, t0);
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int row = 16 * sub + 4 * g + r;
-            const bool in = row >= row0 && row < end;
-            raw[r] = load_raw<DT>(x, (t0 + (in ? row - row0 : 0)) * xst + xbase);
+            const bool in = row >= from && row < to;
+            const int64_t t = gaps ? t0 + s_tok[in ? row - from : 0] : t0 + (in ? row - row0 : 0);
+            raw[r] = load_raw<DT>(x, t * xst + xbase);
         }
     };
     uint32_t top = 0;
@@ -167,18 +194,30 @@ __device__ __forceinline__ void write_run(const Kv8Update& p, int64_t t0, int n,
 // the waves of the window's workgroups.
 template <int ENC, int DT>
 __global__ __launch_bounds__(64 * kWaves) void kv8_update_kernel(Kv8Update p) {
+    __shared__ int s_tok_all[kWaves][16];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int* s_tok = s_tok_all[wave];
     const int64_t t0 = (int64_t)(blockIdx.x / (uint32_t)p.window_wg) * p.window;
     const int part = (int)(blockIdx.x % (uint32_t)p.window_wg) * kWaves + wave;
     const int64_t slots = p.a.num_blocks * p.a.block_size;
-    // lane i: token t0 + i (window <= 64)
+    // lane i: token t0 + i (window <= 64), and token t0 - 64 + i for what lies before
     const int64_t t = t0 + lane;
     const bool in = lane < p.window && t < p.a.num_tokens;
     const int64_t slot = in ? slot_at(p, t) : -1;
-    const int64_t before = in && t > 0 ? slot_at(p, t - 1) : -1;
+    const int64_t early = t >= 64 ? slot_at(p, t - 64) : -1;
     const bool valid = slot >= 0 && slot < slots;
-    const bool starts = valid && !(before + 1 == slot && before >= 0 && slot % p.a.block_size != 0);
+    const uint64_t here = __builtin_amdgcn_ballot_w64(valid), there = __builtin_amdgcn_ballot_w64(early >= 0 && early < slots);
+    if (!here) return;
+    // the slot of the last token before this one that has one, of the 64 before it
+    int64_t before = -2;
+    {
+        const uint64_t below = here & ((1ull << lane) - 1), reach = there & ~((1ull << lane) - 1);
+        const int from = below ? 63 - __builtin_clzll(below) : reach ? 63 - __builtin_clzll(reach) : 0;
+        const int64_t a = __shfl(slot, from, 64), b = __shfl(early, from, 64);
+        before = below ? a : reach ? b : before;
+    }
+    const bool starts = valid && !(before + 1 == slot && slot % p.a.block_size != 0);
     uint64_t heads_of = __builtin_amdgcn_ballot_w64(starts);
     const int jobs = 2 * p.a.num_heads;
     int first = part;  // this wave's next job of the run at hand
@@ -190,24 +229,32 @@ __global__ __launch_bounds__(64 * kWaves) void kv8_update_kernel(Kv8Update p) {
                               (uint32_t)__builtin_amdgcn_readlane((int)slot, i);
             const int64_t block = s / p.a.block_size;
             const int row0 = (int)(s - block * p.a.block_size);
-            // the run's length: 64 tokens at a time
+            // the run's length: the 64 tokens behind its last one at a time
             const int most = p.a.block_size - row0;
             int n = 1;
-            for (;;) {
-                const int64_t u = t0 + i + n + lane;
-                const bool follows = n + lane < most && u < p.a.num_tokens && slot_at(p, u) == s + n + lane;
-                const uint64_t no = ~__builtin_amdgcn_ballot_w64(follows);
-                if (no) {
-                    n += __builtin_ctzll(no);
-                    break;
-                }
-                n += 64;
+            bool gaps = false;
+            for (int64_t a = t0 + i + 1; n < most;) {
+                const int64_t u = a + lane;
+                const int64_t su = u < p.a.num_tokens ? slot_at(p, u) : -1;
+                const bool vu = su >= 0 && su < slots;
+                const uint64_t mask = __builtin_amdgcn_ballot_w64(vu);
+                if (!mask) break;
+                const int rank = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
+                const uint64_t off = __builtin_amdgcn_ballot_w64(vu && (n + rank >= most || su != s + n + rank));
+                // the tokens that follow: those with a slot before the first that does not
+                const uint64_t follow = off ? mask & ((off & -off) - 1) : mask;
+                if (!follow) break;
+                const int last = 63 - __builtin_clzll(follow);
+                gaps = gaps || follow != (last == 63 ? ~0ull : (1ull << (last + 1)) - 1);
+                n += __builtin_popcountll(follow);
+                if (off) break;
+                a += last + 1;
             }
             for (; first < jobs; first += kWaves * p.window_wg) {
                 if (first < p.a.num_heads)
-                    write_run<ENC, DT, false>(p, t0 + i, n, block, row0, first);
+                    write_run<ENC, DT, false>(p, t0 + i, n, gaps, s_tok, block, row0, first);
                 else
-                    write_run<ENC, DT, true>(p, t0 + i, n, block, row0, first - p.a.num_heads);
+                    write_run<ENC, DT, true>(p, t0 + i, n, gaps, s_tok, block, row0, first - p.a.num_heads);
             }
         }
         first -= jobs;

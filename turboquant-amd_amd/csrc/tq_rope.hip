@@ -28,8 +28,9 @@ __device__ __forceinline__ double position(const Rope& p, int64_t t) {
 }
 // magnitude * (cos, sin) of pair i at position pos
 __device__ __forceinline__ float2 factors(const Rope& p, double pos, int i) {
-    const double turns = pos * p.a.turns[i];
-    const float r = (float)(turns - __builtin_rint(turns));  // [-1/2, 1/2]
+    // (the fused step rounds once, after the whole part is gone, so far positions lose nothing)
+    const double t = p.a.turns[i];
+    const float r = (float)__builtin_fma(pos, t, -__builtin_rint(pos * t));  // [-1/2, 1/2]
     float s, c;
     sincospif(2.0f * r, &s, &c);
     return make_float2(c * p.a.magnitude, s * p.a.magnitude);

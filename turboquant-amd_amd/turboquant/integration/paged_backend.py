@@ -14,7 +14,9 @@ the hot path is here, in the shapes the reference's backends use:
   TurboQuantFP8Config / get_tq_fp8_config (integration/vllm_backend.py:237-337): the first and
   last `num_protected_layers` layers are not compressed (get_state returns None and the caller
   keeps its own attention for them, as the reference does), or, with `protected_bits`, get a
-  4-bit (or other) packed format of their own.
+  4-bit (or other) packed format of their own, or with protected_bits=8 a cache of 8 bits a value.
+- TurboQuantPaged8State: the state of such a layer (kernels.paged8), with the same methods, so that
+  TurboQuantPagedImpl runs on either.
 - TurboQuantPagedImpl: an attention implementation in vLLM's shape
   (TurboQuantFP4Impl.do_kv_cache_update / forward and TurboQuantFP4Backend.get_kv_cache_shape,
   integration/tq_fp4_backend.py:389-735).  One uint8 tensor [num_blocks, num_kv_heads,
@@ -34,6 +36,8 @@ import torch
 
 from turboquant.core import make_codebook, make_wht_matrix
 from turboquant.kernels.paged import PagedKVFormat, compress_paged, compress_paged_kv, decode_paged, prefill_paged
+from turboquant.kernels.paged8 import Paged8Format, decode_paged8, prefill_paged8, quantize_paged8_kv
+from turboquant.kernels.plan import StepPlan
 from turboquant.kernels.rotation import wht_rows
 
 
@@ -139,19 +143,78 @@ class TurboQuantPagedState:
                              rotate=not self.weights_fused, max_q_len=max_q_len, out=out)
 
 
+class TurboQuantPaged8State:
+    """Per-layer state of a cache of 8 bits a value: formats, cache writes, decode and prefill.
+
+    encoding: "e4m3" or "int8".  There is no rotation: rows and queries are taken in the basis they come in.
+    """
+
+    def __init__(self, head_size: int = 128, layer_idx: int = 0, device=None, encoding: str = "e4m3", block_size: int = 16):
+        if head_size != 128:
+            raise ValueError("the paged kernels take head_size 128")
+        self.head_size = head_size
+        self.layer_idx = layer_idx
+        self.device = torch.device(device) if device is not None else None
+        self.block_size = block_size
+        self.k_format = Paged8Format.for_keys(encoding, block_size)
+        self.v_format = Paged8Format.for_values(encoding, block_size)
+
+    @property
+    def tile_bytes(self) -> int:
+        """Bytes per (block, KV head) of the combined cache: K tile then V tile."""
+        return self.k_format.tile_bytes + self.v_format.tile_bytes
+
+    def kv_cache_shape(self, num_blocks: int, num_kv_heads: int) -> tuple[int, int, int]:
+        return (num_blocks, num_kv_heads, self.tile_bytes)
+
+    def allocate_kv_cache(self, num_blocks: int, num_kv_heads: int, device=None) -> torch.Tensor:
+        dev = device if device is not None else self.device
+        return torch.zeros(self.kv_cache_shape(num_blocks, num_kv_heads), dtype=torch.uint8, device=dev)
+
+    def split_kv_cache(self, kv_cache: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """(K cache, V cache) views of a combined cache."""
+        if kv_cache.dtype != torch.uint8 or kv_cache.dim() != 3 or kv_cache.shape[2] != self.tile_bytes:
+            raise ValueError(f"kv_cache must be uint8 [num_blocks, num_kv_heads, {self.tile_bytes}]")
+        kt = self.k_format.tile_bytes
+        return kv_cache[:, :, :kt], kv_cache[:, :, kt:]
+
+    def compress_kv_and_scatter(self, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                                v_cache: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+        """The layer's K + V cache update in one launch."""
+        quantize_paged8_kv(k, v, slot_mapping, k_cache, v_cache, self.k_format, self.v_format)
+
+    def decode(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+               seq_lens: torch.Tensor, sm_scale: Optional[float] = None, sparse_threshold: float = 0.0,
+               max_seq_len: Optional[int] = None, seq_lens_host: Optional[Sequence[int]] = None,
+               out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Decode attention of q [S, Hq, 128].  sparse_threshold and seq_lens_host are taken for the packed state's
+        sake: every token's values are read, and the split over the keys is planned on the device."""
+        return decode_paged8(q, k_cache, self.k_format, v_cache, self.v_format, block_tables, seq_lens, sm_scale=sm_scale,
+                             max_seq_len=max_seq_len, out=out, workspace=workspace)
+
+    def prefill(self, q: torch.Tensor, cu_seqlens_q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                block_tables: torch.Tensor, seq_lens: torch.Tensor, sm_scale: Optional[float] = None,
+                max_q_len: Optional[int] = None, out: Optional[torch.Tensor] = None,
+                causal: bool = True) -> torch.Tensor:
+        """Prefill / extend attention of q [T, Hq, 128] (new tokens of each sequence, already in the cache)."""
+        return prefill_paged8(q, cu_seqlens_q, k_cache, self.k_format, v_cache, self.v_format, block_tables, seq_lens,
+                              sm_scale=sm_scale, causal=causal, max_q_len=max_q_len, out=out)
+
+
 class TurboQuantPagedConfig:
     """Which layers are compressed, and with which formats.
 
     protect_boundary_layers / num_protected_layers: the first and last N layers are not
     compressed with the configured formats (integration/vllm_backend.py:266-278).  Their
     get_state is None (the caller's own attention, as in the reference) unless
-    protected_bits is given: then they get k_bits = v_bits = protected_bits without QJL.
+    protected_bits is given: then they get k_bits = v_bits = protected_bits without QJL, and with
+    protected_bits=8 a TurboQuantPaged8State of protected_encoding ("e4m3" or "int8").
     """
 
     def __init__(self, head_size: int = 128, num_layers: int = 0, protect_boundary_layers: bool = True,
                  num_protected_layers: int = 2, k_bits: int = 4, v_bits: Optional[int] = None,
                  k_qjl: bool = False, block_size: int = 16, weights_fused: bool = False,
-                 protected_bits: Optional[int] = None):
+                 protected_bits: Optional[int] = None, protected_encoding: str = "e4m3"):
         self.head_size = head_size
         self.num_layers = num_layers
         self.protect_boundary_layers = protect_boundary_layers
@@ -162,7 +225,8 @@ class TurboQuantPagedConfig:
         self.block_size = block_size
         self.weights_fused = weights_fused
         self.protected_bits = protected_bits
-        self.layer_states: dict[int, TurboQuantPagedState] = {}
+        self.protected_encoding = protected_encoding
+        self.layer_states: dict[int, TurboQuantPagedState | TurboQuantPaged8State] = {}
 
     def should_compress(self, layer_idx: int) -> bool:
         if not self.protect_boundary_layers or self.num_layers == 0:
@@ -173,10 +237,15 @@ class TurboQuantPagedConfig:
             return False
         return True
 
-    def get_state(self, layer_idx: int, device=None) -> Optional[TurboQuantPagedState]:
+    def get_state(self, layer_idx: int, device=None) -> Optional[TurboQuantPagedState | TurboQuantPaged8State]:
         protected = not self.should_compress(layer_idx)
         if protected and self.protected_bits is None:
             return None
+        if protected and self.protected_bits == 8:
+            if layer_idx not in self.layer_states:
+                self.layer_states[layer_idx] = TurboQuantPaged8State(self.head_size, layer_idx, device,
+                                                                     self.protected_encoding, self.block_size)
+            return self.layer_states[layer_idx]
         if layer_idx not in self.layer_states:
             if protected:
                 kb, vb, kq = self.protected_bits, self.protected_bits, False
@@ -194,7 +263,8 @@ _tq_paged_config: Optional[TurboQuantPagedConfig] = None
 def get_tq_paged_config(head_size: int = 128, num_layers: int = 0, protect_boundary_layers: bool = True,
                         num_protected_layers: int = 2, k_bits: int = 4, v_bits: Optional[int] = None,
                         k_qjl: bool = False, block_size: int = 16, weights_fused: bool = False,
-                        protected_bits: Optional[int] = None) -> TurboQuantPagedConfig:
+                        protected_bits: Optional[int] = None,
+                        protected_encoding: str = "e4m3") -> TurboQuantPagedConfig:
     """The process-wide config, created by the first call (later arguments are ignored, as in
     get_tq_fp8_config, integration/vllm_backend.py:295-337)."""
     global _tq_paged_config
@@ -202,7 +272,8 @@ def get_tq_paged_config(head_size: int = 128, num_layers: int = 0, protect_bound
         _tq_paged_config = TurboQuantPagedConfig(
             head_size=head_size, num_layers=num_layers, protect_boundary_layers=protect_boundary_layers,
             num_protected_layers=num_protected_layers, k_bits=k_bits, v_bits=v_bits, k_qjl=k_qjl,
-            block_size=block_size, weights_fused=weights_fused, protected_bits=protected_bits)
+            block_size=block_size, weights_fused=weights_fused, protected_bits=protected_bits,
+            protected_encoding=protected_encoding)
     return _tq_paged_config
 
 
@@ -229,14 +300,23 @@ class PagedDecodeMetadata:
     num_decodes: Optional[int] = None            # default: all sequences when query_start_loc is None
     max_query_len: Optional[int] = None          # host-side bound of the prefill query counts
 
+    @classmethod
+    def from_plan(cls, plan: StepPlan, block_tables: torch.Tensor, max_seq_len: int, num_decodes: Optional[int] = None,
+                  max_query_len: Optional[int] = None) -> "PagedDecodeMetadata":
+        """The metadata of a step planned by kernels.plan.plan_step over the same block_tables.  num_decodes
+        None: every request gets one new token; otherwise the first num_decodes do."""
+        return cls(block_tables, plan.seq_lens, max_seq_len,
+                   query_start_loc=None if num_decodes is None else plan.query_start_loc, num_decodes=num_decodes,
+                   max_query_len=max_query_len)
+
 
 class TurboQuantPagedImpl:
-    """Decode attention over the packed paged cache, in the shape of a vLLM AttentionImpl."""
+    """Attention over a packed or 8-bit paged cache, in the shape of a vLLM AttentionImpl."""
 
     forward_includes_kv_cache_update = False  # do_kv_cache_update is called separately
 
     def __init__(self, num_heads: int, head_size: int, scale: float, num_kv_heads: int,
-                 state: TurboQuantPagedState, sparse_threshold: float = 0.0):
+                 state: TurboQuantPagedState | TurboQuantPaged8State, sparse_threshold: float = 0.0):
         if num_heads % num_kv_heads:
             raise ValueError("num_heads must be a multiple of num_kv_heads")
         if head_size != state.head_size:
@@ -264,6 +344,10 @@ class TurboQuantPagedImpl:
             raise ValueError("Block size must be a multiple of 16.")
         if head_size != 128:
             raise ValueError("head_size must be 128")
+        if k_bits == 8:
+            if v_bits not in (None, 8) or k_qjl:
+                raise ValueError("an 8-bit cache has 8 bits on both sides and no QJL data")
+            return (num_blocks, num_kv_heads, 2 * Paged8Format(block_size=block_size).tile_bytes)
         kf = PagedKVFormat(bits=k_bits, qjl=k_qjl, block_size=block_size)
         vf = PagedKVFormat(bits=v_bits if v_bits is not None else k_bits, qjl=False, block_size=block_size,
                            layout="values")

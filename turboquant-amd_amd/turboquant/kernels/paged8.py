@@ -126,8 +126,9 @@ def quantize_paged8_kv(
     Negative slots, and slots behind the cache, are skipped.  A block that is written from its first row on
     starts anew: its scale is that of the new rows alone and its other rows hold nothing.
     Otherwise a block's scale only grows, and its other rows are requantised when it does.  The tokens of one
-    call that go to one block must be consecutive tokens with consecutive slots, as a sequence's
-    new tokens are; a block for which that does not hold, or a slot named twice, has unspecified contents afterwards.
+    call that go to one block must follow each other with consecutive slots, as a sequence's new tokens do (up
+    to 63 skipped tokens between two of them); a block for which that does not hold, or a slot named
+    twice, has unspecified contents afterwards.
     """
     dev = _lib.require_gpu("quantize_paged8_kv", k, v, slot_mapping, k_cache, v_cache)
     if k.dim() != 3 or k.shape[2] != 128 or v.shape != k.shape:
