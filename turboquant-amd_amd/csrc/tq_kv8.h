@@ -80,6 +80,7 @@ struct Kv8Attn {
     int workers;          // at most
     float* ws_acc;        // [slot][row][128]
     float* ws_ml;         // [slot][row][2]: exponent base (log2), sum
+    int* ends;            // decode: [segment][2], the waves with its first and its last step
 };
 
 // The factor +-2^k that brings a query row with the largest |x| m to [1, 4), and 2^-k.  Rows that are all zero or

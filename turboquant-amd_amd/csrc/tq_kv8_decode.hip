@@ -5,7 +5,7 @@
 // floor((w + 1) P / R)): found on the device from seq_lens, so no length is needed on the host.  A
 // segment inside one wave is written directly; the pieces of a cut one go to workspace slot w + (segment
 // number), which never repeats since along the waves the segments never decrease, and
-// kv8_decode_merge_kernel joins them.  Each wave works alone: no LDS, no barriers.
+// kv8_decode_merge_kernel joins them: the waves with a segment's first and last step leave their numbers.  Each wave works alone: no LDS, no barriers.
 //
 // MFMA layout, lane l, n = l % 16, g = l / 16, tiles A and B of 16 tokens per step:
 //   S^T [16 tokens x 16 heads] = K . Q^T   4 x mfma_f32_16x16x32_f16 per tile; slice cc covers dims 32g + 8cc + (0..7),
@@ -40,9 +40,24 @@ __device__ __forceinline__ int64_t total_steps(const Kv8Attn& p) {
     for (int m = 32; m >= 1; m >>= 1) t += __shfl_xor(t, m, 64);
     return t;
 }
-__device__ __forceinline__ int64_t workers_of(const Kv8Attn& p, int64_t P) {
+// floor(w P / R) = w floor(P / R) + floor(w (P mod R) / R), R waves in use
+struct Share {
+    int64_t each;
+    uint32_t rest, R;
+    __device__ __forceinline__ int64_t at(uint32_t w) const { return w * each + w * rest / R; }  // (w, R below 2^12)
+};
+__device__ __forceinline__ Share share_of(const Kv8Attn& p, int64_t P) {
     const int64_t m = P / kMinSteps;
-    return m < 1 ? 1 : m < p.workers ? m : p.workers;
+    Share h;
+    h.R = m < 1 ? 1u : m < p.workers ? (uint32_t)m : (uint32_t)p.workers;
+    if (P >> 32) {
+        h.each = P / h.R;
+        h.rest = (uint32_t)(P - h.each * h.R);
+    } else {
+        h.each = (uint32_t)P / h.R;
+        h.rest = (uint32_t)P - (uint32_t)h.each * h.R;
+    }
+    return h;
 }
 
 template <int ENC, bool FINE>
@@ -53,10 +68,10 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
     const int64_t w = (int64_t)blockIdx.x * kWaves + wave;
     const int hkv = p.a.num_kv_heads;
     const int64_t P = total_steps(p) * hkv;
-    const int64_t R = workers_of(p, P);
-    if (P == 0 || w >= R) return;
-    int64_t pos = w * P / R;
-    const int64_t end = (w + 1) * P / R;
+    const Share share = share_of(p, P);
+    if (P == 0 || w >= share.R) return;
+    int64_t pos = share.at((uint32_t)w);
+    const int64_t end = share.at((uint32_t)w + 1);
 
     // ---- the sequence that holds step pos ----
     int s = 0;
@@ -254,9 +269,14 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
 
         // ---- acc[a][r] is dim 32g + 8r + a of head n ----
         const float l = tq_sum_over_groups(lsum);
+        const bool complete = j0 == 0 && j1 == np;
+        if (lane == 0) {
+            int* ends = p.ends + 2 * ((int64_t)s * hkv + kh);
+            if (j0 == 0) ends[0] = (int)w;
+            if (j1 == np) ends[1] = (int)w;
+        }
         if (n < p.group) {
             float o[32];
-            const bool complete = j0 == 0 && j1 == np;
             const float f = complete ? (l == 0.f ? 0.f : vref / l) : vref;
 #pragma unroll
             for (int a = 0; a < 8; ++a)
@@ -293,49 +313,28 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
 // to do where one wave held it all, zeros where the sequence is empty.  The workgroup's 8 half-waves share the
 // pieces, a lane has 4 dims.  (With a workgroup per KV head, one sequence of 4099 tokens: merge 13.6 -> 6.6 us.)
 __global__ __launch_bounds__(256) void kv8_decode_merge_kernel(Kv8Attn p) {
-    __shared__ int64_t s_sum[2][4];
     __shared__ float4 s_acc[8][32];
     __shared__ float2 s_ml[8];
     const int hkv = p.a.num_kv_heads;
     const int s = (int)(blockIdx.x / (uint32_t)p.a.num_q_heads), head = (int)(blockIdx.x % (uint32_t)p.a.num_q_heads);
     const int kh = head / p.group, r = head - kh * p.group;
-    int64_t before = 0, all = 0;
-    for (int i = threadIdx.x; i < p.a.num_seqs; i += 256) {
-        const int u = steps_of(p, i);
-        all += u;
-        if (i < s) before += u;
+    const int* ends = p.ends + 2 * ((int64_t)s * hkv + kh);
+    int w0 = ends[0], w1 = ends[1];
+    if (steps_of(p, s) == 0) {  // (no wave had it)
+        w0 = 0;
+        w1 = -1;
     }
-    for (int m = 32; m >= 1; m >>= 1) {
-        before += __shfl_xor(before, m, 64);
-        all += __shfl_xor(all, m, 64);
-    }
-    if ((threadIdx.x & 63) == 0) {
-        s_sum[0][threadIdx.x >> 6] = before;
-        s_sum[1][threadIdx.x >> 6] = all;
-    }
-    __syncthreads();
-    before = s_sum[0][0] + s_sum[0][1] + s_sum[0][2] + s_sum[0][3];
-    const int64_t P = (s_sum[1][0] + s_sum[1][1] + s_sum[1][2] + s_sum[1][3]) * hkv;
-    const int np = steps_of(p, s);
-    int64_t w0 = 0, w1 = -1;
-    if (np > 0) {
-        const int64_t R = workers_of(p, P);
-        const int64_t a = before * hkv + (int64_t)kh * np;
-        // the wave of step x: the largest w with floor(w P / R) <= x
-        w0 = ((a + 1) * R - 1) / P;
-        w1 = ((a + np) * R - 1) / P;
-        if (w0 == w1) return;
-    }
+    if (w0 == w1) return;
     const int half = threadIdx.x >> 5, l32 = threadIdx.x & 31;
     const int64_t seg = (int64_t)s * hkv + kh;
     float M = kKv8NegInf, l = 0.f;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int64_t wb = w0 + half; wb <= w1; wb += 4 * 8) {
+    for (int wb = w0 + half; wb <= w1; wb += 4 * 8) {
         float mp[4], lp[4];
         float4 v[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int64_t wk = wb + k * 8;
+            const int wk = wb + k * 8;
             mp[k] = kKv8NegInf;
             lp[k] = 0.f;
             v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -432,7 +431,7 @@ int tq_kv8_attn_setup(const tq_kv8_attn_args* a, Kv8Attn* p) {
 extern "C" int64_t tq_kv8_decode_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads) {
     if (num_seqs < 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads) return 0;
     const int64_t slots = kMaxWorkers + (int64_t)num_seqs * num_kv_heads;
-    return slots * (num_q_heads / num_kv_heads) * (TQ_HEAD_DIM + 2) * 4;
+    return slots * (num_q_heads / num_kv_heads) * (TQ_HEAD_DIM + 2) * 4 + (int64_t)num_seqs * num_kv_heads * 8;
 }
 
 extern "C" int tq_kv8_decode(const tq_kv8_attn_args* a, tq_stream_t stream) {
@@ -452,6 +451,7 @@ extern "C" int tq_kv8_decode(const tq_kv8_attn_args* a, tq_stream_t stream) {
     const int64_t slots = kMaxWorkers + (int64_t)a->num_seqs * a->num_kv_heads;
     p.ws_acc = static_cast<float*>(a->workspace);
     p.ws_ml = p.ws_acc + slots * p.group * TQ_HEAD_DIM;
+    p.ends = reinterpret_cast<int*>(p.ws_ml + slots * p.group * 2);
     // no more waves than the lengths can ask for
     const int64_t most = (int64_t)a->num_seqs * a->num_kv_heads * ((p.cap + 31) / 32) / kMinSteps;
     int64_t workers = (int64_t)cus * kWavesPerCu;
