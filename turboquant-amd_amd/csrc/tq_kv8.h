@@ -104,23 +104,22 @@ __device__ __forceinline__ void kv8_query_half(const float (&x)[32], float f, tq
     }
 }
 
-// 32 elements from element off on (16-byte aligned)
-__device__ __forceinline__ void kv8_load32(const void* base, int64_t off, int dt, float (&x)[32]) {
+// 16 elements from element off on and 16 from off + second on (16-byte aligned)
+__device__ __forceinline__ void kv8_load32(const void* base, int64_t off, int second, int dt, float (&x)[32]) {
     if (dt == TQ_F32) {
-        const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(base) + off);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float4 v = s[i];
+            const float4 v = reinterpret_cast<const float4*>(static_cast<const float*>(base) + off + (i < 4 ? 0 : second - 16))[i];
             x[4 * i] = v.x;
             x[4 * i + 1] = v.y;
             x[4 * i + 2] = v.z;
             x[4 * i + 3] = v.w;
         }
     } else {
-        const tq_u32x4* s = reinterpret_cast<const tq_u32x4*>(static_cast<const uint16_t*>(base) + off);
         tq_u32x4 raw[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) raw[i] = s[i];
+        for (int i = 0; i < 4; ++i)
+            raw[i] = reinterpret_cast<const tq_u32x4*>(static_cast<const uint16_t*>(base) + off + (i < 2 ? 0 : second - 16))[i];
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
             const uint32_t b = (raw[i >> 3][(i >> 1) & 3] >> (16 * (i & 1))) & 0xffffu;

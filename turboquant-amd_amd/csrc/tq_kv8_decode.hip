@@ -16,7 +16,9 @@
 // factor; V's scale, relative to the largest met so far, into the conversion to fp16, which is
 // exact (and the accumulators are rescaled when a larger one is met).
 //
-// Bound: HBM reads, 256 bytes per token and KV head.
+// Bound: HBM reads, 256 bytes per token and KV head: 64 x 32768 tokens of 8 heads in 759 us, 5.7 TB/s, where a plain
+// read of 2 GiB reaches 5.8.  Small calls: launches, start-up (the search for the wave's part, block table, scales) and
+// the merge, about 15 us.
 #include "tq_kv8.h"
 
 #include <atomic>
@@ -24,21 +26,28 @@
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kWavesPerCu = 12;  // resident: 3 per SIMD at up to 168 registers
+// 16-token tiles of a step (4: one sequence of 4099 tokens 15.9 -> 14.9 us, 32 x 1K..8K 70.9 -> 75.2)
+constexpr int kTiles = 2;
+// Resident waves (12: 64 x 32768 tokens 759 -> 776 us, 32 x 1K..8K 70.9 -> 76.0; 6: 852 and 75)
+constexpr int kWavesPerCu = 8;
 constexpr int kMaxWorkers = 256 * kWavesPerCu;
 constexpr int kMinSteps = 2;     // steps a wave takes at least (1 x 4099 tokens: 1 18.2 us, 2 16.9, 4 16.9, 8 18.9)
 
 __device__ __forceinline__ int steps_of(const Kv8Attn& p, int s) {
     int L = p.a.seq_lens[s];
     L = L < p.cap ? L : p.cap;
-    return L > 0 ? (L + 31) >> 5 : 0;
+    return (int)(((uint32_t)(L > 0 ? L : 0) + 16 * kTiles - 1) / (16 * kTiles));
 }
-// steps of all sequences (one KV head), every lane
-__device__ __forceinline__ int64_t total_steps(const Kv8Attn& p) {
-    int64_t t = 0;
-    for (int s = threadIdx.x & 63; s < p.a.num_seqs; s += 64) t += steps_of(p, s);
-    for (int m = 32; m >= 1; m >>= 1) t += __shfl_xor(t, m, 64);
-    return t;
+// Steps (one KV head) of the 64 sequences from s0 on: this lane's, and the sum up to it (below 2^32: 64 times 2^26)
+__device__ __forceinline__ uint32_t scan_steps(const Kv8Attn& p, int s0, uint32_t& mine) {
+    const int lane = threadIdx.x & 63;
+    mine = s0 + lane < p.a.num_seqs ? (uint32_t)steps_of(p, s0 + lane) : 0u;
+    uint32_t in = mine;
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t x = (uint32_t)__shfl_up((int)in, d, 64);
+        if (lane >= d) in += x;
+    }
+    return in;
 }
 // floor(w P / R) = w floor(P / R) + floor(w (P mod R) / R), R waves in use
 struct Share {
@@ -61,13 +70,20 @@ __device__ __forceinline__ Share share_of(const Kv8Attn& p, int64_t P) {
 }
 
 template <int ENC, bool FINE>
-__global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
+__global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kernel(Kv8Attn p) {
     using Code = Kv8Code<ENC>;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t w = (int64_t)blockIdx.x * kWaves + wave;
     const int hkv = p.a.num_kv_heads;
-    const int64_t P = total_steps(p) * hkv;
+    uint32_t mine;
+    uint32_t in = scan_steps(p, 0, mine);
+    int64_t P = (uint32_t)__builtin_amdgcn_readlane((int)in, 63);
+    if (p.a.num_seqs > 64) {
+        uint32_t u;
+        for (int s0 = 64; s0 < p.a.num_seqs; s0 += 64) P += (uint32_t)__builtin_amdgcn_readlane((int)scan_steps(p, s0, u), 63);
+    }
+    P *= hkv;
     const Share share = share_of(p, P);
     if (P == 0 || w >= share.R) return;
     int64_t pos = share.at((uint32_t)w);
@@ -76,22 +92,17 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
     // ---- the sequence that holds step pos ----
     int s = 0;
     int64_t seq0 = 0;  // its first step
-    for (int s0 = 0; s0 < p.a.num_seqs; s0 += 64) {
-        const int64_t u = s0 + lane < p.a.num_seqs ? (int64_t)steps_of(p, s0 + lane) * hkv : 0;
-        int64_t in = u;
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t x = __shfl_up(in, d, 64);
-            if (lane >= d) in += x;
-        }
-        in += seq0;
-        const uint64_t over = __builtin_amdgcn_ballot_w64(in > pos);
+    for (int s0 = 0;;) {
+        const uint64_t over = __builtin_amdgcn_ballot_w64((int64_t)in * hkv + seq0 > pos);
         if (over) {
             const int l = __builtin_ctzll(over);
             s = s0 + l;
-            seq0 = __shfl(in - u, l, 64);
+            seq0 += (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)(in - mine), l) * hkv;
             break;
         }
-        seq0 = __shfl(in, 63, 64);
+        seq0 += (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)in, 63) * hkv;
+        s0 += 64;  // (pos is below the last one's end)
+        in = scan_steps(p, s0, mine);
     }
     s = __builtin_amdgcn_readfirstlane(s);
     int np = steps_of(p, s);
@@ -130,15 +141,15 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
             t.vs = *reinterpret_cast<const float*>(vb + t.blk * p.a.v_stride_block + scale_at);
             return t;
         };
-        Tiles nxt = tiles_from(2 * j0);
+        Tiles nxt = tiles_from(kTiles * j0);
 
         // ---- the query: heads kh * group + n ----
         tq_half8 qh[4], ql[4];
         float c1;
         {
             float x[32];
-            const int64_t off = s * p.a.q_stride_token + (int64_t)(kh * p.group + (n < p.group ? n : 0)) * p.a.q_stride_head + 32 * g;
-            kv8_load32(p.a.q, off, p.a.q_dtype, x);
+            const int64_t off = s * p.a.q_stride_token + (int64_t)(kh * p.group + (n < p.group ? n : 0)) * p.a.q_stride_head + 16 * g;
+            kv8_load32(p.a.q, off, 64, p.a.q_dtype, x);
             float m = 0.f, back;
 #pragma unroll
             for (int i = 0; i < 32; ++i) m = fmaxf(m, __builtin_fabsf(x[i]));
@@ -147,10 +158,11 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
             c1 = __builtin_fabsf(p.a.sm_scale) * kKv8Log2e * back;
         }
 
-        uint32_t kw[2][8], vw[2][8];
-        auto load = [&](const uint8_t* tile, uint32_t at, uint32_t (&x)[8]) {
+        uint32_t kw[kTiles][8], vw[kTiles][8];
+        auto load = [&](const uint8_t* tile, uint32_t at, int second, uint32_t (&x)[8]) {
             const tq_u32x4* src = reinterpret_cast<const tq_u32x4*>(tile + at);
-            const tq_u32x4 a = src[0], b = src[1];
+            // (each byte is read once: kept out of the caches' way, 64 x 32768 tokens 792 -> 759 us)
+            const tq_u32x4 a = __builtin_nontemporal_load(src), b = __builtin_nontemporal_load(src + second);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 x[i] = a[i];
@@ -162,21 +174,27 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
             const int tc = ti < last_tile ? ti : last_tile;
             return blk * stride + (int64_t)(tc - p.tpb * (int)tq_udiv_apply((uint32_t)tc, p.tpb_div)) * (16 * TQ_HEAD_DIM);
         };
-        const uint32_t k_off = 128 * n + 32 * g, v_off = 512 * g + 32 * n;
-        auto load_keys = [&](int b0, int b1, int ti) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) load(kb + tile_at(ti + h, h ? b1 : b0, p.a.k_stride_block), k_off, kw[h]);
+        // (each load's lanes next to each other: a token's 64 bytes of keys, 256 bytes of values)
+        const uint32_t k_off = 128 * n + 16 * g, v_off = 512 * g + 16 * n;
+        struct Blocks {
+            int b[kTiles];
         };
-        auto load_values = [&](int b0, int b1, int ti) {
+        auto load_keys = [&](const Blocks& b, int ti) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) load(vb + tile_at(ti + h, h ? b1 : b0, p.a.v_stride_block), v_off, vw[h]);
+            for (int h = 0; h < kTiles; ++h) load(kb + tile_at(ti + h, b.b[h], p.a.k_stride_block), k_off, 4, kw[h]);
+        };
+        auto load_values = [&](const Blocks& b, int ti) {
+#pragma unroll
+            for (int h = 0; h < kTiles; ++h) load(vb + tile_at(ti + h, b.b[h], p.a.v_stride_block), v_off, 16, vw[h]);
         };
         // (the loads of step j + 1 go out during step j without a condition, the last step repeats its own: where the
         // compiler cannot count what is under way, it waits for all of it)
         {
-            const int b0 = __builtin_amdgcn_readlane(nxt.blk, 0), b1 = __builtin_amdgcn_readlane(nxt.blk, 1);
-            load_keys(b0, b1, 2 * j0);
-            load_values(b0, b1, 2 * j0);
+            Blocks b;
+#pragma unroll
+            for (int h = 0; h < kTiles; ++h) b.b[h] = __builtin_amdgcn_readlane(nxt.blk, h);
+            load_keys(b, kTiles * j0);
+            load_values(b, kTiles * j0);
         }
 
         float M = kKv8None, lsum = 0.f, vref = 0.f;
@@ -184,30 +202,31 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
 #pragma unroll
         for (int a = 0; a < 8; ++a) acc[a] = tq_floatx4{0.f, 0.f, 0.f, 0.f};
 
-        for (int jg = j0; jg < j1; jg += 32) {  // 32 steps: 64 tiles
-        const int t0 = 2 * jg, je = jg + 32 < j1 ? jg + 32 : j1;
+        for (int jg = j0; jg < j1; jg += 64 / kTiles) {
+        const int t0 = kTiles * jg, je = jg + 64 / kTiles < j1 ? jg + 64 / kTiles : j1;
         const Tiles cur = nxt;
-        if (t0 + 64 < 2 * j1) nxt = tiles_from(t0 + 64);
+        if (t0 + 64 < kTiles * j1) nxt = tiles_from(t0 + 64);
         for (int j = jg; j < je; ++j) {
-            const int i = 2 * j - t0;  // lane of tile A in cur
+            const int i = kTiles * j - t0;  // lane of the step's first tile in cur
             const bool more = j + 1 < j1;
             // the next step's tiles
-            const int jn = more ? j + 1 : j, fi = (more ? i + 2 : i) & 63;
-            const bool over = more && i == 62;
-            const int nb0 = over ? __builtin_amdgcn_readlane(nxt.blk, 0) : __builtin_amdgcn_readlane(cur.blk, fi);
-            const int nb1 = over ? __builtin_amdgcn_readlane(nxt.blk, 1) : __builtin_amdgcn_readlane(cur.blk, fi + 1);
-            float ks[2], vs[2];
-            int nv[2];
+            const int jn = more ? j + 1 : j, fi = (more ? i + kTiles : i) & 63;
+            const bool over = more && i == 64 - kTiles;
+            Blocks next;
+            float ks[kTiles], vs[kTiles];
+            int nv[kTiles], all = 0;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < kTiles; ++h) {
+                next.b[h] = over ? __builtin_amdgcn_readlane(nxt.blk, h) : __builtin_amdgcn_readlane(cur.blk, fi + h);
                 ks[h] = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(cur.ks), i + h));
                 vs[h] = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(cur.vs), i + h));
                 nv[h] = __builtin_amdgcn_readlane(cur.nv, i + h);
+                all += nv[h];
             }
-            // ---- scores of both tiles in log2 units: tokens 4g + r of head n ----
-            float sv[8];
+            // ---- scores in log2 units: tokens 4g + r of each tile, head n ----
+            float sv[4 * kTiles];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < kTiles; ++h) {
                 tq_floatx4 sc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int cc = 0; cc < 4; ++cc) {
@@ -219,13 +238,13 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) sv[4 * h + r] = sc[r] * f;
             }
-            load_keys(nb0, nb1, 2 * jn);
-            if (nv[0] + nv[1] != 32) {
+            load_keys(next, kTiles * jn);
+            if (all != 16 * kTiles) {
 #pragma unroll
-                for (int r = 0; r < 8; ++r)
+                for (int r = 0; r < 4 * kTiles; ++r)
                     if (4 * g + (r & 3) >= nv[r >> 2]) sv[r] = kKv8NegInf;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < kTiles; ++h) {
                     const uint32_t keep = kv8_keep(nv[h] - 4 * g);
 #pragma unroll
                     for (int a = 0; a < 8; ++a) vw[h][a] &= keep;
@@ -233,7 +252,11 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
                 }
             }
             // ---- online softmax ----
-            float mx = fmaxf(fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3])), fmaxf(fmaxf(sv[4], sv[5]), fmaxf(sv[6], sv[7])));
+            float mx = sv[0], vmax = vs[0];
+#pragma unroll
+            for (int r = 1; r < 4 * kTiles; ++r) mx = fmaxf(mx, sv[r]);
+#pragma unroll
+            for (int h = 1; h < kTiles; ++h) vmax = fmaxf(vmax, vs[h]);
             if (__builtin_amdgcn_ballot_w64(mx > M)) {
                 const float Mn = fmaxf(M, tq_max_over_groups(mx));
                 const float alpha = __builtin_amdgcn_exp2f(M - Mn);
@@ -242,13 +265,6 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
                 for (int a = 0; a < 8; ++a) acc[a] *= alpha;
                 M = Mn;
             }
-            float pr[8];
-#pragma unroll
-            for (int r = 0; r < 8; ++r) pr[r] = __builtin_amdgcn_exp2f(sv[r] - M);
-            tq_half8 ph, pl;
-            kv8_prob8<FINE>(pr, ph, pl);
-            lsum += kv8_sum8<FINE>(pr, ph);
-            const float vmax = fmaxf(vs[0], vs[1]);
             if (vmax > vref) {  // wave-uniform
                 const float f = vref / vmax;
 #pragma unroll
@@ -256,18 +272,27 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
                 vref = vmax;
             }
             const float rv = vref > 0.f ? 1.f / vref : 0.f;
-            const float va = kv8_relative(vs[0], rv), vbs = kv8_relative(vs[1], rv);
 #pragma unroll
-            for (int a = 0; a < 8; ++a) {
-                const tq_half8 v = kv8_half8<ENC>(vw[0][a], vw[1][a], va, vbs);
-                acc[a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, acc[a], 0, 0, 0);
-                if (FINE) acc[a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, acc[a], 0, 0, 0);
+            for (int h = 0; h < kTiles; h += 2) {
+                float pr[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r) pr[r] = __builtin_amdgcn_exp2f(sv[4 * h + r] - M);
+                tq_half8 ph, pl;
+                kv8_prob8<FINE>(pr, ph, pl);
+                lsum += kv8_sum8<FINE>(pr, ph);
+                const float va = kv8_relative(vs[h], rv), vb2 = kv8_relative(vs[h + 1], rv);
+#pragma unroll
+                for (int a = 0; a < 8; ++a) {
+                    const tq_half8 v = kv8_half8<ENC>(vw[h][a], vw[h + 1][a], va, vb2);
+                    acc[a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph, acc[a], 0, 0, 0);
+                    if (FINE) acc[a] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl, acc[a], 0, 0, 0);
+                }
             }
-            load_values(nb0, nb1, 2 * jn);
+            load_values(next, kTiles * jn);
         }
         }
 
-        // ---- acc[a][r] is dim 32g + 8r + a of head n ----
+        // ---- acc[a][r] is dim 64 (a / 4) + 16g + 4r + a % 4 of head n ----
         const float l = tq_sum_over_groups(lsum);
         const bool complete = j0 == 0 && j1 == np;
         if (lane == 0) {
@@ -276,18 +301,18 @@ __global__ __launch_bounds__(64 * kWaves, 3) void kv8_decode_kernel(Kv8Attn p) {
             if (j1 == np) ends[1] = (int)w;
         }
         if (n < p.group) {
-            float o[32];
+            float o[2][16];
             const float f = complete ? (l == 0.f ? 0.f : vref / l) : vref;
 #pragma unroll
             for (int a = 0; a < 8; ++a)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) o[8 * r + a] = acc[a][r] * f;
-            if (complete) {
-                kv8_store<32>(p.a.out, s * p.a.out_stride_token + (int64_t)(kh * p.group + n) * p.a.out_stride_head + 32 * g,
-                              p.a.out_dtype, o);
-            } else {
-                const int64_t row = (w + (int64_t)s * hkv + kh) * p.group + n;
-                kv8_store<32>(p.ws_acc, row * TQ_HEAD_DIM + 32 * g, TQ_F32, o);
+                for (int r = 0; r < 4; ++r) o[a >> 2][4 * r + (a & 3)] = acc[a][r] * f;
+            const int64_t row = (w + (int64_t)s * hkv + kh) * p.group + n;
+            const int64_t at = complete ? s * p.a.out_stride_token + (int64_t)(kh * p.group + n) * p.a.out_stride_head : row * TQ_HEAD_DIM;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+                kv8_store<16>(complete ? p.a.out : (void*)p.ws_acc, at + 64 * k + 16 * g, complete ? p.a.out_dtype : TQ_F32, o[k]);
+            if (!complete) {
                 if (g == 0) {
                     p.ws_ml[2 * row] = M;
                     p.ws_ml[2 * row + 1] = l;
@@ -453,7 +478,7 @@ extern "C" int tq_kv8_decode(const tq_kv8_attn_args* a, tq_stream_t stream) {
     p.ws_ml = p.ws_acc + slots * p.group * TQ_HEAD_DIM;
     p.ends = reinterpret_cast<int*>(p.ws_ml + slots * p.group * 2);
     // no more waves than the lengths can ask for
-    const int64_t most = (int64_t)a->num_seqs * a->num_kv_heads * ((p.cap + 31) / 32) / kMinSteps;
+    const int64_t most = (int64_t)a->num_seqs * a->num_kv_heads * ((p.cap + 16 * kTiles - 1) / (16 * kTiles)) / kMinSteps;
     int64_t workers = (int64_t)cus * kWavesPerCu;
     workers = workers < kMaxWorkers ? workers : kMaxWorkers;
     workers = workers < most ? workers : most;

@@ -3,8 +3,8 @@
 // A row is one (new token, query head of the GQA group) pair, token-major; a segment is a block of 64 rows
 // (32 with FINE) of a (sequence, KV head) with the keys that its rows see, walked in steps of 32 (two 16-token
 // tiles).  A wave works on its own, without barriers.  MFMA layout, lane l, n = l % 32, h = l / 32:
-//   S^T [32 tokens x 32 rows] = K . Q^T      8 x mfma_f32_32x32x16_f16; slice c covers dims 64h + 8c + (0..7), so the
-//                                            lane's operand is 64 bytes of token n
+//   S^T [32 tokens x 32 rows] = K . Q^T      8 x mfma_f32_32x32x16_f16; slices 2c and 2c + 1 cover dims 32c + 16h + (0..15):
+//                                            16 bytes of token n, the lane halves' next to each other
 //   O^T [dim 4m + d][row] += V^T . P^T       4 x mfma_f32_32x32x16_f16 per tile, k = 8h + i being tokens 4h + i and 8 + 4h + i:
 //                                            what S^T leaves in the lane, and two words of the values layout
 // A code converted to fp16 feeds both of the wave's 32-row tiles.  The query operands of 64 rows stay in LDS:
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
 
     uint32_t q_at = (uint32_t)(wave * (8 * kRT * 64) + lane);
     const uint32_t scale_at = (uint32_t)a.block_size * TQ_HEAD_DIM;
-    const uint32_t k_off = 128 * (n & 15) + 64 * h, v_off = 512 * h + 16 * n;
+    const uint32_t k_off = 128 * (n & 15) + 16 * h, v_off = 512 * h + 16 * n;
 
     while (dealt == kTickets || seg < p1) {
         const int64_t u = q.a + (int64_t)q.step * rb;
@@ -329,10 +329,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                 const bool real = i < computed;
                 const int sn = p.causal ? q.L - q.nq + i + 1 : q.L;  // tokens that the row sees
                 seen[rt] = real && sn > 0 ? (sn < q.L ? sn : q.L) : 0;
-                const int64_t off = (int64_t)(q.q0 + (real ? i : 0)) * a.q_stride_token + (int64_t)(real ? head : 0) * a.q_stride_head + 64 * h;
+                const int64_t off = (int64_t)(q.q0 + (real ? i : 0)) * a.q_stride_token + (int64_t)(real ? head : 0) * a.q_stride_head + 16 * h;
                 float x[32], y[32], m = 0.f;
-                kv8_load32(a.q, off, a.q_dtype, x);
-                kv8_load32(a.q, off + 32, a.q_dtype, y);
+                kv8_load32(a.q, off, 32, a.q_dtype, x);
+                kv8_load32(a.q, off + 64, 32, a.q_dtype, y);
 #pragma unroll
                 for (int k = 0; k < 32; ++k) m = fmaxf(m, fmaxf(__builtin_fabsf(x[k]), __builtin_fabsf(y[k])));
                 m = fmaxf(m, __shfl_xor(m, 32, 64));
@@ -384,7 +384,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                 const int64_t a0 = tile_at(ti, b0, a.k_stride_block), a1 = tile_at(ti + 1, b1, a.k_stride_block);
                 const tq_u32x4* src = reinterpret_cast<const tq_u32x4*>(kb + (n < 16 ? a0 : a1) + k_off);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) kw[c] = src[c];
+                for (int c = 0; c < 4; ++c) kw[c] = src[2 * c];
             };
             auto load_values = [&](int b0, int b1, int ti) {
 #pragma unroll
