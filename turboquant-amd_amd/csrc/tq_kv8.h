@@ -20,15 +20,21 @@ template <>
 struct Kv8Code<TQ_E4M3> {
     // smallest e with top <= 448 * 2^e: 448 = 1.75 * 2^8, so one is carried where top's mantissa is over 0.75
     static __device__ __forceinline__ int exponent(uint32_t top_bits) { return (int)((top_bits + 0x1fffffu) >> 23) - 127 - 8; }
-    // four codes of scaled values, the first in the low byte
-    static __device__ __forceinline__ uint32_t pack(float a, float b, float c, float d) {
-        int w = __builtin_amdgcn_cvt_pk_fp8_f32(clamp(a), clamp(b), 0, false);
-        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(clamp(c), clamp(d), w, true);
+    // four codes of values times inv, the first in the low byte; ODD: some may not be finite
+    template <bool ODD>
+    static __device__ __forceinline__ uint32_t pack(float a, float b, float c, float d, float inv) {
+        a = clamp<ODD>(a * inv);
+        b = clamp<ODD>(b * inv);
+        c = clamp<ODD>(c * inv);
+        d = clamp<ODD>(d * inv);
+        const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+        return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
     }
     // (only infinities are outside; NaN stays)
+    template <bool ODD>
     static __device__ __forceinline__ float clamp(float x) {
         const float y = __builtin_amdgcn_fmed3f(x, -448.f, 448.f);
-        return x == x ? y : x;
+        return ODD && x == x ? y : x;
     }
     static __device__ __forceinline__ float value(uint32_t w, int i) {
         return i == 0   ? __builtin_amdgcn_cvt_f32_fp8((int)w, 0)
@@ -47,12 +53,16 @@ template <>
 struct Kv8Code<TQ_INT8> {
     // 127 = 1.984375 * 2^6
     static __device__ __forceinline__ int exponent(uint32_t top_bits) { return (int)((top_bits + 0x1ffffu) >> 23) - 127 - 6; }
-    static __device__ __forceinline__ uint32_t code(float x) {
-        const float y = __builtin_amdgcn_fmed3f(__builtin_rintf(x == x ? x : 0.f), -127.f, 127.f);
-        return (uint32_t)(int)y & 0xffu;
+    // x * inv + 1.5 * 2^23 holds the nearest whole number (ties to even) in its low bits
+    template <bool ODD>
+    static __device__ __forceinline__ uint32_t code(float x, float inv) {
+        if (ODD) x = __builtin_amdgcn_fmed3f(x == x ? x * inv : 0.f, -127.f, 127.f);
+        return __float_as_uint(__builtin_fmaf(x, ODD ? 1.f : inv, 12582912.f));
     }
-    static __device__ __forceinline__ uint32_t pack(float a, float b, float c, float d) {
-        return code(a) | code(b) << 8 | code(c) << 16 | code(d) << 24;
+    template <bool ODD>
+    static __device__ __forceinline__ uint32_t pack(float a, float b, float c, float d, float inv) {
+        const uint32_t lo = __builtin_amdgcn_perm(code<ODD>(b, inv), code<ODD>(a, inv), 0x0c0c0400u);
+        return __builtin_amdgcn_perm(code<ODD>(d, inv), code<ODD>(c, inv), 0x04000c0cu) | lo;
     }
     static __device__ __forceinline__ float value(uint32_t w, int i) { return (float)(int8_t)(w >> (8 * i)); }
     // The byte b = code + 128 under the exponent byte 0x64 is the fp16 number 1024 + b; s * (that) - 1152 s is

@@ -16,8 +16,8 @@
 // factor; V's scale, relative to the largest met so far, into the conversion to fp16, which is
 // exact (and the accumulators are rescaled when a larger one is met).
 //
-// Bound: HBM reads, 256 bytes per token and KV head: 64 x 32768 tokens of 8 heads in 759 us, 5.7 TB/s, where a plain
-// read of 2 GiB reaches 5.8.  Small calls: launches, start-up (the search for the wave's part, block table, scales) and
+// Bound: HBM reads, 256 bytes per token and KV head: 64 x 32768 tokens of 8 heads in 759 us, 5.7 TB/s, where a large
+// copy moves 4.9.  Small calls: launches, start-up (the search for the wave's part, block table, scales) and
 // the merge, about 15 us.
 #include "tq_kv8.h"
 
