@@ -521,9 +521,12 @@ int tq_kv8_update(const tq_kv8_update_args* a, tq_stream_t stream);
  * with fp32 (or exact) sums.  q is scaled by a power of two per row to fp16 range and K is exact in
  * fp16; the probabilities are rounded to fp16 before the product with V.  With q or out of type TQ_F32
  * q and the probabilities are taken as the sum of two fp16 numbers instead.
- * A row that sees no token gives 0, as do rows of sequences of length 0.  Block-table entries outside
- * [0, num_blocks) mask their tokens.  Query rows outside every sequence are not written.  Sequences
- * longer than the block table (decode: than max_seq_len) are cut there.  max_q_len >= every n.
+ * A row that sees no token gives 0, as do rows of sequences of length 0.  NaN in K or V reaches the rows
+ * that see its token and no others.  V enters relative to the largest scale so far of the tokens in
+ * order: a block whose scale is below 2^-24 of that counts as zeros, above 2^-15 of it it is exact.
+ * Block-table entries outside [0, num_blocks) mask their tokens.  Query rows outside every sequence are
+ * not written.  Sequences longer than the block table (decode: than max_seq_len) or than 0x7fff0000
+ * tokens are cut there.  cu_seqlens_q ascends from 0 or more to at most T; max_q_len >= every n.
  * workspace: tq_kv8_decode_workspace_bytes / tq_kv8_prefill_workspace_bytes of the same sizes, 256-byte
  * aligned, no initial contents; calls that overlap in time must not share one.  How the keys are cut
  * over the device follows from all lengths of the call: the same call gives the same bits, the same

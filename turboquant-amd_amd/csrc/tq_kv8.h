@@ -80,6 +80,7 @@ __device__ __forceinline__ float kv8_exp2i(int e) { return __uint_as_float((uint
 // ---- attention over the tiles: what the decode and prefill kernels share ----
 constexpr float kKv8NegInf = -__builtin_huge_valf();
 constexpr float kKv8None = -1e30f;  // exponent base of a row that has seen no token
+constexpr int kKv8MaxLen = 0x7fff0000;  // tokens of a sequence
 constexpr float kKv8Log2e = 1.4426950408889634f;
 
 struct Kv8Attn {
@@ -190,6 +191,11 @@ __device__ __forceinline__ float kv8_relative(float s, float inv) {
     return r < 5.9604645e-8f ? 0.f : r;
 }
 
+// The same from the difference of their exponents
+__device__ __forceinline__ float kv8_step(int d) { return d < -24 ? 0.f : kv8_exp2i(d); }
+// A scale from its fp32 exponent field (0: zero)
+__device__ __forceinline__ float kv8_scale(int e) { return __uint_as_float((uint32_t)e << 23); }
+
 // Eight fp16 of two code words, four values each, times sa and sb
 template <int ENC>
 __device__ __forceinline__ tq_half8 kv8_half8(uint32_t a, uint32_t b, float sa, float sb) {
@@ -200,6 +206,9 @@ __device__ __forceinline__ tq_half8 kv8_half8(uint32_t a, uint32_t b, float sa, 
 
 // The word's bytes of the first n of its four tokens
 __device__ __forceinline__ uint32_t kv8_keep(int n) { return n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u; }
+
+// 0x80 in the bytes that are an e4m3 NaN
+__device__ __forceinline__ uint32_t kv8_nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
 // host: checks that decode and prefill share, and the derived fields
 int tq_kv8_attn_setup(const tq_kv8_attn_args* a, Kv8Attn* p);

@@ -447,9 +447,9 @@ int tq_kv8_attn_setup(const tq_kv8_attn_args* a, Kv8Attn* p) {
     p->tpb_div = tq_make_udiv((uint32_t)p->tpb);
     p->group = a->num_q_heads / a->num_kv_heads;
     p->group_div = tq_make_udiv((uint32_t)p->group);
-    // (positions stay below 2^31 with room for a tile)
+    // (positions stay below 2^31, those of the 64 tiles requested ahead included)
     const int64_t cap = (int64_t)a->max_blocks_per_seq * a->block_size;
-    p->cap = (int)(cap < 0x7fffff00 ? cap : 0x7fffff00);
+    p->cap = (int)(cap < kKv8MaxLen ? cap : kKv8MaxLen);
     return TQ_OK;
 }
 
@@ -467,7 +467,7 @@ extern "C" int tq_kv8_decode(const tq_kv8_attn_args* a, tq_stream_t stream) {
     if (p.group > 16) return TQ_ERR_GQA;
     if (a->num_seqs == 0) return TQ_OK;
     if (a->max_seq_len < 0 || (int64_t)a->num_seqs * a->num_q_heads > INT32_MAX) return TQ_ERR_INVALID_ARGUMENT;
-    if (!a->q || !a->out || !a->k_cache || !a->v_cache || !a->block_tables || !a->seq_lens) return TQ_ERR_INVALID_ARGUMENT;
+    if (!a->q || !a->out || !a->k_cache || !a->v_cache || (!a->block_tables && a->max_blocks_per_seq) || !a->seq_lens) return TQ_ERR_INVALID_ARGUMENT;
     const int64_t need = tq_kv8_decode_workspace_bytes(a->num_seqs, a->num_q_heads, a->num_kv_heads);
     if (!a->workspace || (uintptr_t)a->workspace % 256 || a->workspace_bytes < need) return TQ_ERR_WORKSPACE;
     const int cus = tq_kv8_cus();

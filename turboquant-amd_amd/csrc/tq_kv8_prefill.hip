@@ -249,6 +249,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
     // then share in L1.  One counter per XCD for the pairs x, x + 8, .., so that a pair's keys are read by one XCD, the
     // pairs' last (longest) row blocks first; an XCD without work left goes on with the next one's.  The next ticket is
     // taken while the one at hand is worked on.
+    __shared__ int s_nan[kWaves];  // a NaN among the values of the segment's edge steps
+    if (lane == 0) s_nan[wave] = 0;
     __shared__ int s_ticket[2][2];  // pair (-1: none left), row blocks from the last
     const int pairs = a.num_seqs * hkv;
     const int turns = (most_rb + kWaves - 1) / kWaves;
@@ -355,47 +357,51 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
             const int32_t* bt = a.block_tables + s * a.block_table_stride;
             const int last_tile = q.L > 0 ? (q.L - 1) >> 4 : 0;
 
-            // ---- 64 tiles' blocks and scales at a time, one per lane ----
+            // ---- 64 tiles at a time, one per lane: where their codes are, rows in use, the scales' exponents ----
+            // (work on a tile's address is done here once; a scalar instruction per step costs a wave as much as a vector one)
             struct Tiles {
-                int blk, nv;
-                float ks, vs;
+                uint32_t klo, khi, vlo, vhi;
+                int what;  // rows in use, K's exponent << 8, V's exponent << 16, both + 127
             };
             auto tiles_from = [&](int t0) -> Tiles {
-                Tiles t;
                 const int ti = t0 + lane;
-                const int tc = ti < last_tile ? ti : last_tile;
-                t.blk = bt[tq_udiv_apply((uint32_t)tc, p.at.tpb_div)];
-                const int nv = q.L - 16 * ti;
-                t.nv = nv < 16 ? (nv > 0 ? nv : 0) : 16;
-                if ((uint32_t)t.blk >= (uint64_t)a.num_blocks) {
-                    t.blk = 0;
-                    t.nv = 0;
+                const int tc = ti < last_tile ? ti : last_tile;  // (behind the last: a valid address, no rows)
+                const int b = (int)tq_udiv_apply((uint32_t)tc, p.at.tpb_div);
+                int blk = bt[b];
+                int nv = q.L - 16 * ti;
+                nv = nv < 16 ? (nv > 0 ? nv : 0) : 16;
+                if ((uint32_t)blk >= (uint64_t)a.num_blocks) {
+                    blk = 0;
+                    nv = 0;
                 }
-                t.ks = *reinterpret_cast<const float*>(kb + t.blk * a.k_stride_block + scale_at);
-                t.vs = *reinterpret_cast<const float*>(vb + t.blk * a.v_stride_block + scale_at);
-                return t;
+                const uint64_t kblk = (uint64_t)kb + blk * a.k_stride_block, vblk = (uint64_t)vb + blk * a.v_stride_block;
+                const uint32_t ke = *reinterpret_cast<const uint32_t*>(kblk + scale_at) >> 23;
+                const uint32_t ve = *reinterpret_cast<const uint32_t*>(vblk + scale_at) >> 23;
+                const uint32_t in = (uint32_t)(tc - p.at.tpb * b) * (16 * TQ_HEAD_DIM);
+                return {(uint32_t)(kblk + in), (uint32_t)((kblk + in) >> 32), (uint32_t)(vblk + in), (uint32_t)((vblk + in) >> 32),
+                        (int)((uint32_t)nv | (ke & 255u) << 8 | (nv ? ve & 255u : 0u) << 16)};
             };
-            auto tile_at = [&](int ti, int blk, int64_t stride) -> int64_t {
-                const int tc = ti < last_tile ? ti : last_tile;
-                return blk * stride + (int64_t)(tc - p.at.tpb * (int)tq_udiv_apply((uint32_t)tc, p.at.tpb_div)) * (16 * TQ_HEAD_DIM);
+            auto address = [](uint32_t lo, uint32_t hi, int i) -> uint64_t {
+                return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)lo, i) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, i) << 32;
             };
             tq_u32x4 kw[4], vw[2][2];
-            auto load_keys = [&](int b0, int b1, int ti) {
-                const int64_t a0 = tile_at(ti, b0, a.k_stride_block), a1 = tile_at(ti + 1, b1, a.k_stride_block);
-                const tq_u32x4* src = reinterpret_cast<const tq_u32x4*>(kb + (n < 16 ? a0 : a1) + k_off);
+            auto load_keys = [&](const Tiles& t, int i) {
+                const uint64_t a0 = address(t.klo, t.khi, i), a1 = address(t.klo, t.khi, i + 1);
+                const tq_u32x4* src = reinterpret_cast<const tq_u32x4*>((n < 16 ? a0 : a1) + k_off);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) kw[c] = src[2 * c];
             };
-            auto load_values = [&](int b0, int b1, int ti) {
+            auto load_values = [&](const Tiles& t, int i) {
 #pragma unroll
                 for (int v = 0; v < 2; ++v) {
-                    const uint8_t* src = vb + tile_at(ti + v, v ? b1 : b0, a.v_stride_block);
+                    const uint8_t* src = reinterpret_cast<const uint8_t*>(address(t.vlo, t.vhi, i + v));
 #pragma unroll
                     for (int k = 0; k < 2; ++k) vw[v][k] = *reinterpret_cast<const tq_u32x4*>(src + v_off + 1024 * k);
                 }
             };
 
-            float M[kRT], lsum[kRT], vref = 0.f, rv = 0.f;
+            float M[kRT], lsum[kRT];
+            int vref = 0;  // exponent + 127 of the largest V scale so far (0: none)
             f32x16 acc[kRT][4];
 #pragma unroll
             for (int rt = 0; rt < kRT; ++rt) {
@@ -407,34 +413,33 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                     for (int v = 0; v < 16; ++v) acc[rt][d][v] = 0.f;
             }
 
-            // The loads of step j + 1 go out during step j without a condition (the last step repeats its own): where the
-            // compiler cannot count what is under way, it waits for all of it.
-            Tiles nxt = {0, 0, 0.f, 0.f};
+            // The loads of step j + 1 go out during step j without a condition (behind the last step, those of the sequence's last
+            // tile): where the compiler cannot count what is under way, it waits for all of it.  31 steps use a group of 64
+            // tiles, whose last two are the first of the next.
+            Tiles nxt = {0, 0, 0, 0, 0};
+            tq_half8 b_first[kAhead];  // the first query operands, the same in every step
             if (j0 < j1) {
                 nxt = tiles_from(2 * j0);
-                const int b0 = __builtin_amdgcn_readlane(nxt.blk, 0), b1 = __builtin_amdgcn_readlane(nxt.blk, 1);
-                load_keys(b0, b1, 2 * j0);
-                load_values(b0, b1, 2 * j0);
+                load_keys(nxt, 0);
+                load_values(nxt, 0);
+                if (kQLds) {
+#pragma unroll
+                    for (int i = 0; i < kAhead; ++i) b_first[i] = reinterpret_cast<const tq_half8*>(s_lds)[q_at + i * 64];
+                }
             }
-            for (int jg = j0; jg < j1; jg += 32) {  // 32 steps: 64 tiles
-                const int t0 = 2 * jg, je = jg + 32 < j1 ? jg + 32 : j1;
+            for (int jg = j0; jg < j1; jg += 31) {
+                const int je = jg + 31 < j1 ? jg + 31 : j1;
                 const Tiles cur = nxt;
-                nxt = tiles_from(t0 + 64);
+                nxt = tiles_from(2 * jg + 62);
                 for (int j = jg; j < je; ++j) {
-                    const int i = 2 * j - t0;
-                    const bool more = j + 1 < j1;
-                    // the next step's tiles
-                    const int jn = more ? j + 1 : j, fi = (more ? i + 2 : i) & 63;
-                    const bool over = more && i == 62;
-                    const int nb0 = over ? __builtin_amdgcn_readlane(nxt.blk, 0) : __builtin_amdgcn_readlane(cur.blk, fi);
-                    const int nb1 = over ? __builtin_amdgcn_readlane(nxt.blk, 1) : __builtin_amdgcn_readlane(cur.blk, fi + 1);
-                    float ks[2], vs[2];
-                    int nv[2];
+                    const int i = 2 * (j - jg);
+                    int ke[2], ve[2], nv[2];
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        ks[t] = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(cur.ks), i + t));
-                        vs[t] = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(cur.vs), i + t));
-                        nv[t] = __builtin_amdgcn_readlane(cur.nv, i + t);
+                        const int w = __builtin_amdgcn_readlane(cur.what, i + t);
+                        nv[t] = w & 255;
+                        ke[t] = (w >> 8) & 255;
+                        ve[t] = (w >> 16) & 255;
                     }
                     // ---- scores ----
                     // (the operands' place is hidden from the compiler, which would keep all of them in registers)
@@ -449,7 +454,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                         // operand i = slice i / 2, row tile i % 2, read kAhead products before its own
                         tq_half8 b[kAhead + 1], k;
 #pragma unroll
-                        for (int i = 0; i < kAhead; ++i) b[i] = q_in[i * 64];
+                        for (int i = 0; i < kAhead; ++i) b[i] = b_first[i];
 #pragma unroll
                         for (int i = 0; i < 8 * kRT; ++i) {
                             const int c = i / kRT, rt = i % kRT;
@@ -469,18 +474,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                             }
                         }
                     }
-                    load_keys(nb0, nb1, 2 * jn);
+                    load_keys(cur, i + 2);
                     if (32 * j + 32 > least || nv[0] + nv[1] != 32) {
 #pragma unroll
                         for (int rt = 0; rt < kRT; ++rt)
 #pragma unroll
-                            for (int v = 0; v < 16; ++v) {
-                                const int t = v >> 3, in = 8 * ((v >> 2) & 1) + 4 * h + (v & 3);
-                                if (in >= nv[t] || 32 * j + 16 * t + in >= seen[rt]) sc[rt][v] = kKv8NegInf;
+                            for (int t = 0; t < 2; ++t) {
+                                const int sn = seen[rt] - 32 * j - 16 * t, upto = (sn < nv[t] ? sn : nv[t]) - 4 * h;
+#pragma unroll
+                                for (int v = 0; v < 8; ++v)
+                                    if (8 * (v >> 2) + (v & 3) >= upto) sc[rt][8 * t + v] = kKv8NegInf;
                             }
 #pragma unroll
                         for (int t = 0; t < 2; ++t) {
-                            if (nv[t] <= 0) vs[t] = 0.f;
 #pragma unroll
                             for (int k = 0; k < 2; ++k) {
                                 const uint32_t keep = kv8_keep(nv[t] - 8 * k - 4 * h);
@@ -488,23 +494,29 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                                 for (int d = 0; d < 4; ++d) vw[t][k][d] &= keep;
                             }
                         }
-                    }
-                    const float vmax = fmaxf(vs[0], vs[1]);
-                    if (vmax > vref) {  // wave-uniform
-                        const float r = vref / vmax;
+                        // (a NaN among the values must not reach the rows that do not see its token, as 0 * NaN: here its code
+                        // becomes 0, and the rows that do see it get theirs after the stores)
+                        if (ENC == TQ_E4M3 && 32 * j + 32 > least) {
+                            uint32_t nans = 0;
 #pragma unroll
-                        for (int rt = 0; rt < kRT; ++rt)
+                            for (int t = 0; t < 2; ++t)
 #pragma unroll
-                            for (int d = 0; d < 4; ++d) acc[rt][d] *= r;
-                        vref = vmax;
-                        rv = 1.f / vref;
+                                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                                    for (int d = 0; d < 4; ++d) {
+                                        const uint32_t nan = kv8_nan_bytes(vw[t][k][d]);
+                                        nans |= nan;
+                                        vw[t][k][d] &= ~((nan << 1) - (nan >> 7));
+                                    }
+                            if (nans) s_nan[wave] = 1;
+                        }
                     }
                     // ---- online softmax ----
                     tq_half8 ph[kRT][2], pl[FINE ? kRT : 1][2];
 #pragma unroll
                     for (int rt = 0; rt < kRT; ++rt) {
                         // (over zero, so that a masked score stays -inf)
-                        const float f[2] = {fmaxf(c1[rt] * ks[0], 1e-37f), fmaxf(c1[rt] * ks[1], 1e-37f)};
+                        const float f[2] = {fmaxf(c1[rt] * kv8_scale(ke[0]), 1e-37f), fmaxf(c1[rt] * kv8_scale(ke[1]), 1e-37f)};
                         auto probabilities = [&]() -> float {
                             float sum[2];
 #pragma unroll
@@ -537,7 +549,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                     }
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        const float vf = kv8_relative(vs[t], rv);
+                        // (tile by tile: a row that sees the first alone keeps all bits of it)
+                        if (ve[t] > vref) {  // wave-uniform
+                            const float r = kv8_scale(127 + vref - ve[t] > 0 ? 127 + vref - ve[t] : 0);
+#pragma unroll
+                            for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+                                for (int d = 0; d < 4; ++d) acc[rt][d] *= r;
+                            vref = ve[t];
+                        }
+                        const float vf = kv8_step(ve[t] - vref);
 #pragma unroll
                         for (int d = 0; d < 4; ++d) {
                             const tq_half8 v = kv8_half8<ENC>(vw[t][0][d], vw[t][1][d], vf, vf);
@@ -548,7 +569,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                             }
                         }
                     }
-                    load_values(nb0, nb1, 2 * jn);
+                    load_values(cur, i + 2);
                 }
             }
 
@@ -559,7 +580,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                 const float l = lsum[rt] + __shfl_xor(lsum[rt], 32, 64);
                 int i, head;
                 row_of(rt, i, head);
-                const float f = complete ? (l == 0.f ? 0.f : vref / l) : vref;
+                const float f = complete ? (l == 0.f ? 0.f : kv8_scale(vref) / l) : kv8_scale(vref);
                 if (i < computed) {
                     const int64_t row = (int64_t)(2 * w + (seg > p0 ? 1 : 0)) * kRows + 32 * rt + n;
                     const int64_t at = complete ? (int64_t)(q.q0 + i) * a.out_stride_token + (int64_t)head * a.out_stride_head : row * TQ_HEAD_DIM;
@@ -577,6 +598,28 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                     if (!complete && h == 0) {
                         p.at.ws_ml[2 * row] = M[rt];
                         p.at.ws_ml[2 * row + 1] = l;
+                    }
+                }
+            }
+            if (ENC == TQ_E4M3 && uniform(s_nan[wave])) {
+                s_nan[wave] = 0;
+                __threadfence_block();
+                const int from = least > 32 * j0 ? least & ~31 : 32 * j0, to = 32 * j1 < q.L ? 32 * j1 : q.L;
+                for (int t = from; t < to; ++t) {
+                    const int b = (int)tq_udiv_apply((uint32_t)(t >> 4), p.at.tpb_div), in = t - b * a.block_size;
+                    const int blk = bt[b];
+                    if ((uint32_t)blk >= (uint64_t)a.num_blocks) continue;
+                    const uint8_t* codes = vb + blk * a.v_stride_block + 512 * (in >> 2) + (in & 3);
+                    for (int d = lane; d < TQ_HEAD_DIM; d += 64) {
+                        if ((codes[4 * d] & 0x7f) != 0x7f) continue;
+                        for (int r = 0; r < kRows; ++r) {
+                            const uint32_t x = (uint32_t)(rb * kRows + r);
+                            const int i = (int)tq_udiv_apply(x, p.at.group_div);
+                            if (i >= computed || t >= (p.causal ? q.L - q.nq + i + 1 : q.L)) continue;
+                            const int head = kh * group + (int)(x - (uint32_t)i * (uint32_t)group);
+                            if (complete) tq_store1(a.out, (int64_t)(q.q0 + i) * a.out_stride_token + (int64_t)head * a.out_stride_head + d, a.out_dtype, __builtin_nanf(""));
+                            else p.at.ws_acc[((int64_t)(2 * w + (seg > p0 ? 1 : 0)) * kRows + r) * TQ_HEAD_DIM + d] = __builtin_nanf("");
+                        }
                     }
                 }
             }
@@ -691,7 +734,7 @@ extern "C" int tq_kv8_prefill(const tq_kv8_attn_args* a, tq_stream_t stream) {
     if (rc != TQ_OK) return rc;
     if (a->max_q_len < 0 || (a->flags & ~TQ_PREFILL_CAUSAL)) return TQ_ERR_INVALID_ARGUMENT;
     if (a->num_seqs == 0 || a->max_q_len == 0) return TQ_OK;
-    if (!a->q || !a->out || !a->k_cache || !a->v_cache || !a->block_tables || !a->seq_lens || !a->cu_seqlens_q)
+    if (!a->q || !a->out || !a->k_cache || !a->v_cache || (!a->block_tables && a->max_blocks_per_seq) || !a->seq_lens || !a->cu_seqlens_q)
         return TQ_ERR_INVALID_ARGUMENT;
     // (row numbers and a row block's tokens stay in 32 bits)
     if ((int64_t)a->max_q_len * p.at.group > 0x7fffff00) return TQ_ERR_INVALID_ARGUMENT;

@@ -239,7 +239,7 @@ def decode_paged8(
     caches = _check_pair(k_cache, k_fmt, v_cache, v_fmt, "decode_paged8")
     if caches[1] and q.shape[1] > 16 * caches[1]:
         raise ValueError("decode_paged8 takes up to 16 query heads per KV head")
-    cap = min(block_tables.shape[-1] * k_fmt.block_size, 0x7fffff00) if block_tables.dim() else 0
+    cap = min(block_tables.shape[-1] * k_fmt.block_size, 0x7fff0000) if block_tables.dim() else 0
     msl = cap if max_seq_len is None else max(0, min(int(max_seq_len), cap))
     return _attention("tq_kv8_decode", dev, q, caches, k_cache, v_cache, k_fmt, block_tables, seq_lens, None, sm_scale, msl, 1,
                       0, out, workspace)
@@ -262,9 +262,10 @@ def prefill_paged8(
 ) -> torch.Tensor:
     """Attention of several new tokens per sequence, q [T, Hq, 128], over 8-bit paged K/V caches.
 
-    Sequence s owns query rows cu_seqlens_q[s] .. cu_seqlens_q[s+1] - 1 (int32 [S+1], device) and
+    Sequence s owns query rows cu_seqlens_q[s] .. cu_seqlens_q[s+1] - 1 (int32 [S+1], device, ascending, at most T) and
     seq_lens[s] cache tokens, the new ones included.  causal: query i of n sees the tokens up to position
-    seq_lens - n + i, otherwise all of them; a row that sees none gives zeros.  Any number of query heads per KV head.
+    seq_lens - n + i, otherwise all of them; a row that sees none gives zeros, and NaN in the cache reaches
+    the rows that see it alone.  Any number of query heads per KV head.
     max_q_len: host-side bound of the query counts (default: T).  Rows of q that belong to no sequence are
     left as they were in out.  Types and workspace as in decode_paged8.
     """

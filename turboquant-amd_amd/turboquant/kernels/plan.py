@@ -56,7 +56,8 @@ def plan_step(
     place) and given-up blocks go to the ring's end; blocks given up in a step are handed out from the next one on.
     A request that the ring cannot serve any more (the needs of the requests before it counted), or
     whose table is too narrow, is not extended: its seq_lens entry stays past_lens and its tokens get slot
-    -1, so that the cache writes skip them.  num_tokens: size of the token arrays, at least the
+    -1, so that the cache writes skip them (what attention gives for those tokens means nothing).  A block
+    belongs to one request: blocks that tables share would be given up twice.  num_tokens: size of the token arrays, at least the
     sum of the positive new_lens.  pool_out: where the ring's new (first, count) goes (default: pool
     itself).  out: a StepPlan whose arrays are written instead of new ones; its seq_lens may be past_lens.
     """
