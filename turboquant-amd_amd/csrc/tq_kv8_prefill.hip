@@ -34,7 +34,7 @@ constexpr int kMergeTokens = 384;  // the cut pieces' set-up and their merge in 
 // reaches from 2^14 above the base to 2^-14 below it.
 constexpr float kDown = 4.f;
 constexpr float kMoveSum = 16384.f;
-constexpr int kAhead = 2;        // query operands read ahead of their products (0: 4 x 4096 tokens 3 % slower)
+constexpr int kFirst = 2;          // query operands that stay in registers (1 .. 4: 4 x 4096 tokens 910, 906, 920, 921 us)
 
 struct Cut {  // a segment that several workers share
     int q0, nq, kh, rb, slot0, w0, w1;  // w0 -1: none; worker 0's rb: the workers in use
@@ -375,8 +375,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                     nv = 0;
                 }
                 const uint64_t kblk = (uint64_t)kb + blk * a.k_stride_block, vblk = (uint64_t)vb + blk * a.v_stride_block;
-                const uint32_t ke = *reinterpret_cast<const uint32_t*>(kblk + scale_at) >> 23;
-                const uint32_t ve = *reinterpret_cast<const uint32_t*>(vblk + scale_at) >> 23;
+                const uint32_t ke = *reinterpret_cast<const uint32_t*>(kb + blk * a.k_stride_block + scale_at) >> 23;
+                const uint32_t ve = *reinterpret_cast<const uint32_t*>(vb + blk * a.v_stride_block + scale_at) >> 23;
                 const uint32_t in = (uint32_t)(tc - p.at.tpb * b) * (16 * TQ_HEAD_DIM);
                 return {(uint32_t)(kblk + in), (uint32_t)((kblk + in) >> 32), (uint32_t)(vblk + in), (uint32_t)((vblk + in) >> 32),
                         (int)((uint32_t)nv | (ke & 255u) << 8 | (nv ? ve & 255u : 0u) << 16)};
@@ -384,19 +384,22 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
             auto address = [](uint32_t lo, uint32_t hi, int i) -> uint64_t {
                 return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)lo, i) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, i) << 32;
             };
+            // (named as global memory: the compiler takes a number for any kind, and a load that may be from LDS keeps the
+            // query operands' waits waiting)
+            using GlobalWords = const __attribute__((address_space(1))) tq_u32x4*;
             tq_u32x4 kw[4], vw[2][2];
             auto load_keys = [&](const Tiles& t, int i) {
                 const uint64_t a0 = address(t.klo, t.khi, i), a1 = address(t.klo, t.khi, i + 1);
-                const tq_u32x4* src = reinterpret_cast<const tq_u32x4*>((n < 16 ? a0 : a1) + k_off);
+                const GlobalWords src = (GlobalWords)((n < 16 ? a0 : a1) + k_off);
 #pragma unroll
                 for (int c = 0; c < 4; ++c) kw[c] = src[2 * c];
             };
             auto load_values = [&](const Tiles& t, int i) {
 #pragma unroll
                 for (int v = 0; v < 2; ++v) {
-                    const uint8_t* src = reinterpret_cast<const uint8_t*>(address(t.vlo, t.vhi, i + v));
+                    const GlobalWords src = (GlobalWords)(address(t.vlo, t.vhi, i + v) + v_off);
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) vw[v][k] = *reinterpret_cast<const tq_u32x4*>(src + v_off + 1024 * k);
+                    for (int k = 0; k < 2; ++k) vw[v][k] = src[64 * k];
                 }
             };
 
@@ -417,14 +420,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
             // tile): where the compiler cannot count what is under way, it waits for all of it.  31 steps use a group of 64
             // tiles, whose last two are the first of the next.
             Tiles nxt = {0, 0, 0, 0, 0};
-            tq_half8 b_first[kAhead];  // the first query operands, the same in every step
+            tq_half8 b_first[kFirst];  // the first query operands, the same in every step
             if (j0 < j1) {
                 nxt = tiles_from(2 * j0);
                 load_keys(nxt, 0);
                 load_values(nxt, 0);
                 if (kQLds) {
 #pragma unroll
-                    for (int i = 0; i < kAhead; ++i) b_first[i] = reinterpret_cast<const tq_half8*>(s_lds)[q_at + i * 64];
+                    for (int i = 0; i < kFirst; ++i) b_first[i] = reinterpret_cast<const tq_half8*>(s_lds)[q_at + i * 64];
                 }
             }
             for (int jg = j0; jg < j1; jg += 31) {
@@ -451,17 +454,13 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
 #pragma unroll
                         for (int v = 0; v < 16; ++v) sc[rt][v] = 0.f;
                     if (kQLds) {
-                        // operand i = slice i / 2, row tile i % 2, read kAhead products before its own
-                        tq_half8 b[kAhead + 1], k;
-#pragma unroll
-                        for (int i = 0; i < kAhead; ++i) b[i] = b_first[i];
+                        // operand i = slice i / 2, row tile i % 2
+                        tq_half8 k;
 #pragma unroll
                         for (int i = 0; i < 8 * kRT; ++i) {
                             const int c = i / kRT, rt = i % kRT;
-                            if (i + kAhead < 8 * kRT) b[(i + kAhead) % (kAhead + 1)] = q_in[(i + kAhead) * 64];
                             if (rt == 0) k = kv8_half8<ENC>(kw[c >> 1][2 * (c & 1)], kw[c >> 1][2 * (c & 1) + 1], 1.f, 1.f);
-                            sc[rt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, b[i % (kAhead + 1)], sc[rt], 0, 0, 0);
-                            __builtin_amdgcn_sched_barrier(0);
+                            sc[rt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, i < kFirst ? b_first[i < kFirst ? i : 0] : q_in[i * 64], sc[rt], 0, 0, 0);
                         }
                     } else {
 #pragma unroll
