@@ -139,6 +139,8 @@ __device__ __forceinline__ void kv8_load32(const void* base, int64_t off, int se
     }
 }
 
+typedef __bf16 kv8_bf162 __attribute__((ext_vector_type(2)));
+
 // N (a multiple of 4) consecutive elements to element off (8-byte aligned for 16-bit types, N = 4)
 template <int N>
 __device__ __forceinline__ void kv8_store(void* base, int64_t off, int dt, const float* o) {
@@ -151,8 +153,8 @@ __device__ __forceinline__ void kv8_store(void* base, int64_t off, int dt, const
     uint32_t w[N / 2];
 #pragma unroll
     for (int i = 0; i < N / 2; ++i)
-        w[i] = dt == TQ_BF16 ? (tq_f32_to_bf16_bits(o[2 * i]) | tq_f32_to_bf16_bits(o[2 * i + 1]) << 16)
-                             : tq_pack_half2(o[2 * i], o[2 * i + 1]);
+        w[i] = dt == TQ_BF16 ? __builtin_bit_cast(uint32_t, kv8_bf162{(__bf16)o[2 * i], (__bf16)o[2 * i + 1]})
+                             : __builtin_bit_cast(uint32_t, kv8_half2{(_Float16)o[2 * i], (_Float16)o[2 * i + 1]});
     uint16_t* d = static_cast<uint16_t*>(base) + off;
     if constexpr (N % 8 == 0) {
 #pragma unroll

@@ -16,7 +16,16 @@
 // in all, worker (wave) w of R takes positions [floor(w P / R), floor((w + 1) P / R)), and of a segment the
 // steps that begin there.  A segment inside one worker is written directly; the pieces of a cut one (at most the
 // first and the last of a worker, slots 2w and 2w + 1) go to the workspace and kv8_prefill_merge_kernel joins
-// them.
+// them.  (A workgroup's four waves on one segment, joined in LDS, leave a quarter of the pieces: 300 new after 2000
+// tokens 58 -> 49 us, but 8 prompts of 900 to 1300 tokens 161 -> 290 and the six long extends 145 -> 147.)
+//
+// Bound: issue.  4 x 4096 tokens of 48 / 8 heads, 0.82 TFLOP, in 860 us, 0.96 PFLOP/s, where a large fp16 matrix product
+// reaches 1.25.  Of a step's time the matrix unit works 44 % and the vector unit 56 % (per step 32 products, 64
+// conversions, 32 exponentials with their scaling, 16 packings, 16 sums): two waves per SIMD do not overlap more.  Without
+// the loads of K and V a step takes 9 % less, without the LDS reads 4.5 %, without the exponentials 5 %.  Tried
+// and slower: 32 rows a wave (1180 us, two or three waves per SIMD), products ordered among the exponentials by
+// hand (1130, spills), the same with one wave per SIMD (1540), a barrier per step so that a workgroup's waves
+// share L1 (+ 3 %).  Calls of few tokens: 20 us of start-up (search, query rows, first loads) and merge.
 #include "tq_kv8.h"
 
 namespace {
@@ -27,8 +36,11 @@ constexpr int kWaves = 4;          // of a workgroup
 constexpr int kWavesPerCu = 8;     // resident
 constexpr int kMaxWorkers = 256 * kWavesPerCu;
 constexpr int kMinTokens = 128;    // stream tokens a worker takes at least (32 or more: see the merge)
-constexpr int kSegTokens = 320;    // a segment's set-up (query loads, first steps, output) in tokens
-constexpr int kMergeTokens = 384;  // the cut pieces' set-up and their merge in tokens
+// A segment's set-up (query loads, first steps, output) in tokens (160, 320, 480, 640: 8 prompts of 900 to 1300 tokens 195, 161,
+// 157, 157 us; 37 to 512 new after 1000 to 16000 of six sequences 147, 145, 145, 148)
+constexpr int kSegTokens = 480;
+// The cut pieces' set-up and their merge in tokens (1500: 8 to 40 new after 100 to 700 of 32 sequences 50.5 -> 53.6 us)
+constexpr int kMergeTokens = 384;
 // A row's exponent base lies kDown below the largest score of the step that set it, and moves only when a lane's
 // 16 probabilities of a step sum to more than kMoveSum: no maximum is worked out otherwise, and fp16's normal range
 // reaches from 2^14 above the base to 2^-14 below it.
@@ -90,8 +102,9 @@ __device__ __forceinline__ int64_t before(const Seq& q, int64_t rb) { return rb 
 // Tokens of the whole stream, and how it is dealt to the workers:
 //   whole     the segments, at kMinTokens each, if they are no more than the workers and the longest takes no longer
 //             than a cut one's worker and the merge;
-//   tickets   whole segments, the next one to whoever is free, if there are several per worker and the ones that come
-//             last are short against a worker's share;
+//   tickets   whole segments, the next one to whoever is free, if there is one per worker and the ones that come last
+//             are short against a worker's share (4 x 2048 tokens 235 -> 210 us, 4 x 4096 1055 -> 908; with half that
+//             demand 64 prompts of 64 to 200 tokens 86 -> 131);
 //   shares    otherwise.
 enum { kShares, kWhole, kTickets };
 __device__ __forceinline__ int64_t stream_total(const Prefill& p, int& dealt, int& most_rb) {
@@ -126,7 +139,7 @@ __device__ __forceinline__ int64_t stream_total(const Prefill& p, int& dealt, in
     if (segs <= p.at.workers && (int64_t)(longest - kMergeTokens) * p.at.workers <= P) dealt = kWhole;
     // (the tickets' numbers run over every sequence's row blocks as if all had the most; those that do not exist cost a
     // ticket)
-    else if (p.tickets && (int64_t)nrb * p.at.a.num_seqs * p.at.a.num_kv_heads <= 2 * segs && segs >= 3 * p.at.workers &&
+    else if (p.tickets && (int64_t)nrb * p.at.a.num_seqs * p.at.a.num_kv_heads <= 2 * segs && segs >= p.at.workers &&
              (int64_t)longest * p.at.workers <= P && 4 * (int64_t)last * p.at.workers <= P)
         dealt = kTickets;
     return dealt == kWhole ? segs * kMinTokens : P;
@@ -137,8 +150,12 @@ struct Share {
     uint32_t rest, R;
     __device__ __forceinline__ int64_t at(int64_t w) const { return w * each + (uint32_t)w * rest / R; }
 };
-__device__ __forceinline__ Share share_of(const Prefill& p, int64_t P) {
-    const int64_t m = P / kMinTokens;
+__device__ __forceinline__ Share share_of(const Prefill& p, int64_t P, bool whole) {
+    // (a SIMD's second wave pays from twice the tokens on: 300 new after 2000 tokens 57.0 -> 53.6 us; with that for all
+    // waves 23 new after 700 take 28.6 instead of 24.8)
+    constexpr int64_t half = kMaxWorkers / 2;
+    int64_t m = P / kMinTokens;
+    if (!whole && m > half) m = m >> 1 > half ? m >> 1 : half;
     Share h;
     h.R = m < 1 ? 1u : (uint32_t)(m < p.at.workers ? m : (int64_t)p.at.workers);
     h.each = P / h.R;
@@ -213,7 +230,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
         if (P == 0) return;
     }
     const bool whole = dealt == kWhole;
-    const Share share = share_of(p, P);
+    const Share share = share_of(p, P, whole);
     // consecutive workers share an XCD (workgroups go to the 8 XCDs in turn), so that its L2 holds few
     // sequences' keys; fewer workers than waves spread over all workgroups
     const int nwg = (int)gridDim.x;
@@ -502,12 +519,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
 #pragma unroll
                                 for (int k = 0; k < 2; ++k)
 #pragma unroll
-                                    for (int d = 0; d < 4; ++d) {
-                                        const uint32_t nan = kv8_nan_bytes(vw[t][k][d]);
-                                        nans |= nan;
-                                        vw[t][k][d] &= ~((nan << 1) - (nan >> 7));
-                                    }
-                            if (nans) s_nan[wave] = 1;
+                                    for (int d = 0; d < 4; ++d) nans |= kv8_nan_bytes(vw[t][k][d]);
+                            if (__builtin_amdgcn_ballot_w64(nans != 0)) {
+#pragma unroll
+                                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                                        for (int d = 0; d < 4; ++d) {
+                                            const uint32_t nan = kv8_nan_bytes(vw[t][k][d]);
+                                            vw[t][k][d] &= ~((nan << 1) - (nan >> 7));
+                                        }
+                                s_nan[wave] = 1;
+                            }
                         }
                     }
                     // ---- online softmax ----
@@ -759,7 +783,7 @@ extern "C" int tq_kv8_prefill(const tq_kv8_attn_args* a, tq_stream_t stream) {
     // (at most as many segments as this)
     const int64_t pairs = (int64_t)a->num_seqs * a->num_kv_heads;
     const int64_t blocks = ((int64_t)a->max_q_len * p.at.group + p.rows - 1) / p.rows;
-    if (pairs <= 0x7fffff && blocks <= 0x7fffffff / pairs && pairs * blocks >= 3 * resident && p.at.workers == resident && resident % 8 == 0)
+    if (pairs <= 0x7fffff && blocks <= 0x7fffffff / pairs && pairs * blocks >= resident && p.at.workers == resident && resident % 8 == 0)
         p.tickets = tickets;
     const void* kern = a->encoding == TQ_E4M3 ? (fine ? (const void*)kv8_prefill_kernel<TQ_E4M3, true> : (const void*)kv8_prefill_kernel<TQ_E4M3, false>)
                                               : (fine ? (const void*)kv8_prefill_kernel<TQ_INT8, true> : (const void*)kv8_prefill_kernel<TQ_INT8, false>);
