@@ -9,7 +9,8 @@
 //
 // The ring needs no order between taking and giving: entries are taken from its occupied part and put behind it.
 //
-// Bound: launch and memory latency (a step of 64 requests touches a few KB).
+// Bound: launch and memory latency: 64 requests with a token each take 5.7 us in one launch; 500 requests with 36000
+// tokens, 0.5 MB, take 4.3 + 5.6 us in two.
 #include "tq_common.h"
 
 namespace {
@@ -208,7 +209,8 @@ extern "C" int tq_plan_step(const tq_plan_args* a, tq_stream_t stream) {
     p.a = *a;
     p.rec = static_cast<Record*>(a->workspace);
     p.block_div = tq_make_udiv((uint32_t)a->block_size);
-    // One workgroup fills four rounds of its threads' tokens in less time than a second launch takes.
+    // A second launch costs 2.5 us from the host, a round of the one workgroup's threads 0.9 (64 requests, 64 / 1024 / 2000 /
+    // 4000 tokens, one launch 13 us from Python and 6.1 / 8.3 / 9.8 / 12.8 in a graph, two 15.5 and 6.7 / 8.6 / 8.6 / 8.5).
     int fill = a->num_seqs <= kThreads && a->num_tokens <= 4 * kThreads;
     void* args[] = {&p, &fill};
     hipError_t e = hipLaunchKernel((const void*)plan_scan_kernel, dim3(1), dim3(kThreads), args, 0, stream);
