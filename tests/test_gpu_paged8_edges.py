@@ -169,3 +169,35 @@ def test_calls_side_by_side(dev):
     for i, w in enumerate(want):
         for r in got[i]:
             assert torch.equal(r[0], w[0]) and torch.equal(r[1], w[1])
+
+
+@pytest.mark.parametrize("dtype,seqs,new,hkv,group", [(torch.float32, 8, 2500, 4, 4), (torch.bfloat16, 4, 2048, 8, 4),
+                                                      (torch.bfloat16, 64, 130, 8, 4), (torch.float16, 5, 333, 3, 5)])
+def test_prefill_prompts(dev, dtype, seqs, new, hkv, group):
+    """Prompts of unequal lengths (one of them empty): whole row blocks by tickets, in 32 and 64 rows, and cut ones."""
+    g = torch.Generator(device=dev).manual_seed(new)
+    block = 16
+    lens = [0 if s == 1 else new - 29 * (s % 4) for s in range(seqs)]
+    width = -(-new // block)
+    kf, vf = formats("e4m3", block)
+    kc, vc = (allocate_cache(seqs * width, hkv, f, device=dev) for f in (kf, vf))
+    bt = torch.randperm(seqs * width, generator=torch.Generator().manual_seed(1)).to(torch.int32).to(dev).view(seqs, width)
+    for s, n in enumerate(lens):
+        t = torch.arange(n, device=dev)
+        k, v = (torch.randn(n, hkv, 128, generator=g, device=dev) for _ in range(2))
+        quantize_paged8_kv(k, v, bt[s].long()[t // block] * block + t % block, kc, vc, kf, vf)
+    starts = np.concatenate([[0], np.cumsum(lens)])
+    q = torch.randn(int(starts[-1]), hkv * group, 128, generator=g, device=dev).to(dtype)
+    cu, sl = (torch.tensor(np.asarray(x), dtype=torch.int32, device=dev) for x in (starts, lens))
+    got = prefill_paged8(q, cu, kc, kf, vc, vf, bt, sl, max_q_len=new)
+    assert torch.equal(got, prefill_paged8(q, cu, kc, kf, vc, vf, bt, sl, max_q_len=new))
+    kval, vval = dequantize_paged8(kc, kf).double(), dequantize_paged8(vc, vf).double()
+    for s in {0, seqs // 2, seqs - 1}:
+        n = lens[s]
+        rows = slice(int(starts[s]), int(starts[s + 1]))
+        for h in {0, hkv * group - 1}:
+            k, v = (x[bt[s].long(), h // group].reshape(-1, 128)[:n] for x in (kval, vval))
+            sc = q[rows, h].double() @ k.T.contiguous() * SM
+            want = torch.softmax(sc + torch.triu(torch.full_like(sc, -math.inf), diagonal=1), -1) @ v
+            lim = bound(float(v.abs().max()), n, dtype, dtype, want.cpu().numpy())
+            assert np.all((got[rows, h].double() - want).abs().cpu().numpy() <= lim)

@@ -191,3 +191,17 @@ def test_c_plan_refusals():
         (dict(ring=0), -1), (dict(pout=0), -1), (dict(start=0), -1), (dict(slots=0), -1), (dict(ws=0), -5), (dict(ws=P + 8), -5),
         (dict(wsb=8), -5)])
     assert _lib.lib().tq_plan_step_workspace_bytes(-1) == 0
+
+
+def test_c_launch_limits():
+    """Calls whose launches would have 2^32 threads or more."""
+    order = ("q out kc vc bt lens cu ws wsb qst qsh ost osh ksb ksh vsb vsh blocks bts qd od enc seqs hq hkv dim block mb msl mq "
+             "flags sm zero").split()
+    f = dict(q=P, out=P, kc=P, vc=P, bt=P, lens=P, cu=P, ws=P, wsb=1 << 40, qst=1024, qsh=128, ost=1024, osh=128, ksb=4128, ksh=2064,
+             vsb=4128, vsh=2064, blocks=8, bts=4, qd=2, od=2, enc=1, seqs=1 << 18, hq=64, hkv=4, dim=128, block=16, mb=4, msl=64, mq=3,
+             flags=1, sm=1.0, zero=0)
+    refused("tq_kv8_decode", f, order, paged8._ATTN, [(dict(), -1)])
+    order = ("q k qo ko qst qsh kst ksh qost qosh kost kosh pos turns tokens dtype pd hq hk dim rot inter mag").split()
+    f = dict(q=P, k=P, qo=2 * P, ko=2 * P, qst=1024, qsh=128, kst=256, ksh=128, qost=1024, qosh=128, kost=256, kosh=128, pos=P, turns=P,
+             tokens=1 << 27, dtype=2, pd=3, hq=8, hk=2, dim=128, rot=128, inter=0, mag=1.0)
+    refused("tq_rope", f, order, rotation._ROPE, [(dict(), -1)])

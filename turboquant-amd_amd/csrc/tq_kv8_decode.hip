@@ -466,7 +466,8 @@ extern "C" int tq_kv8_decode(const tq_kv8_attn_args* a, tq_stream_t stream) {
     if (rc != TQ_OK) return rc;
     if (p.group > 16) return TQ_ERR_GQA;
     if (a->num_seqs == 0) return TQ_OK;
-    if (a->max_seq_len < 0 || (int64_t)a->num_seqs * a->num_q_heads > INT32_MAX) return TQ_ERR_INVALID_ARGUMENT;
+    // (a launch's threads stay below 2^32)
+    if (a->max_seq_len < 0 || (int64_t)a->num_seqs * a->num_q_heads > 0xffffff) return TQ_ERR_INVALID_ARGUMENT;
     if (!a->q || !a->out || !a->k_cache || !a->v_cache || (!a->block_tables && a->max_blocks_per_seq) || !a->seq_lens) return TQ_ERR_INVALID_ARGUMENT;
     const int64_t need = tq_kv8_decode_workspace_bytes(a->num_seqs, a->num_q_heads, a->num_kv_heads);
     if (!a->workspace || (uintptr_t)a->workspace % 256 || a->workspace_bytes < need) return TQ_ERR_WORKSPACE;

@@ -353,7 +353,7 @@ extern "C" int tq_kv8_update(const tq_kv8_update_args* a, tq_stream_t stream) {
     if (a->num_tokens * per_run <= 2048) p.window = 1;
     p.window_wg = per_run;
     const int64_t grid = (a->num_tokens + p.window - 1) / p.window * p.window_wg;
-    if (grid > 0x7fffffff) return TQ_ERR_INVALID_ARGUMENT;
+    if (grid > 0xffffff) return TQ_ERR_INVALID_ARGUMENT;  // (a launch's threads stay below 2^32)
     const void* kern = nullptr;
 #define TQ_K8U(E, D) \
     if (a->encoding == E && a->x_dtype == D) kern = (const void*)kv8_update_kernel<E, D>;

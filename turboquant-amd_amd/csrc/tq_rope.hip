@@ -203,7 +203,7 @@ extern "C" int tq_rope(const tq_rope_args* a, tq_stream_t stream) {
     p.split = (int)split;
     const int64_t units = a->num_tokens * split;
     const int64_t grid = (units + kWaves - 1) / kWaves;
-    if (grid > 0x7fffffff) return TQ_ERR_INVALID_ARGUMENT;
+    if (grid > 0xffffff) return TQ_ERR_INVALID_ARGUMENT;  // (a launch's threads stay below 2^32)
     const void* kern = (const void*)rope_any_kernel;
     if (wide) {
 #define TQ_ROPE(D) \
