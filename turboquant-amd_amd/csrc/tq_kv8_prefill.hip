@@ -19,13 +19,15 @@
 // them.  (A workgroup's four waves on one segment, joined in LDS, leave a quarter of the pieces: 300 new after 2000
 // tokens 58 -> 49 us, but 8 prompts of 900 to 1300 tokens 161 -> 290 and the six long extends 145 -> 147.)
 //
-// Bound: issue.  4 x 4096 tokens of 48 / 8 heads, 0.82 TFLOP, in 860 us, 0.96 PFLOP/s, where a large fp16 matrix product
-// reaches 1.25.  Of a step's time the matrix unit works 44 % and the vector unit 56 % (per step 32 products, 64
-// conversions, 32 exponentials with their scaling, 16 packings, 16 sums): two waves per SIMD do not overlap more.  Without
-// the loads of K and V a step takes 9 % less, without the LDS reads 4.5 %, without the exponentials 5 %.  Tried
-// and slower: 32 rows a wave (1180 us, two or three waves per SIMD), products ordered among the exponentials by
-// hand (1130, spills), the same with one wave per SIMD (1540), a barrier per step so that a workgroup's waves
-// share L1 (+ 3 %).  Calls of few tokens: 20 us of start-up (search, query rows, first loads) and merge.
+// Bound: the vector port, which products and vector instructions share.  4 x 4096 tokens of 48 / 8 heads, 0.82 TFLOP, take
+// 860 us, 0.96 PFLOP/s, where a large fp16 matrix product reaches 1.25.  A step has 32 products and some 204 vector
+// instructions (64 conversions, 32 exponentials with their scaling, 16 packings, 16 sums): matrix unit 46 % busy, vector
+// unit 58 %.  Without the loads of K and V a step takes 9 % less, without the LDS reads 4.5 %, without the
+// exponentials 5 %.  Tried and slower: 32 rows a wave (1180 us, two or three waves per SIMD), products ordered
+// among the exponentials by hand (1130, spills), the same with one wave per SIMD (1540), a barrier per step so that a
+// workgroup's waves share L1 (+ 3 %), a SIMD's two waves in turn by barriers (1115); raised priority around the
+// products gives 0.7 % here and costs 4 x 2048 tokens 7 %.  Calls of few tokens: 20 us of start-up (search, query
+// rows, first loads) and merge.
 #include "tq_kv8.h"
 
 namespace {
