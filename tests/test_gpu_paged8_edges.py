@@ -201,3 +201,34 @@ def test_prefill_prompts(dev, dtype, seqs, new, hkv, group):
             want = torch.softmax(sc + torch.triu(torch.full_like(sc, -math.inf), diagonal=1), -1) @ v
             lim = bound(float(v.abs().max()), n, dtype, dtype, want.cpu().numpy())
             assert np.all((got[rows, h].double() - want).abs().cpu().numpy() <= lim)
+
+
+@pytest.mark.parametrize("dtype,seqs,new,past", [(torch.float32, 8, 2500, 0), (torch.bfloat16, 8, 2048, 0), (torch.bfloat16, 3, 333, 0),
+                                                 (torch.float16, 2, 200, 9000)])
+def test_prefill_nan_changes_nothing_else(dev, dtype, seqs, new, past):
+    """NaN against 0 in the same places of V, however the work is dealt: all other outputs keep their bits."""
+    g = torch.Generator(device=dev).manual_seed(past + new)
+    hkv, group, block, n = 4, 4, 16, past + new
+    width = -(-n // block)
+    kf, vf = formats("e4m3", block)
+    bt = torch.randperm(seqs * width, generator=torch.Generator().manual_seed(2)).to(torch.int32).to(dev).view(seqs, width)
+    t = torch.arange(n, device=dev)
+    slots = (bt.long()[:, t // block] * block + t % block).reshape(-1)
+    k, v = (torch.randn(seqs * n, hkv, 128, generator=g, device=dev) for _ in range(2))
+    at = [(s, past + int(f * (new - 1)), h, d) for s, f, h, d in ((0, 0.0, 0, 0), (0, 0.3, 1, 77), (1, 0.77, 3, 127), (seqs - 1, 1.0, 2, 64))]
+    outs = []
+    q = torch.randn(seqs * new, hkv * group, 128, generator=g, device=dev).to(dtype)
+    cu = torch.arange(0, seqs * new + 1, new, dtype=torch.int32, device=dev)
+    sl = torch.full((seqs,), n, dtype=torch.int32, device=dev)
+    for bad in (float("nan"), 0.0):
+        for s, p, h, d in at:
+            v[s * n + p, h, d] = bad
+        kc, vc = (allocate_cache(seqs * width, hkv, f, device=dev) for f in (kf, vf))
+        quantize_paged8_kv(k, v, slots, kc, vc, kf, vf)
+        outs.append(prefill_paged8(q, cu, kc, kf, vc, vf, bt, sl, max_q_len=new))
+    want = outs[1].clone().view(seqs, new, hkv, group, 128)
+    for s, p, h, d in at:
+        want[s, p - past:, h, :, d] = float("nan")
+    want = want.view_as(outs[0])
+    assert torch.equal(torch.isnan(outs[0]), torch.isnan(want))
+    assert torch.equal(torch.nan_to_num(outs[0]), torch.nan_to_num(want))
