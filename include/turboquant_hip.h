@@ -523,8 +523,8 @@ int tq_kv8_update(const tq_kv8_update_args* a, tq_stream_t stream);
  * q and the probabilities are taken as the sum of two fp16 numbers instead.
  * A row that sees no token gives 0, as do rows of sequences of length 0.  NaN in K or V reaches the rows
  * that see its token and no others.  V enters relative to the largest scale so far of the tokens in
- * order: a block whose scale is below 2^-24 of that counts as zeros, above 2^-15 of it it is exact.  |V|
- * stays below 2^80 (the sums of a sequence that is cut over the device are not yet divided).
+ * order: a block whose scale is below 2^-24 of that counts as zeros, above 2^-15 of it it is exact.  V may have any
+ * finite values (where every scale is below 2^-80, the outputs lose bits to fp32's subnormal numbers).
  * Block-table entries outside [0, num_blocks) mask their tokens.  Query rows outside every sequence are
  * not written.  Sequences longer than the block table (decode: than max_seq_len) or than 0x7fff0000
  * tokens are cut there.  cu_seqlens_q ascends from 0 or more to at most T; max_q_len >= every n.

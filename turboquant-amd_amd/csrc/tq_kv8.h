@@ -89,7 +89,7 @@ struct Kv8Attn {
     tq_udiv group_div;
     int tpb, group, cap;  // cap: tokens a block table can hold
     int workers;          // at most
-    float* ws_acc;        // [slot][row][128]
+    float* ws_acc;        // [slot][row][128]: a piece's output, divided by its sum
     float* ws_ml;         // [slot][row][2]: exponent base (log2), sum
     int* ends;            // decode: [segment][2], the waves with its first and its last step
 };
@@ -204,6 +204,37 @@ __device__ __forceinline__ tq_half8 kv8_half8(uint32_t a, uint32_t b, float sa, 
     const kv8_half2 x0 = Kv8Code<ENC>::half2(a, 0, sa), x1 = Kv8Code<ENC>::half2(a, 1, sa);
     const kv8_half2 x2 = Kv8Code<ENC>::half2(b, 0, sb), x3 = Kv8Code<ENC>::half2(b, 1, sb);
     return tq_half8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+}
+
+// N more pieces of a cut segment into the running mean a with exponent base M (none yet: -inf) and sum l; a piece has base
+// mp (-inf: no piece), sum lp and mean v; Mn is the largest of all bases
+template <int N>
+__device__ __forceinline__ void kv8_join(float& M, float& l, float4& a, float Mn, const float (&mp)[N], const float (&lp)[N],
+                                         const float4 (&v)[N]) {
+    float w[N];
+    l *= M == kKv8NegInf ? 0.f : __builtin_amdgcn_exp2f(M - Mn);
+    float sum = l;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        w[k] = mp[k] == kKv8NegInf ? 0.f : __builtin_amdgcn_exp2f(mp[k] - Mn) * lp[k];
+        sum += w[k];
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const float keep = l * inv;
+    a.x *= keep;
+    a.y *= keep;
+    a.z *= keep;
+    a.w *= keep;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const float f = w[k] * inv;
+        a.x = __builtin_fmaf(f, v[k].x, a.x);
+        a.y = __builtin_fmaf(f, v[k].y, a.y);
+        a.z = __builtin_fmaf(f, v[k].z, a.z);
+        a.w = __builtin_fmaf(f, v[k].w, a.w);
+    }
+    M = Mn;
+    l = sum;
 }
 
 // The word's bytes of the first n of its four tokens

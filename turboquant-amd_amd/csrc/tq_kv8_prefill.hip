@@ -605,7 +605,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                 const float l = lsum[rt] + __shfl_xor(lsum[rt], 32, 64);
                 int i, head;
                 row_of(rt, i, head);
-                const float f = complete ? (l == 0.f ? 0.f : kv8_scale(vref) / l) : kv8_scale(vref);
+                // (a piece is divided by its own sum: plain sums of large values pass fp32's range)
+                const float f = l == 0.f ? 0.f : kv8_scale(vref) / l;
                 if (i < computed) {
                     const int64_t row = (int64_t)(2 * w + (seg > p0 ? 1 : 0)) * kRows + 32 * rt + n;
                     const int64_t at = complete ? (int64_t)(q.q0 + i) * a.out_stride_token + (int64_t)head * a.out_stride_head : row * TQ_HEAD_DIM;
@@ -672,7 +673,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
 // Joins the pieces of the segments that several workers share: workgroup (w - 1, y) takes the segment that worker
 // w's record names; 32 lanes per row (4 dims each), 8 rows, 8 pieces requested together.  Every piece
 // holds at least one step: a worker's range is at least kMinTokens long.
-// out = sum_i 2^(M_i - M) acc_i / sum_i 2^(M_i - M) l_i.
+// out = sum_i w_i out_i / sum_i w_i, w_i = 2^(M_i - M) l_i, as a running mean, which stays within the values' range.
 __global__ __launch_bounds__(256) void kv8_prefill_merge_kernel(Prefill p) {
     const int w = (int)blockIdx.x + 1;
     if (w >= p.cuts[0].rb) return;
@@ -705,25 +706,9 @@ __global__ __launch_bounds__(256) void kv8_prefill_merge_kernel(Prefill p) {
         float Mn = M;
 #pragma unroll
         for (int k = 0; k < 8; ++k) Mn = fmaxf(Mn, mp[k]);
-        const float f = M == kKv8NegInf ? 0.f : __builtin_amdgcn_exp2f(M - Mn);
-        l *= f;
-        a.x *= f;
-        a.y *= f;
-        a.z *= f;
-        a.w *= f;
-        M = Mn;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            const float e = mp[k] == kKv8NegInf ? 0.f : __builtin_amdgcn_exp2f(mp[k] - M);
-            l = __builtin_fmaf(e, lp[k], l);
-            a.x = __builtin_fmaf(e, v[k].x, a.x);
-            a.y = __builtin_fmaf(e, v[k].y, a.y);
-            a.z = __builtin_fmaf(e, v[k].z, a.z);
-            a.w = __builtin_fmaf(e, v[k].w, a.w);
-        }
+        kv8_join<8>(M, l, a, Mn, mp, lp, v);
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const float o[4] = {a.x * inv, a.y * inv, a.z * inv, a.w * inv};
+    const float o[4] = {a.x, a.y, a.z, a.w};
     const int head = cut.kh * p.at.group + (int)(row - (uint32_t)i * (uint32_t)p.at.group);
     kv8_store<4>(args.out, (int64_t)(cut.q0 + i) * args.out_stride_token + (int64_t)head * args.out_stride_head + 4 * l32, args.out_dtype, o);
 }
