@@ -519,7 +519,8 @@ int tq_kv8_update(const tq_kv8_update_args* a, tq_stream_t stream);
  * query i of n sees the tokens t <= seq_lens[s] - n + i, without it all of them.
  *   out = sum_t softmax_t(sm_scale * q . k_t) v_t,  k_t, v_t = code * scale
  * with fp32 (or exact) sums.  q is scaled by a power of two per row to fp16 range and K is exact in
- * fp16; the probabilities are rounded to fp16 before the product with V.  With q or out of type TQ_F32
+ * fp16; the probabilities are rounded to fp16 before the product with V: to 11 bits where they are at least
+ * 2^-28 (prefill: 2^-18) of the row's largest, to 0 below 2^-39 (2^-29) of it.  With q or out of type TQ_F32
  * q and the probabilities are taken as the sum of two fp16 numbers instead.
  * A row that sees no token gives 0, as do rows of sequences of length 0.  NaN in K or V reaches the rows
  * that see its token and no others.  V enters relative to the largest scale so far of the tokens in

@@ -1,9 +1,11 @@
-"""8-bit paged attention at the ends of its number ranges: values far from 1."""
+"""8-bit paged attention at the ends of its number ranges: many small probabilities, values far from 1."""
+
+import math
 
 import pytest
 import torch
 
-from test_gpu_paged8 import bound
+from test_gpu_paged8 import HALF, bound
 from test_gpu_paged8_edges import causal64, filled
 from turboquant.kernels.paged8 import decode_paged8, prefill_paged8
 
@@ -19,6 +21,55 @@ def attend(entry, q, args, seqs, n, **kw):
         return decode_paged8(q, kc, kf, vc, vf, bt, sl, **kw)
     cu = torch.arange(0, q.shape[0] + 1, q.shape[0] // seqs, dtype=torch.int32, device=q.device)
     return prefill_paged8(q, cu, kc, kf, vc, vf, bt, sl, **kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("entry,down", [("decode", 26.5), ("decode", 20.5)])
+@pytest.mark.parametrize("seqs,at", [(1, 15000), (512, 0), (512, 15000)])
+def test_small_probabilities_add_up(dev, entry, down, code, dtype, seqs, at):
+    """One token's probability is 2^down times that of each of 29999 others, which alone have values in dims 64 and up:
+    outputs there are the sum of the small ones.  (512 sequences of 4 heads: a wave has all tokens of one.)
+
+    All small probabilities are one number; as normal fp16 numbers they are off by 2^-11 of it, the large one by as
+    much.  Scores are single products, exact but for three factors' roundings: 27 * 2^-22 in log2 units, below 2^-17.  A
+    wave adds its at most 940 steps one after the other, 940 * 2^-24 of rounding at most in either sum, or 470 waves'
+    pieces are joined: below 2^-13 together.  Then the output's own rounding."""
+    n = 30000
+    k, v = (torch.zeros(n, 4, 128, device=dev) for _ in range(2))
+    k[at, :, 9] = 1.0
+    v[:, :, 64:] = 1.0
+    v[at] = 0.0
+    v[at, :, :64] = 1.0
+    args, _, _ = filled(k, v, code, 16, dev)
+    q = torch.zeros(seqs, 4, 128, dtype=dtype, device=dev)
+    q[..., 9] = 1.0
+    got = attend(entry, q, args, seqs, n, sm_scale=down * math.log(2)).double()
+    tail = (n - 1) * 2.0 ** -down
+    want = torch.full((128,), 1 / (1 + tail), dtype=torch.float64, device=dev)
+    want[64:] = tail / (1 + tail)
+    lim = want * (2 * 2.0 ** -11 + 2.0 ** -13 + 2.0 ** -17 + HALF[dtype])
+    assert torch.all((got - want).abs() <= lim), float(((got - want).abs() / want).max())
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("entry", ["decode"])
+def test_small_probabilities_in_fp32(dev, entry, code):
+    """As above in fp32, where a probability is the sum of two fp16 numbers: off by half of their smallest step, 2^-25,
+    with the largest at 2^10 or more.  The small ones are 2^-18 of that, half a step between two numbers of a scale with the
+    largest at 2^4: 2^-18 of them.  Scores: 19 * 2^-22, below 2^-17.  125 steps' sums, twice: 2^-16.  The fp32 output."""
+    n, seqs, down = 4000, 512, 28 - math.log2(1000.5)
+    k, v = (torch.zeros(n, 4, 128, device=dev) for _ in range(2))
+    k[0, :, 9] = 1.0
+    v[:, :, 64:] = 1.0
+    v[0] = 0.0
+    args, _, _ = filled(k, v, code, 16, dev)
+    q = torch.zeros(seqs, 4, 128, device=dev)
+    q[..., 9] = 1.0
+    got = attend(entry, q, args, seqs, n, sm_scale=down * math.log(2)).double()[..., 64:]
+    tail = (n - 1) * 2.0 ** -down
+    want = tail / (1 + tail)
+    assert float((got / want - 1).abs().max()) <= 2.0 ** -18 + 2.0 ** -17 + 2.0 ** -16 + 2.0 ** -24
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])

@@ -32,6 +32,10 @@ constexpr int kTiles = 2;
 constexpr int kWavesPerCu = 8;
 constexpr int kMaxWorkers = 256 * kWavesPerCu;
 constexpr int kMinSteps = 2;     // steps a wave takes at least (1 x 4099 tokens: 1 18.2 us, 2 16.9, 4 16.9, 8 18.9)
+// A row's exponent base lies kUp below its largest score so far: as fp16 numbers the probabilities then keep 11 bits down
+// to 2^-28 of the largest, and count as zero only below 2^-39 of it (with the base at the largest: 2^-14 and 2^-25; a long tail
+// of small ones was lost).
+constexpr float kUp = 14.f;
 
 __device__ __forceinline__ int steps_of(const Kv8Attn& p, int s) {
     int L = p.a.seq_lens[s];
@@ -197,7 +201,7 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
             load_values(b, kTiles * j0);
         }
 
-        float M = kKv8None, lsum = 0.f, vref = 0.f;
+        float M = kKv8None, base = kKv8None, lsum = 0.f, vref = 0.f;  // largest score so far, M - kUp
         tq_floatx4 acc[8];
 #pragma unroll
         for (int a = 0; a < 8; ++a) acc[a] = tq_floatx4{0.f, 0.f, 0.f, 0.f};
@@ -264,6 +268,7 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
 #pragma unroll
                 for (int a = 0; a < 8; ++a) acc[a] *= alpha;
                 M = Mn;
+                base = Mn - kUp;
             }
             if (vmax > vref) {  // wave-uniform
                 const float f = vref / vmax;
@@ -276,7 +281,7 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
             for (int h = 0; h < kTiles; h += 2) {
                 float pr[8];
 #pragma unroll
-                for (int r = 0; r < 8; ++r) pr[r] = __builtin_amdgcn_exp2f(sv[4 * h + r] - M);
+                for (int r = 0; r < 8; ++r) pr[r] = __builtin_amdgcn_exp2f(sv[4 * h + r] - base);
                 tq_half8 ph, pl;
                 kv8_prob8<FINE>(pr, ph, pl);
                 lsum += kv8_sum8<FINE>(pr, ph);
