@@ -521,7 +521,8 @@ int tq_kv8_update(const tq_kv8_update_args* a, tq_stream_t stream);
  * with fp32 (or exact) sums.  q is scaled by a power of two per row to fp16 range and K is exact in
  * fp16; the probabilities are rounded to fp16 before the product with V: to 11 bits where they are at least
  * 2^-28 (prefill: 2^-18) of the row's largest, to 0 below 2^-39 (2^-29) of it.  With q or out of type TQ_F32
- * q and the probabilities are taken as the sum of two fp16 numbers instead.
+ * q and the probabilities are taken as the sum of two fp16 numbers instead, which resolves 2^-35 of a row's
+ * largest probability or finer.
  * A row that sees no token gives 0, as do rows of sequences of length 0.  NaN in K or V reaches the rows
  * that see its token and no others.  V enters relative to the largest scale so far of the tokens in
  * order: a block whose scale is below 2^-24 of that counts as zeros, above 2^-15 of it it is exact.  V may have any

@@ -25,7 +25,7 @@ def attend(entry, q, args, seqs, n, **kw):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("code", ["e4m3", "int8"])
-@pytest.mark.parametrize("entry,down", [("decode", 26.5), ("decode", 20.5)])
+@pytest.mark.parametrize("entry,down", [("decode", 26.5), ("decode", 20.5), ("prefill", 17.5)])
 @pytest.mark.parametrize("seqs,at", [(1, 15000), (512, 0), (512, 15000)])
 def test_small_probabilities_add_up(dev, entry, down, code, dtype, seqs, at):
     """One token's probability is 2^down times that of each of 29999 others, which alone have values in dims 64 and up:
@@ -53,7 +53,7 @@ def test_small_probabilities_add_up(dev, entry, down, code, dtype, seqs, at):
 
 
 @pytest.mark.parametrize("code", ["e4m3", "int8"])
-@pytest.mark.parametrize("entry", ["decode"])
+@pytest.mark.parametrize("entry", ["decode", "prefill"])
 def test_small_probabilities_in_fp32(dev, entry, code):
     """As above in fp32, where a probability is the sum of two fp16 numbers: off by half of their smallest step, 2^-25,
     with the largest at 2^10 or more.  The small ones are 2^-18 of that, half a step between two numbers of a scale with the

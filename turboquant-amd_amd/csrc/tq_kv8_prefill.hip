@@ -43,11 +43,16 @@ constexpr int kMinTokens = 128;    // stream tokens a worker takes at least (32 
 constexpr int kSegTokens = 480;
 // The cut pieces' set-up and their merge in tokens (1500: 8 to 40 new after 100 to 700 of 32 sequences 50.5 -> 53.6 us)
 constexpr int kMergeTokens = 384;
-// A row's exponent base lies kDown below the largest score of the step that set it, and moves only when a lane's
-// 16 probabilities of a step sum to more than kMoveSum: no maximum is worked out otherwise, and fp16's normal range
-// reaches from 2^14 above the base to 2^-14 below it.
-constexpr float kDown = 4.f;
-constexpr float kMoveSum = 16384.f;
+// A row's exponent base lies `down` below the largest score of the step that set it, and moves only when a lane's
+// 16 probabilities of a step sum to more than move_sum: no maximum is worked out otherwise, and fp16's normal range
+// reaches from 2^15 above the base to 2^-14 below it.  In 16 bits the largest probability is thus 2^4 or more, and one
+// below 2^-18 of it loses bits; FINE, whose two numbers resolve 2^-25, has it at 2^10 or more.  (The lower base moves
+// more often: 4 x 4096 tokens in f32 1533 -> 1547 us; in bf16 it would take 883 -> 901.)
+template <bool FINE>
+struct Base {
+    static constexpr float down = FINE ? 10.f : 4.f;
+    static constexpr float move_sum = FINE ? 32768.f : 16384.f;
+};
 constexpr int kFirst = 2;          // query operands that stay in registers (1 .. 4: 4 x 4096 tokens 910, 906, 920, 921 us)
 
 struct Cut {  // a segment that several workers share
@@ -555,14 +560,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                             return sum[0] + sum[1];
                         };
                         float sum = probabilities();
-                        if (__builtin_amdgcn_ballot_w64(sum > kMoveSum)) {
+                        if (__builtin_amdgcn_ballot_w64(sum > Base<FINE>::move_sum)) {
                             float mt[2];
 #pragma unroll
                             for (int t = 0; t < 2; ++t)
                                 mt[t] = fmaxf(fmaxf(fmaxf(sc[rt][8 * t], sc[rt][8 * t + 1]), fmaxf(sc[rt][8 * t + 2], sc[rt][8 * t + 3])),
                                               fmaxf(fmaxf(sc[rt][8 * t + 4], sc[rt][8 * t + 5]), fmaxf(sc[rt][8 * t + 6], sc[rt][8 * t + 7])));
                             const float mx = fmaxf(mt[0] * f[0], mt[1] * f[1]);
-                            const float Mn = fmaxf(M[rt], fmaxf(mx, __shfl_xor(mx, 32, 64)) - kDown);
+                            const float Mn = fmaxf(M[rt], fmaxf(mx, __shfl_xor(mx, 32, 64)) - Base<FINE>::down);
                             const float alpha = __builtin_amdgcn_exp2f(M[rt] - Mn);
                             lsum[rt] *= alpha;
 #pragma unroll
