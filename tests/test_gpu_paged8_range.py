@@ -104,3 +104,31 @@ def test_sums_of_large_values(dev, entry, code, dtype, seqs, power):
     got = attend(entry, q, args, seqs, n).double().cpu().numpy()
     want = vval.mean(0).cpu().numpy()[None]
     assert (abs(got - want) <= bound(float(vval.abs().max()), n, dtype, dtype, want)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("entry", ["decode", "prefill"])
+@pytest.mark.parametrize("power", [20, 21, 22, 23, 24, 25, 26, 27, 28, 30, 40, 70, 110, 120])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_any_size(dev, entry, code, dtype, power, sign):
+    """Scores of about 2^power in log2 units, of either sign, whose largest several tokens share: the mean of these tokens' values.
+    (The others lie 2^-6 of that lower, 2^14 in log2 units and more, so that nothing of them is left.)  A short sequence, and
+    a cut one with the largest in its middle and at its end."""
+    g = torch.Generator(device=dev).manual_seed(power)
+    for n, at in ((70, (3, 40, 69)), (5000, (2100, 2111, 4999)), (70, (0, 1))):
+        k = torch.zeros(n, 2, 128, device=dev)
+        k[:, :, 9] = 1.0 if sign > 0 else 1.0 + 2.0 ** -2      # (exact in e4m3 and, with the block's scale, in int8)
+        for t in at:
+            k[t, :, 9] = 1.0 + 2.0 ** -2 if sign > 0 else 1.0
+        k *= sign * 2.0 ** (power // 2)
+        v = torch.randn(n, 2, 128, generator=g, device=dev)
+        args, kval, vval = filled(k, v, code, 16, dev)
+        assert torch.equal(kval, k.double())
+        q = torch.zeros(1, 8, 128, dtype=dtype, device=dev)
+        # seven bits of mantissa, other ones in each head
+        q[..., 9] = (1.0 + torch.arange(8, device=dev) * 15 / 128) * 2.0 ** (power - power // 2)
+        got = attend(entry, q, args, 1, n, sm_scale=1.0 / 1.7).double()
+        want = vval[list(at)].mean(0).repeat_interleave(4, 0)[None].cpu().numpy()
+        lim = bound(float(vval.abs().max()), n, dtype, dtype, want)
+        assert (abs(got.cpu().numpy() - want) <= lim).all(), n

@@ -79,7 +79,8 @@ __device__ __forceinline__ float kv8_exp2i(int e) { return __uint_as_float((uint
 
 // ---- attention over the tiles: what the decode and prefill kernels share ----
 constexpr float kKv8NegInf = -__builtin_huge_valf();
-constexpr float kKv8None = -1e30f;  // exponent base of a row that has seen no token
+constexpr float kKv8None = -3.4e38f;  // exponent base of a row that has seen no token
+constexpr float kKv8Far = 4194304.f;  // 2^22: scores from here on have no room for a base beside the largest one
 constexpr int kKv8MaxLen = 0x7fff0000;  // tokens of a sequence
 constexpr float kKv8Log2e = 1.4426950408889634f;
 

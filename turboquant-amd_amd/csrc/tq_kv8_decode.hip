@@ -201,7 +201,7 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
             load_values(b, kTiles * j0);
         }
 
-        float M = kKv8None, base = kKv8None, lsum = 0.f, vref = 0.f;  // largest score so far, M - kUp
+        float M = kKv8None, base = kKv8None, lsum = 0.f, vref = 0.f;  // M: largest score so far
         tq_floatx4 acc[8];
 #pragma unroll
         for (int a = 0; a < 8; ++a) acc[a] = tq_floatx4{0.f, 0.f, 0.f, 0.f};
@@ -263,12 +263,13 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
             for (int h = 1; h < kTiles; ++h) vmax = fmaxf(vmax, vs[h]);
             if (__builtin_amdgcn_ballot_w64(mx > M)) {
                 const float Mn = fmaxf(M, tq_max_over_groups(mx));
-                const float alpha = __builtin_amdgcn_exp2f(M - Mn);
+                const float bn = __builtin_fabsf(Mn) < kKv8Far ? Mn - kUp : Mn;
+                const float alpha = __builtin_amdgcn_exp2f(base - bn);
                 lsum *= alpha;
 #pragma unroll
                 for (int a = 0; a < 8; ++a) acc[a] *= alpha;
                 M = Mn;
-                base = Mn - kUp;
+                base = bn;
             }
             if (vmax > vref) {  // wave-uniform
                 const float f = vref / vmax;
@@ -320,7 +321,7 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
                 kv8_store<16>(complete ? p.a.out : (void*)p.ws_acc, at + 64 * k + 16 * g, complete ? p.a.out_dtype : TQ_F32, o[k]);
             if (!complete) {
                 if (g == 0) {
-                    p.ws_ml[2 * row] = M;
+                    p.ws_ml[2 * row] = base;
                     p.ws_ml[2 * row + 1] = l;
                 }
             }
@@ -372,7 +373,7 @@ __global__ __launch_bounds__(256) void kv8_decode_merge_kernel(Kv8Attn p) {
             v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (wk <= w1) {
                 const int64_t row = (wk + seg) * p.group + r;
-                mp[k] = fmaxf(p.ws_ml[2 * row], kKv8None);  // (also where M is NaN)
+                mp[k] = p.ws_ml[2 * row];
                 lp[k] = p.ws_ml[2 * row + 1];
                 v[k] = *reinterpret_cast<const float4*>(p.ws_acc + row * TQ_HEAD_DIM + 4 * l32);
             }

@@ -275,6 +275,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
     // taken while the one at hand is worked on.
     __shared__ int s_nan[kWaves];  // a NaN among the values of the segment's edge steps
     if (lane == 0) s_nan[wave] = 0;
+    // the exponent base of rows whose scores lie beyond kKv8Far: their M stays kKv8None, so that every step moves it
+    __shared__ float s_base[kWaves][kRT][64];
     __shared__ int s_ticket[2][2];  // pair (-1: none left), row blocks from the last
     const int pairs = a.num_seqs * hkv;
     const int turns = (most_rb + kWaves - 1) / kWaves;
@@ -428,6 +430,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
             };
 
             float M[kRT], lsum[kRT];
+            bool far = false;  // s_base holds the rows' bases
             int vref = 0;  // exponent + 127 of the largest V scale so far (0: none)
             f32x16 acc[kRT][4];
 #pragma unroll
@@ -546,34 +549,58 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
 #pragma unroll
                     for (int rt = 0; rt < kRT; ++rt) {
                         // (over zero, so that a masked score stays -inf)
-                        const float f[2] = {fmaxf(c1[rt] * kv8_scale(ke[0]), 1e-37f), fmaxf(c1[rt] * kv8_scale(ke[1]), 1e-37f)};
-                        auto probabilities = [&]() -> float {
+                        float f[2] = {fmaxf(c1[rt] * kv8_scale(ke[0]), 1e-37f), fmaxf(c1[rt] * kv8_scale(ke[1]), 1e-37f)};
+                        auto probabilities = [&](float base) -> float {
                             float sum[2];
 #pragma unroll
                             for (int t = 0; t < 2; ++t) {
                                 float pr[8];
 #pragma unroll
-                                for (int v = 0; v < 8; ++v) pr[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rt][8 * t + v], f[t], -M[rt]));
+                                for (int v = 0; v < 8; ++v) pr[v] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[rt][8 * t + v], f[t], -base));
                                 kv8_prob8<FINE>(pr, ph[rt][t], pl[FINE ? rt : 0][t]);
                                 sum[t] = kv8_sum8<FINE>(pr, ph[rt][t]);
                             }
                             return sum[0] + sum[1];
                         };
-                        float sum = probabilities();
-                        if (__builtin_amdgcn_ballot_w64(sum > Base<FINE>::move_sum)) {
+                        float sum = probabilities(M[rt]);
+                        if (__builtin_expect(__builtin_amdgcn_ballot_w64(sum > Base<FINE>::move_sum) != 0, 0)) {
                             float mt[2];
 #pragma unroll
                             for (int t = 0; t < 2; ++t)
                                 mt[t] = fmaxf(fmaxf(fmaxf(sc[rt][8 * t], sc[rt][8 * t + 1]), fmaxf(sc[rt][8 * t + 2], sc[rt][8 * t + 3])),
                                               fmaxf(fmaxf(sc[rt][8 * t + 4], sc[rt][8 * t + 5]), fmaxf(sc[rt][8 * t + 6], sc[rt][8 * t + 7])));
                             const float mx = fmaxf(mt[0] * f[0], mt[1] * f[1]);
-                            const float Mn = fmaxf(M[rt], fmaxf(mx, __shfl_xor(mx, 32, 64)) - Base<FINE>::down);
-                            const float alpha = __builtin_amdgcn_exp2f(M[rt] - Mn);
+                            const float top = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                            float old = M[rt];
+                            if (far && old == kKv8None) old = s_base[wave][rt][lane];
+                            const float Mn = fmaxf(old, __builtin_fabsf(top) < kKv8Far ? top - Base<FINE>::down : top);
+                            const float alpha = __builtin_amdgcn_exp2f(old - Mn);
                             lsum[rt] *= alpha;
 #pragma unroll
                             for (int d = 0; d < 4; ++d) acc[rt][d] *= alpha;
                             M[rt] = Mn;
-                            sum = probabilities();
+                            float base = Mn;
+                            if (far || __builtin_amdgcn_ballot_w64(!(__builtin_fabsf(Mn) < kKv8Far) && Mn != kKv8None)) {
+                                if (!far) {
+#pragma unroll
+                                    for (int r = 0; r < kRT; ++r) s_base[wave][r][lane] = M[r];
+                                    far = true;
+                                }
+                                // far scores are rounded as their base was: what fp32 drops of a product may be many units
+                                s_base[wave][rt][lane] = Mn;
+                                if (!(__builtin_fabsf(Mn) < kKv8Far)) {
+#pragma unroll
+                                    for (int v = 0; v < 16; ++v) {
+                                        float x = sc[rt][v] * f[v >> 3];
+                                        asm("" : "+v"(x));  // (kept from becoming a fused step)
+                                        sc[rt][v] = x - Mn;
+                                    }
+                                    f[0] = f[1] = 1.f;
+                                    base = 0.f;
+                                    M[rt] = kKv8None;
+                                }
+                            }
+                            sum = probabilities(base);
                         }
                         lsum[rt] += sum;
                     }
@@ -627,7 +654,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                         kv8_store<16>(dst, at + 32 * k + 16 * h, dt, o);
                     }
                     if (!complete && h == 0) {
-                        p.at.ws_ml[2 * row] = M[rt];
+                        p.at.ws_ml[2 * row] = far && M[rt] == kKv8None ? s_base[wave][rt][lane] : M[rt];
                         p.at.ws_ml[2 * row + 1] = l;
                     }
                 }
@@ -703,7 +730,7 @@ __global__ __launch_bounds__(256) void kv8_prefill_merge_kernel(Prefill p) {
             v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (wk <= cut.w1) {
                 const int64_t x = (int64_t)(wk == cut.w0 ? cut.slot0 : 2 * wk) * p.rows + r0;
-                mp[k] = fmaxf(p.at.ws_ml[2 * x], kKv8None);  // (also where M is NaN)
+                mp[k] = p.at.ws_ml[2 * x];
                 lp[k] = p.at.ws_ml[2 * x + 1];
                 v[k] = *reinterpret_cast<const float4*>(p.at.ws_acc + x * TQ_HEAD_DIM + 4 * l32);
             }
