@@ -15,8 +15,8 @@ the hot path is here, in the shapes the reference's backends use:
   last `num_protected_layers` layers are not compressed (get_state returns None and the caller
   keeps its own attention for them, as the reference does), or, with `protected_bits`, get a
   4-bit (or other) packed format of their own, or with protected_bits=8 a cache of 8 bits a value.
-- TurboQuantPaged8State: the state of such a layer (kernels.paged8), with the same methods, so that
-  TurboQuantPagedImpl runs on either.
+- TurboQuantPaged8State: the state of such a layer, or of all with k_bits=8 (kernels.paged8), with the methods that
+  TurboQuantPagedImpl calls, so that it runs on either.
 - TurboQuantPagedImpl: an attention implementation in vLLM's shape
   (TurboQuantFP4Impl.do_kv_cache_update / forward and TurboQuantFP4Backend.get_kv_cache_shape,
   integration/tq_fp4_backend.py:389-735).  One uint8 tensor [num_blocks, num_kv_heads,
@@ -201,6 +201,11 @@ class TurboQuantPaged8State:
                               sm_scale=sm_scale, causal=causal, max_q_len=max_q_len, out=out)
 
 
+def _check_8bit(v_bits: Optional[int], k_qjl: bool) -> None:
+    if v_bits not in (None, 8) or k_qjl:
+        raise ValueError("an 8-bit cache has 8 bits on both sides and no QJL data")
+
+
 class TurboQuantPagedConfig:
     """Which layers are compressed, and with which formats.
 
@@ -208,13 +213,16 @@ class TurboQuantPagedConfig:
     compressed with the configured formats (integration/vllm_backend.py:266-278).  Their
     get_state is None (the caller's own attention, as in the reference) unless
     protected_bits is given: then they get k_bits = v_bits = protected_bits without QJL, and with
-    protected_bits=8 a TurboQuantPaged8State of protected_encoding ("e4m3" or "int8").
+    protected_bits=8 a TurboQuantPaged8State of protected_encoding ("e4m3" or "int8").  With k_bits=8 (v_bits None
+    or 8, no QJL) the other layers get one of `encoding`.
     """
 
     def __init__(self, head_size: int = 128, num_layers: int = 0, protect_boundary_layers: bool = True,
                  num_protected_layers: int = 2, k_bits: int = 4, v_bits: Optional[int] = None,
                  k_qjl: bool = False, block_size: int = 16, weights_fused: bool = False,
-                 protected_bits: Optional[int] = None, protected_encoding: str = "e4m3"):
+                 protected_bits: Optional[int] = None, protected_encoding: str = "e4m3", encoding: str = "e4m3"):
+        if k_bits == 8:
+            _check_8bit(v_bits, k_qjl)
         self.head_size = head_size
         self.num_layers = num_layers
         self.protect_boundary_layers = protect_boundary_layers
@@ -226,6 +234,7 @@ class TurboQuantPagedConfig:
         self.weights_fused = weights_fused
         self.protected_bits = protected_bits
         self.protected_encoding = protected_encoding
+        self.encoding = encoding
         self.layer_states: dict[int, TurboQuantPagedState | TurboQuantPaged8State] = {}
 
     def should_compress(self, layer_idx: int) -> bool:
@@ -241,10 +250,11 @@ class TurboQuantPagedConfig:
         protected = not self.should_compress(layer_idx)
         if protected and self.protected_bits is None:
             return None
-        if protected and self.protected_bits == 8:
+        if (self.protected_bits if protected else self.k_bits) == 8:
             if layer_idx not in self.layer_states:
-                self.layer_states[layer_idx] = TurboQuantPaged8State(self.head_size, layer_idx, device,
-                                                                     self.protected_encoding, self.block_size)
+                self.layer_states[layer_idx] = TurboQuantPaged8State(
+                    self.head_size, layer_idx, device, self.protected_encoding if protected else self.encoding,
+                    self.block_size)
             return self.layer_states[layer_idx]
         if layer_idx not in self.layer_states:
             if protected:
@@ -263,8 +273,8 @@ _tq_paged_config: Optional[TurboQuantPagedConfig] = None
 def get_tq_paged_config(head_size: int = 128, num_layers: int = 0, protect_boundary_layers: bool = True,
                         num_protected_layers: int = 2, k_bits: int = 4, v_bits: Optional[int] = None,
                         k_qjl: bool = False, block_size: int = 16, weights_fused: bool = False,
-                        protected_bits: Optional[int] = None,
-                        protected_encoding: str = "e4m3") -> TurboQuantPagedConfig:
+                        protected_bits: Optional[int] = None, protected_encoding: str = "e4m3",
+                        encoding: str = "e4m3") -> TurboQuantPagedConfig:
     """The process-wide config, created by the first call (later arguments are ignored, as in
     get_tq_fp8_config, integration/vllm_backend.py:295-337)."""
     global _tq_paged_config
@@ -273,7 +283,7 @@ def get_tq_paged_config(head_size: int = 128, num_layers: int = 0, protect_bound
             head_size=head_size, num_layers=num_layers, protect_boundary_layers=protect_boundary_layers,
             num_protected_layers=num_protected_layers, k_bits=k_bits, v_bits=v_bits, k_qjl=k_qjl,
             block_size=block_size, weights_fused=weights_fused, protected_bits=protected_bits,
-            protected_encoding=protected_encoding)
+            protected_encoding=protected_encoding, encoding=encoding)
     return _tq_paged_config
 
 
@@ -345,8 +355,7 @@ class TurboQuantPagedImpl:
         if head_size != 128:
             raise ValueError("head_size must be 128")
         if k_bits == 8:
-            if v_bits not in (None, 8) or k_qjl:
-                raise ValueError("an 8-bit cache has 8 bits on both sides and no QJL data")
+            _check_8bit(v_bits, k_qjl)
             return (num_blocks, num_kv_heads, 2 * Paged8Format(block_size=block_size).tile_bytes)
         kf = PagedKVFormat(bits=k_bits, qjl=k_qjl, block_size=block_size)
         vf = PagedKVFormat(bits=v_bits if v_bits is not None else k_bits, qjl=False, block_size=block_size,
