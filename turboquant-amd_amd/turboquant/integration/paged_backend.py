@@ -321,7 +321,11 @@ class PagedDecodeMetadata:
 
 
 class TurboQuantPagedImpl:
-    """Attention over a packed or 8-bit paged cache, in the shape of a vLLM AttentionImpl."""
+    """Attention over a packed or 8-bit paged cache, in the shape of a vLLM AttentionImpl.
+
+    sparse_threshold acts on packed caches; over an 8-bit one every token's values are read.  Decode takes up to 16
+    query heads per KV head on either, prefill any number.
+    """
 
     forward_includes_kv_cache_update = False  # do_kv_cache_update is called separately
 
