@@ -13,10 +13,11 @@
 //   O^T [dim 8m + a][head] += V^T . P^T    8 x mfma_f32_16x16x32_f16 per step, k = 8g + i being tokens 4g..4g+3 of A, then
 //                                          of B: what S^T leaves in the lane, and a word of the values layout each
 // One pass with the running maximum and sum of the softmax.  The tile's K scale goes into the score's
-// factor; V's scale, relative to the largest met so far, into the conversion to fp16, which is
-// exact (and the accumulators are rescaled when a larger one is met).
+// factor; V's scale, relative to the largest met so far, into the conversion to fp16, which is exact down to
+// 2^-15 of that, where codes pass below fp16's numbers, and gives zeros from 2^-24 on (the accumulators are rescaled
+// when a larger scale is met).
 //
-// Bound: HBM reads, 256 bytes per token and KV head: 64 x 32768 tokens of 8 heads in 759 us, 5.7 TB/s, where a large
+// Bound: HBM reads, 256 bytes per token and KV head: 64 x 32768 tokens of 8 heads in 762 us, 5.6 TB/s, where a large
 // copy moves 4.9.  Small calls: launches, start-up (the search for the wave's part, block table, scales) and
 // the merge, about 15 us.
 #include "tq_kv8.h"

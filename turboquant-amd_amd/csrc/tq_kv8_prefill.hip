@@ -19,11 +19,13 @@
 // them.  (A workgroup's four waves on one segment, joined in LDS, leave a quarter of the pieces: 300 new after 2000
 // tokens 58 -> 49 us, but 8 prompts of 900 to 1300 tokens 161 -> 290 and the six long extends 145 -> 147.)
 //
-// Bound: the vector port, which products and vector instructions share.  4 x 4096 tokens of 48 / 8 heads, 0.82 TFLOP, take
-// 860 us, 0.96 PFLOP/s, where a large fp16 matrix product reaches 1.25.  A step has 32 products and some 204 vector
-// instructions (64 conversions, 32 exponentials with their scaling, 16 packings, 16 sums): matrix unit 46 % busy, vector
-// unit 58 %.  Without the loads of K and V a step takes 9 % less, without the LDS reads 4.5 %, without the
-// exponentials 5 %.  Tried and slower: 32 rows a wave (1180 us, two or three waves per SIMD), products ordered
+// Bound: a SIMD's waves, whose products and vector instructions hardly overlap.  4 x 4096 tokens of 48 / 8 heads, 0.82
+// TFLOP, take 867 us, 0.95 PFLOP/s, where a large fp16 matrix product reaches 1.22.  A step has 32 products and, over a
+// whole launch, 245 other vector instructions (64 conversions, 64 of the exponentials and their scaling, 16 packings, 16
+// sums; the rest moves operands and addresses): matrix unit 46 % busy, vector unit 57 %, 6 % of it the products'
+// issue, 97 % together.  What keeps the two waves from overlapping more is open.  int8 takes 930 us (its conversions are
+// more instructions), f32 1549 (twice the products; int8 1664).  Without the loads of K and V a step takes 9 % less,
+// without the LDS reads 4.5 %, without the exponentials 5 %.  Tried and slower: 32 rows a wave (1180 us, two or three waves per SIMD), products ordered
 // among the exponentials by hand (1130, spills), the same with one wave per SIMD (1540), a barrier per step so that a
 // workgroup's waves share L1 (+ 3 %), a SIMD's two waves in turn by barriers (1115); raised priority around the
 // products gives 0.7 % here and costs 4 x 2048 tokens 7 %.  Calls of few tokens: 20 us of start-up (search, query
@@ -38,8 +40,8 @@ constexpr int kWaves = 4;          // of a workgroup
 constexpr int kWavesPerCu = 8;     // resident
 constexpr int kMaxWorkers = 256 * kWavesPerCu;
 constexpr int kMinTokens = 128;    // stream tokens a worker takes at least (32 or more: see the merge)
-// A segment's set-up (query loads, first steps, output) in tokens (160, 320, 480, 640: 8 prompts of 900 to 1300 tokens 195, 161,
-// 157, 157 us; 37 to 512 new after 1000 to 16000 of six sequences 147, 145, 145, 148)
+// A segment's set-up (query loads, first steps, output) in tokens (160, 320, 480, 640: 8 prompts of 900 to 1300 tokens 158, 158,
+// 158, 162 us; 37 to 512 new after 1000 to 16000 of six sequences 134, 130, 129, 133)
 constexpr int kSegTokens = 480;
 // The cut pieces' set-up and their merge in tokens (1500: 8 to 40 new after 100 to 700 of 32 sequences 50.5 -> 53.6 us)
 constexpr int kMergeTokens = 384;

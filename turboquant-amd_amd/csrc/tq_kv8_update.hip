@@ -347,7 +347,10 @@ extern "C" int tq_kv8_update(const tq_kv8_update_args* a, tq_stream_t stream) {
     Kv8Update p = {};
     p.a = *a;
     // A window of a block's length holds about one run of a prompt; single tokens of many sequences are a run
-    // each, and a window of one token gives each run's heads waves of their own.
+    // each, and a window of one token gives each run's heads waves of their own.  The host knows the tokens alone, not
+    // the runs: short calls are taken for single tokens, long ones for prompts.  At the rule's border, 1024 tokens of 8
+    // heads, a window of one and one of a block take 12.7 and 41 us (blocks of 64: 12.7 and 152) for single tokens, 13.1 and
+    // 6.0 (23.4 and 12.3) for a prompt; 8192 single tokens, a block's window each: 76 (182).
     const int per_run = (a->num_heads + kWaves - 1) / kWaves;
     p.window = a->block_size < 64 ? a->block_size : 64;
     if (a->num_tokens * per_run <= 2048) p.window = 1;

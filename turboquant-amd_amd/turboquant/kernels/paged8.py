@@ -227,9 +227,12 @@ def decode_paged8(
 
     block_tables int32 [S, max_blocks] (entries outside the cache mask their tokens), seq_lens int32 [S];
     max_seq_len: host-side bound of seq_lens (default: the tables' capacity; longer sequences are cut there).
-    Up to 16 query heads per KV head.  Output dtype = out.dtype or q.dtype; with f32 on either side the
-    operands are carried in twice the precision.  A sequence of length 0 gives zeros.  workspace: uint8 of
-    tq_kv8_decode_workspace_bytes(...) for callers that keep one (calls that overlap must not share it).
+    Up to 16 query heads per KV head.  Output dtype = out.dtype or q.dtype; a row's q and probabilities are rounded
+    to fp16 (probabilities below 2^-39 of the row's largest count as zero), with f32 on either side they are
+    carried in twice the precision.  V enters relative to the largest scale so far of the sequence's blocks: exact
+    down to 2^-15 of it, zero below 2^-24.  A sequence of length 0 gives zeros; a NaN in the cache reaches the
+    heads that see it.  workspace: uint8 of tq_kv8_decode_workspace_bytes(...) for callers that keep one (calls that
+    overlap must not share it).
     """
     dev = _lib.require_gpu("decode_paged8", q, k_cache, v_cache, block_tables, seq_lens, out, workspace)
     if q.dim() != 3 or q.shape[2] != 128:
@@ -267,7 +270,8 @@ def prefill_paged8(
     seq_lens - n + i, otherwise all of them; a row that sees none gives zeros, and NaN in the cache reaches
     the rows that see it alone.  Any number of query heads per KV head.
     max_q_len: host-side bound of the query counts (default: T).  Rows of q that belong to no sequence are
-    left as they were in out.  Types and workspace as in decode_paged8.
+    left as they were in out.  Types, roundings and workspace as in decode_paged8, but 16-bit calls round probabilities below
+    2^-18 of the row's largest to fewer bits and those below 2^-29 to zero.
     """
     dev = _lib.require_gpu("prefill_paged8", q, cu_seqlens_q, k_cache, v_cache, block_tables, seq_lens, out, workspace)
     if q.dim() != 3 or q.shape[2] != 128:
