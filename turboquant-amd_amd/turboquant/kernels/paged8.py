@@ -183,6 +183,8 @@ def _attention(name, dev, q, caches, k_cache, v_cache, k_fmt, block_tables, seq_
         return out
     target = out
     ot, oh, o1 = out.stride()
+    if (rows > 1 and not ot) or (hq > 1 and not oh):
+        raise ValueError("rows of out share memory")
     if o1 != 1 or (ot | oh) % 8 or out.data_ptr() % 16:
         # a destination that takes no vector stores gets a copy of the result (rows of no sequence stay as they were)
         target = out.clone(memory_format=torch.contiguous_format)

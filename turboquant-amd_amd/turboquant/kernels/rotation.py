@@ -71,6 +71,8 @@ def _rope_pair(x: torch.Tensor, out: Optional[torch.Tensor]):
         raise ValueError("destinations must have their input's shape and dtype")
     xt, xh, x1 = x.stride()
     ot, oh, o1 = out.stride()
+    if (not ot and out.shape[0] > 1) or (not oh and out.shape[1] > 1):
+        raise ValueError("rows of a destination share memory")
     dst = out
     if o1 != 1 or (out.data_ptr() == x.data_ptr() and (ot != xt or oh != xh)):
         dst = torch.empty_like(x, memory_format=torch.contiguous_format)
