@@ -132,3 +132,33 @@ def test_scores_of_any_size(dev, entry, code, dtype, power, sign):
         want = vval[list(at)].mean(0).repeat_interleave(4, 0)[None].cpu().numpy()
         lim = bound(float(vval.abs().max()), n, dtype, dtype, want)
         assert (abs(got.cpu().numpy() - want) <= lim).all(), n
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("past", [0, 6000])
+def test_far_and_near_scores_side_by_side(dev, code, dtype, past):
+    """Rows of ordinary scores among rows of far ones, which from token 32 on pass from the first kind to the second.  (Far scores leave the largest one alone: the bound's share for scores is
+    2^-24 of a score, and two of them lie that close in no row, as is checked.)"""
+    g = torch.Generator(device=dev).manual_seed(past + 3)
+    new = 75
+    k, v = (torch.randn(past + new, 2, 128, generator=g, device=dev) for _ in range(2))
+    k[:32] *= 2.0 ** -32
+    args, kval, vval = filled(k, v, code, 16, dev)
+    q = torch.randn(new, 8, 128, generator=g, device=dev)
+    far = torch.arange(new, device=dev) % 3 == 1
+    far[[40, 41, 42, 74]] = True
+    q[far] *= 2.0 ** 34
+    q = q.to(dtype)
+    for entry in ("prefill", "decode"):
+        if entry == "prefill":
+            got, want, n = attend(entry, q, args, 1, past + new), causal64(q, kval, vval, past), past + new
+            s = torch.matmul(q.double().transpose(0, 1), kval.repeat_interleave(4, 1).permute(1, 2, 0)) / math.sqrt(128)
+            s.masked_fill_(torch.arange(n, device=dev) > past + torch.arange(new, device=dev)[:, None], -math.inf)
+            top = s[:, far].topk(2, -1).values if past else s[:, far & (torch.arange(new, device=dev) > 33)].topk(2, -1).values
+            assert float((top[..., 0] - top[..., 1]).min()) > 2.0 ** 12
+        else:
+            row = q[-1:]
+            got, want = attend(entry, row, args, 1, past + new), causal64(row, kval, vval, past + new - 1)
+        w = want.cpu().numpy()
+        assert (abs(got.double().cpu().numpy() - w) <= bound(float(vval.abs().max()), past + new, dtype, dtype, w)).all()
