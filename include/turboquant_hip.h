@@ -561,6 +561,75 @@ int64_t tq_kv8_decode_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_
 int64_t tq_kv8_prefill_workspace_bytes(int num_seqs, int max_q_len, int num_q_heads, int num_kv_heads,
                                        int max_blocks_per_seq, int block_size);
 
+/*
+ * The same with a window, and weights accumulated for an eviction.
+ * window > 0: the query at position p of its sequence (decode: the last; prefill: seq_lens[s] - n + i) sees the tokens
+ * t <= p with t > p - window or t < sinks; tokens that no row of a call sees are not read.  0: no window (sinks 0).
+ * Prefill with a window needs TQ_PREFILL_CAUSAL, and V's largest scale so far counts the tokens that a block of 64 rows sees.
+ * mass (decode and tq_kv8_observe; NULL for prefill): fp32, one number per (block, KV head, row) at
+ * mass + block*stride_block + head*stride_head + row (elements; 16-byte aligned, strides multiples of 4).  A call adds to the
+ * number of every token that a query sees the softmax weights that the KV head's query heads and the call's queries give
+ * it, summed in fp32 from unrounded weights; a token that is new in the call starts from 0, whatever its row held.  A
+ * weight that is not a number adds nothing.  Blocks belong to one sequence of the call: where two name one, its
+ * numbers are unspecified.
+ * last (tq_kv8_observe): the last `last` queries of each sequence count (> 0).
+ * Workspaces: tq_kv8_decode_window_workspace_bytes of the same sizes (max_seq_len: the smaller of attn.max_seq_len and the
+ * block table's capacity; mass: 1 with one); tq_kv8_prefill_workspace_bytes.
+ */
+typedef struct tq_kv8_window_args {
+    tq_kv8_attn_args attn;
+    float* mass;
+    int64_t mass_stride_block, mass_stride_head;
+    int32_t window, sinks, last;
+    int32_t reserved; /* 0 */
+} tq_kv8_window_args;
+int tq_kv8_decode_window(const tq_kv8_window_args* a, tq_stream_t stream);
+int tq_kv8_prefill_window(const tq_kv8_window_args* a, tq_stream_t stream);
+int64_t tq_kv8_decode_window_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads, int max_seq_len, int window,
+                                             int sinks, int mass);
+
+/*
+ * mass of the tokens of prompts, as above, from queries whose attention has its own call: sequence s has the query rows
+ * cu_seqlens_q[s] .. cu_seqlens_q[s+1] - 1 of attn.q, its last (new) tokens; those of the last `last` count, all
+ * n new tokens start from 0.  Sequences without new tokens keep theirs.  attn as for tq_kv8_prefill with
+ * TQ_PREFILL_CAUSAL, without out and v_cache (NULL), and with max_seq_len, an upper bound of seq_lens (longer sequences are
+ * cut there).
+ */
+int tq_kv8_observe(const tq_kv8_window_args* a, tq_stream_t stream);
+int64_t tq_kv8_observe_workspace_bytes(int num_seqs, int max_q_len, int last, int num_q_heads, int num_kv_heads);
+
+/*
+ * Cuts the sequences that hold more than longer_than tokens (at most max_seq_len and the block table's capacity of them count) to
+ * `keep` of them, in place: every KV head keeps the first `sinks`, the last `recent` and, of those between, the
+ * keep - sinks - recent with the largest mass (NaN and tokens of bad table entries last; ties: the earlier token).  What is
+ * kept moves in its order to positions 0 .. keep - 1 of the sequence's blocks, mass with it; other rows
+ * keep their bytes.  The scale of a block whose rows came from elsewhere becomes the largest of the scales of the blocks they
+ * came from, code -> code * 2^(e - f) rounded to nearest even where it is another (NaN stays).  Rows
+ * from bad table entries become zeros, rows for them are dropped.
+ * change[s] = keep - seq_lens[s], or 0 for a sequence that is left as it is: tq_plan_args.new_tokens for the lengths and the
+ * blocks behind them.  seq_lens is not written.
+ * 0 <= sinks + recent <= keep <= longer_than, keep > 0.  Blocks belong to one sequence.  Caches, mass and strides
+ * as above.  workspace: tq_kv8_evict_workspace_bytes, 256-byte aligned, no initial contents; calls that overlap must not
+ * share it.
+ */
+typedef struct tq_kv8_evict_args {
+    void* k_cache;
+    void* v_cache;
+    float* mass;
+    const int32_t* block_tables;
+    const int32_t* seq_lens;
+    int32_t* change;
+    void* workspace;
+    int64_t workspace_bytes;
+    int64_t k_stride_block, k_stride_head, v_stride_block, v_stride_head, mass_stride_block, mass_stride_head;
+    int64_t num_blocks, block_table_stride;
+    int32_t encoding, num_seqs, num_kv_heads, head_dim, block_size, max_blocks_per_seq, max_seq_len;
+    int32_t keep, recent, sinks, longer_than;
+    int32_t reserved; /* 0 */
+} tq_kv8_evict_args;
+int tq_kv8_evict(const tq_kv8_evict_args* a, tq_stream_t stream);
+int64_t tq_kv8_evict_workspace_bytes(int num_seqs, int num_kv_heads, int keep, int block_size);
+
 /* ---- rotary positions -------------------------------------------------------------- */
 
 /*

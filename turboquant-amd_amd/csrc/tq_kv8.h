@@ -93,7 +93,33 @@ struct Kv8Attn {
     float* ws_acc;        // [slot][row][128]: a piece's output, divided by its sum
     float* ws_ml;         // [slot][row][2]: exponent base (log2), sum
     int* ends;            // decode: [segment][2], the waves with its first and its last step
+    // a window with sinks, and accumulated weights (tq_kv8_window_args)
+    int window, sinks;    // (no window: one of 2^31 - 1 tokens)
+    float* mass;
+    int64_t mass_stride_block, mass_stride_head;
+    float* scores;        // decode: [segment][most_steps][2 tiles][group][16], log2 units
+    float* ws_me;         // decode: [slot][row][2]: exponent base (log2) and unrounded sum of every piece
+    int most_steps;
 };
+
+// first token of the window of a query that sees `seen` tokens without one (below 0: a row before its sequence's start)
+__device__ __forceinline__ int kv8_window_from(int seen, int window) { return seen > window ? seen - window : 0; }
+
+// The steps of 32 tokens that hold what the positions first .. last see (first's window begins at lo, last sees the
+// tokens below hi): steps 0 .. ns - 1 of the sinks, then b0 .. ; n in all.
+struct Kv8Span {
+    int lo, ns, b0, n;
+    // the sequence's step that is number j here
+    __device__ __forceinline__ int step(int j) const { return j < ns ? j : j + b0 - ns; }
+};
+__device__ __forceinline__ Kv8Span kv8_span(int lo, int hi, int sinks) {
+    Kv8Span r;
+    r.lo = lo;
+    r.ns = (int)(((uint32_t)(sinks < lo ? sinks : lo) + 31) >> 5);
+    r.b0 = lo >> 5 > r.ns ? lo >> 5 : r.ns;
+    r.n = hi > 0 ? r.ns + (int)(((uint32_t)hi + 31) >> 5) - r.b0 : 0;
+    return r;
+}
 
 // The factor +-2^k that brings a query row with the largest |x| m to [1, 4), and 2^-k.  Rows that are all zero or
 // not finite keep k = 0.
@@ -246,5 +272,7 @@ __device__ __forceinline__ uint32_t kv8_nan_bytes(uint32_t w) { return ((w & 0x7
 
 // host: checks that decode and prefill share, and the derived fields
 int tq_kv8_attn_setup(const tq_kv8_attn_args* a, Kv8Attn* p);
+// host: the same with a window and accumulated weights
+int tq_kv8_window_setup(const tq_kv8_window_args* a, Kv8Attn* p);
 // host: compute units of the current device (0: unknown)
 int tq_kv8_cus();

@@ -38,15 +38,24 @@ constexpr int kMinSteps = 2;     // steps a wave takes at least (1 x 4099 tokens
 // of small ones was lost).
 constexpr float kUp = 14.f;
 
-__device__ __forceinline__ int steps_of(const Kv8Attn& p, int s) {
+__device__ __forceinline__ int length_of(const Kv8Attn& p, int s) {
     int L = p.a.seq_lens[s];
     L = L < p.cap ? L : p.cap;
-    return (int)(((uint32_t)(L > 0 ? L : 0) + 16 * kTiles - 1) / (16 * kTiles));
+    return L > 0 ? L : 0;
+}
+// the steps of a sequence of L tokens that the window and the sinks touch
+__device__ __forceinline__ Kv8Span span_of(const Kv8Attn& p, int L) { return kv8_span(kv8_window_from(L, p.window), L, p.sinks); }
+template <bool WINDOW>
+__device__ __forceinline__ int steps_of(const Kv8Attn& p, int s) {
+    static_assert(kTiles == 2, "kv8_span counts steps of 32 tokens");
+    if (WINDOW) return span_of(p, length_of(p, s)).n;
+    return (int)(((uint32_t)length_of(p, s) + 16 * kTiles - 1) / (16 * kTiles));
 }
 // Steps (one KV head) of the 64 sequences from s0 on: this lane's, and the sum up to it (below 2^32: 64 times 2^26)
+template <bool WINDOW>
 __device__ __forceinline__ uint32_t scan_steps(const Kv8Attn& p, int s0, uint32_t& mine) {
     const int lane = threadIdx.x & 63;
-    mine = s0 + lane < p.a.num_seqs ? (uint32_t)steps_of(p, s0 + lane) : 0u;
+    mine = s0 + lane < p.a.num_seqs ? (uint32_t)steps_of<WINDOW>(p, s0 + lane) : 0u;
     uint32_t in = mine;
     for (int d = 1; d < 64; d <<= 1) {
         const uint32_t x = (uint32_t)__shfl_up((int)in, d, 64);
@@ -74,7 +83,9 @@ __device__ __forceinline__ Share share_of(const Kv8Attn& p, int64_t P) {
     return h;
 }
 
-template <int ENC, bool FINE>
+// WINDOW: each sequence's steps are those that its window and the sinks touch, and with p.scores every step leaves its
+// scores for the accumulated weights.
+template <int ENC, bool FINE, bool WINDOW>
 __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kernel(Kv8Attn p) {
     using Code = Kv8Code<ENC>;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
@@ -82,11 +93,11 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
     const int64_t w = (int64_t)blockIdx.x * kWaves + wave;
     const int hkv = p.a.num_kv_heads;
     uint32_t mine;
-    uint32_t in = scan_steps(p, 0, mine);
+    uint32_t in = scan_steps<WINDOW>(p, 0, mine);
     int64_t P = (uint32_t)__builtin_amdgcn_readlane((int)in, 63);
     if (p.a.num_seqs > 64) {
         uint32_t u;
-        for (int s0 = 64; s0 < p.a.num_seqs; s0 += 64) P += (uint32_t)__builtin_amdgcn_readlane((int)scan_steps(p, s0, u), 63);
+        for (int s0 = 64; s0 < p.a.num_seqs; s0 += 64) P += (uint32_t)__builtin_amdgcn_readlane((int)scan_steps<WINDOW>(p, s0, u), 63);
     }
     P *= hkv;
     const Share share = share_of(p, P);
@@ -107,10 +118,10 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
         }
         seq0 += (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)in, 63) * hkv;
         s0 += 64;  // (pos is below the last one's end)
-        in = scan_steps(p, s0, mine);
+        in = scan_steps<WINDOW>(p, s0, mine);
     }
     s = __builtin_amdgcn_readfirstlane(s);
-    int np = steps_of(p, s);
+    int np = steps_of<WINDOW>(p, s);
     int kh = (int)((pos - seq0) / np);
     int64_t seg0 = seq0 + (int64_t)kh * np;
 
@@ -124,6 +135,9 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
         const int32_t* bt = p.a.block_tables + s * p.a.block_table_stride;
         const int last_tile = (L - 1) >> 4;
         const uint32_t scale_at = (uint32_t)p.a.block_size * TQ_HEAD_DIM;
+        const Kv8Span span = WINDOW ? span_of(p, L) : Kv8Span{0, 0, 0, 0};
+        // the sequence's tile that is number ti here (behind the last: one past the sequence's end)
+        auto tile_of = [&](int ti) -> int { return !WINDOW || ti < 2 * span.ns ? ti : ti + 2 * (span.b0 - span.ns); };
 
         // ---- 64 tiles' blocks and scales at a time, one per lane ----
         // block (tiles past the last and bad entries: a valid block and zero tokens), rows in use, scales
@@ -133,7 +147,7 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
         };
         auto tiles_from = [&](int t0) -> Tiles {
             Tiles t;
-            const int ti = t0 + lane;
+            const int ti = tile_of(t0 + lane);
             const int tc = ti < last_tile ? ti : last_tile;
             t.blk = bt[tq_udiv_apply((uint32_t)tc, p.tpb_div)];
             const int nv = L - 16 * ti;
@@ -141,6 +155,13 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
             if ((uint32_t)t.blk >= (uint64_t)p.a.num_blocks) {
                 t.blk = 0;
                 t.nv = 0;
+            }
+            if (WINDOW) {
+                // rows [from, upto) of it lie between the sinks and the window; all of them: no rows
+                int from = p.sinks - 16 * ti, upto = span.lo - 16 * ti;
+                from = from < 0 ? 0 : from < 16 ? from : 16;
+                upto = upto < from ? from : upto < 16 ? upto : 16;
+                t.nv = upto - from == 16 ? 0 : t.nv | from << 8 | upto << 16;
             }
             t.ks = *reinterpret_cast<const float*>(kb + t.blk * p.a.k_stride_block + scale_at);
             t.vs = *reinterpret_cast<const float*>(vb + t.blk * p.a.v_stride_block + scale_at);
@@ -175,7 +196,8 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
             }
         };
         // the tile's codes: block and row within it
-        auto tile_at = [&](int ti, int blk, int64_t stride) -> int64_t {
+        auto tile_at = [&](int number, int blk, int64_t stride) -> int64_t {
+            const int ti = tile_of(number);
             const int tc = ti < last_tile ? ti : last_tile;
             return blk * stride + (int64_t)(tc - p.tpb * (int)tq_udiv_apply((uint32_t)tc, p.tpb_div)) * (16 * TQ_HEAD_DIM);
         };
@@ -203,6 +225,7 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
         }
 
         float M = kKv8None, base = kKv8None, lsum = 0.f, vref = 0.f;  // M: largest score so far
+        float lfull = 0.f;  // WINDOW: the sum of the probabilities before their rounding
         tq_floatx4 acc[8];
 #pragma unroll
         for (int a = 0; a < 8; ++a) acc[a] = tq_floatx4{0.f, 0.f, 0.f, 0.f};
@@ -219,14 +242,20 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
             const bool over = more && i == 64 - kTiles;
             Blocks next;
             float ks[kTiles], vs[kTiles];
-            int nv[kTiles], all = 0;
+            int nv[kTiles], from[kTiles], upto[kTiles], all = 0;
 #pragma unroll
             for (int h = 0; h < kTiles; ++h) {
                 next.b[h] = over ? __builtin_amdgcn_readlane(nxt.blk, h) : __builtin_amdgcn_readlane(cur.blk, fi + h);
                 ks[h] = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(cur.ks), i + h));
                 vs[h] = __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(cur.vs), i + h));
                 nv[h] = __builtin_amdgcn_readlane(cur.nv, i + h);
-                all += nv[h];
+                from[h] = upto[h] = 0;
+                if (WINDOW) {
+                    from[h] = (nv[h] >> 8) & 255;
+                    upto[h] = nv[h] >> 16;
+                    nv[h] &= 255;
+                }
+                all += nv[h] + from[h] - upto[h];
             }
             // ---- scores in log2 units: tokens 4g + r of each tile, head n ----
             float sv[4 * kTiles];
@@ -246,15 +275,24 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
             load_keys(next, kTiles * jn);
             if (all != 16 * kTiles) {
 #pragma unroll
-                for (int r = 0; r < 4 * kTiles; ++r)
-                    if (4 * g + (r & 3) >= nv[r >> 2]) sv[r] = kKv8NegInf;
+                for (int r = 0; r < 4 * kTiles; ++r) {
+                    const int t = 4 * g + (r & 3);
+                    if (t >= nv[r >> 2] || (WINDOW && t >= from[r >> 2] && t < upto[r >> 2])) sv[r] = kKv8NegInf;
+                }
 #pragma unroll
                 for (int h = 0; h < kTiles; ++h) {
-                    const uint32_t keep = kv8_keep(nv[h] - 4 * g);
+                    uint32_t keep = kv8_keep(nv[h] - 4 * g);
+                    if (WINDOW) keep &= ~kv8_keep(upto[h] - 4 * g) | kv8_keep(from[h] - 4 * g);
 #pragma unroll
                     for (int a = 0; a < 8; ++a) vw[h][a] &= keep;
                     if (nv[h] == 0) vs[h] = 0.f;
                 }
+            }
+            if (WINDOW && p.scores && n < p.group) {
+                float* dst = p.scores + (((int64_t)s * hkv + kh) * p.most_steps + j) * (32 * p.group) + 16 * n + 4 * g;
+#pragma unroll
+                for (int h = 0; h < kTiles; ++h)
+                    *reinterpret_cast<float4*>(dst + 16 * h * p.group) = make_float4(sv[4 * h], sv[4 * h + 1], sv[4 * h + 2], sv[4 * h + 3]);
             }
             // ---- online softmax ----
             float mx = sv[0], vmax = vs[0];
@@ -267,6 +305,7 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
                 const float bn = __builtin_fabsf(Mn) < kKv8Far ? Mn - kUp : Mn;
                 const float alpha = __builtin_amdgcn_exp2f(base - bn);
                 lsum *= alpha;
+                lfull *= alpha;
 #pragma unroll
                 for (int a = 0; a < 8; ++a) acc[a] *= alpha;
                 M = Mn;
@@ -287,6 +326,7 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
                 tq_half8 ph, pl;
                 kv8_prob8<FINE>(pr, ph, pl);
                 lsum += kv8_sum8<FINE>(pr, ph);
+                if (WINDOW) lfull += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
                 const float va = kv8_relative(vs[h], rv), vb2 = kv8_relative(vs[h + 1], rv);
 #pragma unroll
                 for (int a = 0; a < 8; ++a) {
@@ -306,6 +346,14 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
             int* ends = p.ends + 2 * ((int64_t)s * hkv + kh);
             if (j0 == 0) ends[0] = (int)w;
             if (j1 == np) ends[1] = (int)w;
+        }
+        if (WINDOW && p.scores) {
+            const float l1 = tq_sum_over_groups(lfull);
+            if (g == 0 && n < p.group) {
+                const int64_t row = (w + (int64_t)s * hkv + kh) * p.group + n;
+                p.ws_me[2 * row] = base;
+                p.ws_me[2 * row + 1] = l1;
+            }
         }
         if (n < p.group) {
             float o[2][16];
@@ -335,10 +383,72 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
                 kh = 0;
                 do {
                     if (++s >= p.a.num_seqs) return;
-                    np = steps_of(p, s);
+                    np = steps_of<WINDOW>(p, s);
                 } while (np == 0);
             }
         }
+    }
+}
+
+// Adds the weights of a segment's tokens, summed over its query heads, to what they had; the sequence's last token starts
+// from 0.  Workgroup (segment, 32 steps): first each head's base and sum over the segment's pieces, then four tokens a
+// thread.  A weight that is not a number counts as 0.
+__global__ __launch_bounds__(256) void kv8_decode_mass_kernel(Kv8Attn p, int chunks) {
+    __shared__ float2 s_stat[16];
+    const uint32_t seg = blockIdx.x / (uint32_t)chunks, chunk = blockIdx.x - seg * (uint32_t)chunks;
+    const int hkv = p.a.num_kv_heads, s = (int)(seg / (uint32_t)hkv), kh = (int)seg - s * hkv;
+    const int L = length_of(p, s);
+    const Kv8Span span = span_of(p, L);
+    if ((int)chunk * 32 >= span.n) return;
+    const int w0 = p.ends[2 * seg], w1 = p.ends[2 * seg + 1];
+    const int lane = threadIdx.x & 63;
+    for (int r = threadIdx.x >> 6; r < p.group; r += 4) {
+        float M = kKv8None, l = 0.f;
+        for (int w = w0 + lane; w <= w1; w += 64) {
+            const int64_t row = ((int64_t)w + seg) * p.group + r;
+            const float b = p.ws_me[2 * row], x = p.ws_me[2 * row + 1];
+            const float Mn = fmaxf(M, b);
+            l = l * __builtin_amdgcn_exp2f(M - Mn) + x * __builtin_amdgcn_exp2f(b - Mn);
+            M = Mn;
+        }
+        for (int m = 1; m < 64; m <<= 1) {
+            const float b = __shfl_xor(M, m, 64), x = __shfl_xor(l, m, 64);
+            const float Mn = fmaxf(M, b);
+            l = l * __builtin_amdgcn_exp2f(M - Mn) + x * __builtin_amdgcn_exp2f(b - Mn);
+            M = Mn;
+        }
+        if (lane == 0) s_stat[r] = make_float2(M, l == 0.f ? 0.f : 1.f / l);
+    }
+    __syncthreads();
+    const int j = 32 * (int)chunk + (int)(threadIdx.x >> 3);
+    if (j >= span.n) return;
+    const int in = 4 * (int)(threadIdx.x & 7);  // first token within the step
+    const int t = 32 * span.step(j) + in;
+    if (t >= L) return;
+    const float* src = p.scores + (((int64_t)seg) * p.most_steps + j) * (32 * p.group) + (in >> 4) * (16 * p.group) + (in & 15);
+    float add[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < p.group; ++r) {
+        const float4 x = *reinterpret_cast<const float4*>(src + 16 * r);
+        const float2 st = s_stat[r];
+        const float y[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float f = __builtin_amdgcn_exp2f(y[k] - st.x) * st.y;
+            add[k] += f == f ? f : 0.f;
+        }
+    }
+    const int b = (int)tq_udiv_apply((uint32_t)(t >> 4), p.tpb_div);
+    const int blk = p.a.block_tables[s * p.a.block_table_stride + b];
+    if ((uint32_t)blk >= (uint64_t)p.a.num_blocks) return;
+    float* dst = p.mass + blk * p.mass_stride_block + kh * p.mass_stride_head + (t - b * p.a.block_size);
+    if (t + 4 <= L && (t >= span.lo || t + 4 <= p.sinks)) {
+        float4 m = *reinterpret_cast<const float4*>(dst);
+        if (t + 4 == L) m.w = 0.f;
+        *reinterpret_cast<float4*>(dst) = make_float4(m.x + add[0], m.y + add[1], m.z + add[2], m.w + add[3]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (t + k < L && (t + k >= span.lo || t + k < p.sinks)) dst[k] = (t + k == L - 1 ? 0.f : dst[k]) + add[k];
     }
 }
 
@@ -346,6 +456,7 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
 // running mean, which stays within the values' range; nothing to do where one wave held it all, zeros where the
 // sequence is empty.  The workgroup's 8 half-waves share the pieces, a lane has 4 dims.  (With a workgroup per KV
 // head, one sequence of 4099 tokens: merge 13.6 -> 6.6 us.)
+template <bool WINDOW>
 __global__ __launch_bounds__(256) void kv8_decode_merge_kernel(Kv8Attn p) {
     __shared__ float4 s_acc[8][32];
     __shared__ float2 s_ml[8];
@@ -354,7 +465,7 @@ __global__ __launch_bounds__(256) void kv8_decode_merge_kernel(Kv8Attn p) {
     const int kh = head / p.group, r = head - kh * p.group;
     const int* ends = p.ends + 2 * ((int64_t)s * hkv + kh);
     int w0 = ends[0], w1 = ends[1];
-    if (steps_of(p, s) == 0) {  // (no wave had it)
+    if (steps_of<WINDOW>(p, s) == 0) {  // (no wave had it)
         w0 = 0;
         w1 = -1;
     }
@@ -445,44 +556,115 @@ int tq_kv8_attn_setup(const tq_kv8_attn_args* a, Kv8Attn* p) {
     return TQ_OK;
 }
 
+int tq_kv8_window_setup(const tq_kv8_window_args* w, Kv8Attn* p) {
+    const int rc = tq_kv8_attn_setup(&w->attn, p);
+    if (rc != TQ_OK) return rc;
+    if (w->window < 0 || w->sinks < 0 || (w->sinks && !w->window) || w->reserved) return TQ_ERR_INVALID_ARGUMENT;
+    if (w->mass && ((uintptr_t)w->mass % 16 || (w->mass_stride_block | w->mass_stride_head) % 4)) return TQ_ERR_ALIGNMENT;
+    p->window = w->window ? w->window : INT32_MAX;
+    p->sinks = w->sinks;
+    p->mass = w->mass;
+    p->mass_stride_block = w->mass_stride_block;
+    p->mass_stride_head = w->mass_stride_head;
+    return TQ_OK;
+}
+
 extern "C" int64_t tq_kv8_decode_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads) {
     if (num_seqs < 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads) return 0;
     const int64_t slots = kMaxWorkers + (int64_t)num_seqs * num_kv_heads;
     return slots * (num_q_heads / num_kv_heads) * (TQ_HEAD_DIM + 2) * 4 + (int64_t)num_seqs * num_kv_heads * 8;
 }
 
-extern "C" int tq_kv8_decode(const tq_kv8_attn_args* a, tq_stream_t stream) {
-    if (!a) return TQ_ERR_INVALID_ARGUMENT;
-    Kv8Attn p = {};
-    const int rc = tq_kv8_attn_setup(a, &p);
-    if (rc != TQ_OK) return rc;
+namespace {
+
+int64_t align256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+// steps of a sequence of up to len tokens (a window's tokens reach into one step more than they fill)
+int64_t most_steps(int64_t len, int64_t window, int64_t sinks) {
+    const int64_t all = (len + 31) / 32;
+    if (!window) return all;
+    const int64_t m = (window + 31) / 32 + 1 + (sinks + 31) / 32;
+    return m < all ? m : all;
+}
+
+int launch_decode(Kv8Attn& p, bool window, int64_t need, tq_stream_t stream) {
+    const tq_kv8_attn_args* a = &p.a;
     if (p.group > 16) return TQ_ERR_GQA;
     if (a->num_seqs == 0) return TQ_OK;
     // (a launch's threads stay below 2^32)
     if (a->max_seq_len < 0 || (int64_t)a->num_seqs * a->num_q_heads > 0xffffff) return TQ_ERR_INVALID_ARGUMENT;
     if (!a->q || !a->out || !a->k_cache || !a->v_cache || (!a->block_tables && a->max_blocks_per_seq) || !a->seq_lens) return TQ_ERR_INVALID_ARGUMENT;
-    const int64_t need = tq_kv8_decode_workspace_bytes(a->num_seqs, a->num_q_heads, a->num_kv_heads);
     if (!a->workspace || (uintptr_t)a->workspace % 256 || a->workspace_bytes < need) return TQ_ERR_WORKSPACE;
-    const int cus = tq_kv8_cus();
-    if (cus <= 0) return (int)hipErrorNoDevice;
     p.cap = p.cap < a->max_seq_len ? p.cap : a->max_seq_len;
     const int64_t slots = kMaxWorkers + (int64_t)a->num_seqs * a->num_kv_heads;
     p.ws_acc = static_cast<float*>(a->workspace);
     p.ws_ml = p.ws_acc + slots * p.group * TQ_HEAD_DIM;
     p.ends = reinterpret_cast<int*>(p.ws_ml + slots * p.group * 2);
+    // tokens of a sequence that are read
+    const int64_t most = window ? most_steps(p.cap, p.window == INT32_MAX ? 0 : p.window, p.sinks) : (p.cap + 16 * kTiles - 1) / (16 * kTiles);
+    p.most_steps = (int)most;
+    const int64_t chunks = (most + 31) / 32;
+    if (p.mass) {
+        uint8_t* at = static_cast<uint8_t*>(a->workspace) + align256(tq_kv8_decode_workspace_bytes(a->num_seqs, a->num_q_heads, a->num_kv_heads));
+        p.ws_me = reinterpret_cast<float*>(at);
+        p.scores = reinterpret_cast<float*>(at + align256(slots * p.group * 8));
+        if ((int64_t)a->num_seqs * a->num_kv_heads * chunks > 0xffffff) return TQ_ERR_INVALID_ARGUMENT;
+    }
+    const int cus = tq_kv8_cus();
+    if (cus <= 0) return (int)hipErrorNoDevice;
     // no more waves than the lengths can ask for
-    const int64_t most = (int64_t)a->num_seqs * a->num_kv_heads * ((p.cap + 16 * kTiles - 1) / (16 * kTiles)) / kMinSteps;
+    const int64_t ask = (int64_t)a->num_seqs * a->num_kv_heads * most / kMinSteps;
     int64_t workers = (int64_t)cus * kWavesPerCu;
     workers = workers < kMaxWorkers ? workers : kMaxWorkers;
-    workers = workers < most ? workers : most;
+    workers = workers < ask ? workers : ask;
     p.workers = (int)(workers < 1 ? 1 : workers);
     const bool fine = a->q_dtype == TQ_F32 || a->out_dtype == TQ_F32;
-    const void* kern = a->encoding == TQ_E4M3 ? (fine ? (const void*)kv8_decode_kernel<TQ_E4M3, true> : (const void*)kv8_decode_kernel<TQ_E4M3, false>)
-                                              : (fine ? (const void*)kv8_decode_kernel<TQ_INT8, true> : (const void*)kv8_decode_kernel<TQ_INT8, false>);
+    const void* kern = nullptr;
+#define TQ_DECODE(E, F, W) \
+    if (a->encoding == E && fine == F && window == W) kern = (const void*)kv8_decode_kernel<E, F, W>;
+    TQ_DECODE(TQ_E4M3, false, false) TQ_DECODE(TQ_E4M3, true, false) TQ_DECODE(TQ_E4M3, false, true) TQ_DECODE(TQ_E4M3, true, true)
+    TQ_DECODE(TQ_INT8, false, false) TQ_DECODE(TQ_INT8, true, false) TQ_DECODE(TQ_INT8, false, true) TQ_DECODE(TQ_INT8, true, true)
+#undef TQ_DECODE
     void* args[] = {&p};
     hipError_t e = hipLaunchKernel(kern, dim3((unsigned)((p.workers + kWaves - 1) / kWaves)), dim3(64 * kWaves), args, 0, stream);
     if (e == hipSuccess)
-        e = hipLaunchKernel((const void*)kv8_decode_merge_kernel, dim3((unsigned)(a->num_seqs * a->num_q_heads)), dim3(256), args, 0, stream);
+        e = hipLaunchKernel(window ? (const void*)kv8_decode_merge_kernel<true> : (const void*)kv8_decode_merge_kernel<false>,
+                            dim3((unsigned)(a->num_seqs * a->num_q_heads)), dim3(256), args, 0, stream);
+    if (e == hipSuccess && p.mass && chunks) {
+        int n = (int)chunks;
+        void* margs[] = {&p, &n};
+        e = hipLaunchKernel((const void*)kv8_decode_mass_kernel, dim3((unsigned)(a->num_seqs * a->num_kv_heads * chunks)), dim3(256), margs, 0, stream);
+    }
     if (e == hipSuccess) e = hipGetLastError();
     return e == hipSuccess ? TQ_OK : (int)e;
+}
+
+}  // namespace
+
+extern "C" int64_t tq_kv8_decode_window_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads, int max_seq_len, int window,
+                                                        int sinks, int mass) {
+    const int64_t plain = tq_kv8_decode_workspace_bytes(num_seqs, num_q_heads, num_kv_heads);
+    if (plain <= 0 || !mass || max_seq_len < 0 || window < 0 || sinks < 0) return plain;
+    const int64_t slots = kMaxWorkers + (int64_t)num_seqs * num_kv_heads;
+    return align256(plain) + align256(slots * (num_q_heads / num_kv_heads) * 8) +
+           (int64_t)num_seqs * num_q_heads * most_steps(max_seq_len, window, sinks) * 32 * 4;
+}
+
+extern "C" int tq_kv8_decode(const tq_kv8_attn_args* a, tq_stream_t stream) {
+    if (!a) return TQ_ERR_INVALID_ARGUMENT;
+    Kv8Attn p = {};
+    const int rc = tq_kv8_attn_setup(a, &p);
+    return rc != TQ_OK ? rc : launch_decode(p, false, tq_kv8_decode_workspace_bytes(a->num_seqs, a->num_q_heads, a->num_kv_heads), stream);
+}
+
+extern "C" int tq_kv8_decode_window(const tq_kv8_window_args* w, tq_stream_t stream) {
+    if (!w) return TQ_ERR_INVALID_ARGUMENT;
+    const tq_kv8_attn_args* a = &w->attn;
+    Kv8Attn p = {};
+    const int rc = tq_kv8_window_setup(w, &p);
+    if (rc != TQ_OK) return rc;
+    if (!w->window && !w->mass)
+        return launch_decode(p, false, tq_kv8_decode_workspace_bytes(a->num_seqs, a->num_q_heads, a->num_kv_heads), stream);
+    const int len = p.cap < a->max_seq_len ? p.cap : a->max_seq_len;
+    return launch_decode(p, true, tq_kv8_decode_window_workspace_bytes(a->num_seqs, a->num_q_heads, a->num_kv_heads, len, w->window,
+                                                                       w->sinks, w->mass != nullptr), stream);
 }

@@ -1,0 +1,418 @@
+// Eviction from the 8-bit paged caches by accumulated weight (tiles: tq_kv8.h).
+//
+// A segment is a (sequence, KV head).  kv8_evict_plan_kernel finds, a workgroup per segment, which tokens stay: the m-th
+// largest number between the first and the last ones by three passes over 11, 11 and 10 bits of the numbers' order
+// (counts in LDS), then the tokens above it and the first ones equal to it, in order.  kv8_evict_scales_kernel
+// gives every kept block its scale and every row its change of exponent.  The rows then move in units of 16:
+// kv8_evict_gather_kernel into the workspace, kv8_evict_scatter_kernel from there to the segment's first blocks.
+#include "tq_kv8.h"
+
+namespace {
+
+constexpr int kUnit = 16;                         // rows that a wave moves
+constexpr int kStage = 2 * kUnit * TQ_HEAD_DIM;   // their codes
+
+struct Evict {
+    tq_kv8_evict_args a;
+    tq_udiv tpb_div;
+    int tpb, cap, units, blocks;  // units and blocks of what is kept
+    int32_t* list;                // [segment][16 units]: the kept tokens
+    uint16_t* shift;              // [segment][16 units]: exponents that K's (low byte) and V's codes fall by; 63: zeros
+    float2* scales;               // [segment][blocks]: K's and V's
+    uint8_t* stage;               // [segment][units][kStage]
+    float* stage_mass;            // [segment][16 units]
+};
+
+__device__ __forceinline__ int length_of(const Evict& p, int s) {
+    const int L = p.a.seq_lens[s];
+    return L < p.cap ? (L > 0 ? L : 0) : p.cap;
+}
+// order of the numbers as whole numbers: -0 as 0, NaN below all
+__device__ __forceinline__ uint32_t key_of(float x) {
+    if (!(x == x)) return 0u;
+    const uint32_t u = __float_as_uint(x + 0.f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+// block of tile t (16 tokens) of sequence s; -1: a bad entry
+__device__ __forceinline__ int block_of(const Evict& p, int s, int tile, int& row) {
+    const int b = (int)tq_udiv_apply((uint32_t)tile, p.tpb_div);
+    row = 16 * (tile - b * p.tpb);
+    const int blk = p.a.block_tables[s * p.a.block_table_stride + b];
+    return (uint32_t)blk < (uint64_t)p.a.num_blocks ? blk : -1;
+}
+
+constexpr int kPlan = 1024;
+
+// inclusive sum over the workgroup's threads in order; total: of all of them (two barriers)
+__device__ __forceinline__ uint32_t scan(uint32_t x, uint32_t* s_tot, uint32_t& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t y = (uint32_t)__shfl_up((int)x, d, 64);
+        if (lane >= d) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) s_tot[wave] = x;
+    __syncthreads();
+    uint32_t before = 0;
+    total = 0;
+    for (int w = 0; w < kPlan / 64; ++w) {
+        const uint32_t y = s_tot[w];
+        before += w < wave ? y : 0u;
+        total += y;
+    }
+    return x + before;
+}
+
+__global__ __launch_bounds__(kPlan) void kv8_evict_plan_kernel(Evict p) {
+    __shared__ uint32_t s_hist[2048], s_tot[kPlan / 64], s_pick[2];
+    const uint32_t seg = blockIdx.x;
+    const int s = (int)(seg / (uint32_t)p.a.num_kv_heads), kh = (int)seg - s * p.a.num_kv_heads;
+    const int tid = threadIdx.x;
+    const int L = length_of(p, s);
+    const bool cut = L > p.a.longer_than;
+    if (kh == 0 && tid == 0) p.a.change[s] = cut ? p.a.keep - p.a.seq_lens[s] : 0;
+    if (!cut) return;
+    const int c0 = p.a.sinks, c1 = L - p.a.recent;  // candidates
+    const float* mass = p.a.mass + kh * p.a.mass_stride_head;
+    // keys of tokens t .. t + 3 (t a multiple of 4)
+    auto load = [&](int t, uint32_t (&k)[4]) {
+        int row;
+        const int blk = block_of(p, s, t >> 4, row);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (blk >= 0) x = *reinterpret_cast<const float4*>(mass + blk * p.a.mass_stride_block + row + (t & 15));
+        k[0] = blk < 0 ? 0u : key_of(x.x);
+        k[1] = blk < 0 ? 0u : key_of(x.y);
+        k[2] = blk < 0 ? 0u : key_of(x.z);
+        k[3] = blk < 0 ? 0u : key_of(x.w);
+    };
+    // ---- the least key that stays, and how many of the tokens with it ----
+    uint32_t least = 0xffffffffu, need = (uint32_t)(p.a.keep - p.a.sinks - p.a.recent), mask = 0;
+    if (need) {
+        least = 0;
+        for (int pass = 0; pass < 3; ++pass) {
+            const int sh = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : 2048;
+            for (int i = tid; i < 2048; i += kPlan) s_hist[i] = 0;
+            __syncthreads();
+            for (int t = 4 * tid; t < c1; t += 4 * kPlan) {
+                uint32_t k[4];
+                load(t, k);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (t + i >= c0 && t + i < c1 && (k[i] & mask) == least) atomicAdd(&s_hist[(k[i] >> sh) & (bins - 1)], 1u);
+            }
+            __syncthreads();
+            // bins from the largest on, two a thread
+            const int top = 2047 - 2 * tid;
+            const uint32_t a = s_hist[top], b = s_hist[top - 1];
+            uint32_t total;
+            const uint32_t in = scan(a + b, s_tot, total), before = in - a - b;
+            if (before < need && need <= in) {
+                const bool first = need <= before + a;
+                s_pick[0] = (uint32_t)(first ? top : top - 1);
+                s_pick[1] = need - before - (first ? 0u : a);
+            }
+            __syncthreads();
+            least |= s_pick[0] << sh;
+            mask |= (uint32_t)(bins - 1) << sh;
+            need = s_pick[1];
+        }
+    }
+    // ---- the kept tokens, in order ----
+    int32_t* list = p.list + (int64_t)seg * (kUnit * p.units);
+    uint32_t kept = 0, equal = 0;  // before this round: above `least` or always kept; equal to it
+    for (int r0 = 0; r0 < L; r0 += 4 * kPlan) {
+        const int t = r0 + 4 * tid;
+        uint32_t k[4], n = 0;
+        if (t < L) load(t, k);
+        int what[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int x = t + i;
+            what[i] = x >= L ? 0 : x < c0 || x >= c1 || k[i] > least ? 1 : k[i] == least ? 2 : 0;
+            n += what[i] == 1 ? 1u : what[i] == 2 ? 0x10000u : 0u;
+        }
+        uint32_t total;
+        const uint32_t before = scan(n, s_tot, total) - n;
+        uint32_t g = kept + (before & 0xffffu), e = equal + (before >> 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (what[i] == 1 || (what[i] == 2 && e < need)) list[g + (e < need ? e : need)] = t + i;
+            g += what[i] == 1;
+            e += what[i] == 2;
+        }
+        kept += total & 0xffffu;
+        equal += total >> 16;
+    }
+}
+
+// a tile's scale as its exponent + 127; 0: zero
+__device__ __forceinline__ int exponent_at(const uint8_t* tile, const Evict& p) {
+    return (int)(*reinterpret_cast<const uint32_t*>(tile + (int64_t)p.a.block_size * TQ_HEAD_DIM) >> 23) & 255;
+}
+
+// A wave per kept block: the largest scale of the blocks its rows come from, and what each row's codes fall by.
+__global__ __launch_bounds__(256) void kv8_evict_scales_kernel(Evict p) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t unit = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint32_t seg = unit / (uint32_t)p.blocks;
+    const int b = (int)(unit - seg * (uint32_t)p.blocks);
+    if (seg >= (uint32_t)p.a.num_seqs * (uint32_t)p.a.num_kv_heads) return;
+    const int s = (int)(seg / (uint32_t)p.a.num_kv_heads), kh = (int)seg - s * p.a.num_kv_heads;
+    if (length_of(p, s) <= p.a.longer_than) return;
+    const int d0 = b * p.a.block_size, d1 = d0 + p.a.block_size < p.a.keep ? d0 + p.a.block_size : p.a.keep;
+    const uint8_t* kc = static_cast<const uint8_t*>(p.a.k_cache) + kh * p.a.k_stride_head;
+    const uint8_t* vc = static_cast<const uint8_t*>(p.a.v_cache) + kh * p.a.v_stride_head;
+    const int64_t at = (int64_t)seg * (kUnit * p.units);
+    auto exponents = [&](int d, int& ek, int& ev) {
+        int row;
+        const int blk = block_of(p, s, p.list[at + d] >> 4, row);
+        ek = blk < 0 ? 0 : exponent_at(kc + blk * p.a.k_stride_block, p);
+        ev = blk < 0 ? 0 : exponent_at(vc + blk * p.a.v_stride_block, p);
+    };
+    int mk = 0, mv = 0;
+    for (int d = d0 + lane; d < d1; d += 64) {
+        int ek, ev;
+        exponents(d, ek, ev);
+        mk = mk > ek ? mk : ek;
+        mv = mv > ev ? mv : ev;
+    }
+    for (int m = 1; m < 64; m <<= 1) {
+        const int x = __shfl_xor(mk, m, 64), y = __shfl_xor(mv, m, 64);
+        mk = mk > x ? mk : x;
+        mv = mv > y ? mv : y;
+    }
+    if (lane == 0) p.scales[(int64_t)seg * p.blocks + b] = make_float2(kv8_scale(mk), kv8_scale(mv));
+    for (int d = d0 + lane; d < d1; d += 64) {
+        int ek, ev;
+        exponents(d, ek, ev);
+        const int sk = ek && mk - ek < 63 ? mk - ek : 63, sv = ev && mv - ev < 63 ? mv - ev : 63;
+        p.shift[at + d] = (uint16_t)(sk | sv << 8);
+    }
+}
+
+// Codes of a word times f[i] (powers of two, or 0), rounded to nearest even
+template <int ENC>
+__device__ __forceinline__ uint32_t rescale(uint32_t w, float f0, float f1, float f2, float f3) {
+    using Code = Kv8Code<ENC>;
+    return Code::template pack<true>(Code::value(w, 0) * f0, Code::value(w, 1) * f1, Code::value(w, 2) * f2, Code::value(w, 3) * f3, 1.f);
+}
+__device__ __forceinline__ float factor_of(int shift) { return shift < 63 ? kv8_exp2i(-shift) : 0.f; }
+
+// 16 kept rows in a wave's registers: K's row lane / 4, bytes 32 (lane % 4) ..; V's words of dims 2 lane and
+// 2 lane + 1 of the four groups; row lane's number
+struct Unit {
+    tq_u32x4 k[2];
+    tq_u32x2 v[4];
+    float mass;
+};
+
+template <int ENC>
+__device__ __forceinline__ Unit load_unit(const Evict& p, uint32_t seg, int s, int kh, int u) {
+    const int lane = threadIdx.x & 63;
+    const int64_t at = (int64_t)seg * (kUnit * p.units) + kUnit * u;
+    const int rows = p.a.keep - kUnit * u < kUnit ? p.a.keep - kUnit * u : kUnit;
+    // lane r < rows: its row's source
+    int blk = -1, row = 0, sh = 0;
+    if (lane < rows) {
+        const int src = p.list[at + lane];
+        blk = block_of(p, s, src >> 4, row);
+        row += src & 15;
+        sh = p.shift[at + lane];
+    }
+    Unit x;
+    x.mass = 0.f;
+    if (blk >= 0) x.mass = p.a.mass[blk * p.a.mass_stride_block + kh * p.a.mass_stride_head + row];
+    const bool falls = __builtin_amdgcn_ballot_w64(sh != 0) != 0;
+    {
+        const int b = __shfl(blk, lane >> 2, 64), r = __shfl(row, lane >> 2, 64);
+        x.k[0] = x.k[1] = tq_u32x4{0, 0, 0, 0};
+        if (b >= 0) {
+            const tq_u32x4* src = reinterpret_cast<const tq_u32x4*>(static_cast<const uint8_t*>(p.a.k_cache) + b * p.a.k_stride_block +
+                                                                    kh * p.a.k_stride_head + (int64_t)r * TQ_HEAD_DIM + 32 * (lane & 3));
+            x.k[0] = src[0];
+            x.k[1] = src[1];
+        }
+    }
+    const uint8_t* vc = static_cast<const uint8_t*>(p.a.v_cache) + kh * p.a.v_stride_head;
+    tq_u32x2 w[kUnit];
+#pragma unroll
+    for (int i = 0; i < kUnit; ++i) {
+        const int b = __builtin_amdgcn_readlane(blk, i), r = __builtin_amdgcn_readlane(row, i);
+        w[i] = tq_u32x2{0, 0};
+        if (b >= 0) w[i] = reinterpret_cast<const tq_u32x2*>(vc + b * p.a.v_stride_block + (int64_t)(r >> 2) * 512)[lane];
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        x.v[g] = tq_u32x2{0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int from = 8 * (__builtin_amdgcn_readlane(row, 4 * g + i) & 3);
+            x.v[g][0] |= ((w[4 * g + i][0] >> from) & 255u) << (8 * i);
+            x.v[g][1] |= ((w[4 * g + i][1] >> from) & 255u) << (8 * i);
+        }
+    }
+    if (falls) {
+        const float fk = factor_of(__shfl(sh, lane >> 2, 64) & 255);
+        if (fk != 1.f) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x.k[i][j] = rescale<ENC>(x.k[i][j], fk, fk, fk, fk);
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = factor_of(__builtin_amdgcn_readlane(sh, 4 * g + i) >> 8);
+            if (f[0] != 1.f || f[1] != 1.f || f[2] != 1.f || f[3] != 1.f) {
+                x.v[g][0] = rescale<ENC>(x.v[g][0], f[0], f[1], f[2], f[3]);
+                x.v[g][1] = rescale<ENC>(x.v[g][1], f[0], f[1], f[2], f[3]);
+            }
+        }
+    }
+    return x;
+}
+
+__device__ __forceinline__ void store_unit(const Evict& p, uint32_t seg, int s, int kh, int u, const Unit& x) {
+    const int lane = threadIdx.x & 63;
+    int row;
+    const int blk = block_of(p, s, u, row);
+    if (blk < 0) return;
+    const int rows = p.a.keep - kUnit * u < kUnit ? p.a.keep - kUnit * u : kUnit;
+    uint8_t* kt = static_cast<uint8_t*>(p.a.k_cache) + blk * p.a.k_stride_block + kh * p.a.k_stride_head;
+    uint8_t* vt = static_cast<uint8_t*>(p.a.v_cache) + blk * p.a.v_stride_block + kh * p.a.v_stride_head;
+    if (lane < rows) p.a.mass[blk * p.a.mass_stride_block + kh * p.a.mass_stride_head + row + lane] = x.mass;
+    if ((lane >> 2) < rows) {
+        tq_u32x4* dst = reinterpret_cast<tq_u32x4*>(kt + (int64_t)(row + (lane >> 2)) * TQ_HEAD_DIM + 32 * (lane & 3));
+        dst[0] = x.k[0];
+        dst[1] = x.k[1];
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const uint32_t mine = kv8_keep(rows - 4 * g);
+        tq_u32x2* dst = reinterpret_cast<tq_u32x2*>(vt + (int64_t)(row + 4 * g) * TQ_HEAD_DIM) + lane;
+        if (mine == 0xffffffffu) {
+            *dst = x.v[g];
+        } else if (mine) {  // rows behind the kept ones stay
+            const tq_u32x2 old = *dst;
+            *dst = tq_u32x2{(x.v[g][0] & mine) | (old[0] & ~mine), (x.v[g][1] & mine) | (old[1] & ~mine)};
+        }
+    }
+    if (row == 0 && lane == 0) {
+        const float2 sc = p.scales[(int64_t)seg * p.blocks + tq_udiv_apply((uint32_t)u, p.tpb_div)];
+        *reinterpret_cast<float*>(kt + (int64_t)p.a.block_size * TQ_HEAD_DIM) = sc.x;
+        *reinterpret_cast<float*>(vt + (int64_t)p.a.block_size * TQ_HEAD_DIM) = sc.y;
+    }
+}
+
+// wave -> (segment, unit); false: nothing to do
+__device__ __forceinline__ bool unit_of(const Evict& p, uint32_t& seg, int& s, int& kh, int& u) {
+    const uint32_t x = blockIdx.x * 4 + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    seg = x / (uint32_t)p.units;
+    u = (int)(x - seg * (uint32_t)p.units);
+    s = (int)(seg / (uint32_t)p.a.num_kv_heads);
+    kh = (int)seg - s * p.a.num_kv_heads;
+    return s < p.a.num_seqs && length_of(p, s) > p.a.longer_than;
+}
+
+template <int ENC>
+__global__ __launch_bounds__(256) void kv8_evict_gather_kernel(Evict p) {
+    uint32_t seg;
+    int s, kh, u;
+    if (!unit_of(p, seg, s, kh, u)) return;
+    const int lane = threadIdx.x & 63;
+    const Unit x = load_unit<ENC>(p, seg, s, kh, u);
+    const int64_t n = (int64_t)seg * p.units + u;
+    tq_u32x4* dst = reinterpret_cast<tq_u32x4*>(p.stage + n * kStage);
+    dst[2 * lane] = x.k[0];
+    dst[2 * lane + 1] = x.k[1];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) reinterpret_cast<tq_u32x2*>(dst + 128)[64 * g + lane] = x.v[g];
+    if (lane < kUnit) p.stage_mass[n * kUnit + lane] = x.mass;
+}
+
+__global__ __launch_bounds__(256) void kv8_evict_scatter_kernel(Evict p) {
+    uint32_t seg;
+    int s, kh, u;
+    if (!unit_of(p, seg, s, kh, u)) return;
+    const int lane = threadIdx.x & 63;
+    const int64_t n = (int64_t)seg * p.units + u;
+    const tq_u32x4* src = reinterpret_cast<const tq_u32x4*>(p.stage + n * kStage);
+    Unit x;
+    x.k[0] = src[2 * lane];
+    x.k[1] = src[2 * lane + 1];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) x.v[g] = reinterpret_cast<const tq_u32x2*>(src + 128)[64 * g + lane];
+    x.mass = lane < kUnit ? p.stage_mass[n * kUnit + lane] : 0.f;
+    store_unit(p, seg, s, kh, u, x);
+}
+
+int64_t align256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+
+}  // namespace
+
+extern "C" int64_t tq_kv8_evict_workspace_bytes(int num_seqs, int num_kv_heads, int keep, int block_size) {
+    if (num_seqs <= 0 || num_kv_heads <= 0 || keep <= 0 || block_size <= 0 || block_size % 16) return 0;
+    const int64_t segs = (int64_t)num_seqs * num_kv_heads, units = ((int64_t)keep + kUnit - 1) / kUnit;
+    const int64_t blocks = ((int64_t)keep + block_size - 1) / block_size;
+    return align256(segs * units * kUnit * 4) + align256(segs * units * kUnit * 2) + align256(segs * blocks * 8) +
+           align256(segs * units * kUnit * 4) + segs * units * kStage;
+}
+
+extern "C" int tq_kv8_evict(const tq_kv8_evict_args* a, tq_stream_t stream) {
+    if (!a) return TQ_ERR_INVALID_ARGUMENT;
+    if (a->head_dim != TQ_HEAD_DIM) return TQ_ERR_HEAD_DIM;
+    if (a->block_size <= 0 || a->block_size % 16 || a->block_size > 65536) return TQ_ERR_BLOCK_SIZE;
+    if (a->encoding != TQ_E4M3 && a->encoding != TQ_INT8) return TQ_ERR_DTYPE;
+    if (a->num_seqs < 0 || a->num_kv_heads <= 0 || a->num_blocks <= 0 || a->num_blocks > INT32_MAX || a->max_blocks_per_seq < 0 ||
+        a->block_table_stride < a->max_blocks_per_seq || a->max_seq_len < 0 || a->reserved)
+        return TQ_ERR_INVALID_ARGUMENT;
+    if (a->keep <= 0 || a->sinks < 0 || a->recent < 0 || (int64_t)a->sinks + a->recent > a->keep || a->longer_than < a->keep)
+        return TQ_ERR_INVALID_ARGUMENT;
+    const uintptr_t ptrs = (uintptr_t)a->k_cache | (uintptr_t)a->v_cache | (uintptr_t)a->mass;
+    const int64_t by = a->k_stride_block | a->k_stride_head | a->v_stride_block | a->v_stride_head;
+    if (ptrs % 16 || by % 16 || (a->mass_stride_block | a->mass_stride_head) % 4) return TQ_ERR_ALIGNMENT;
+    if (a->num_seqs == 0) return TQ_OK;
+    if (!a->k_cache || !a->v_cache || !a->mass || (!a->block_tables && a->max_blocks_per_seq) || !a->seq_lens || !a->change)
+        return TQ_ERR_INVALID_ARGUMENT;
+    Evict p = {};
+    p.a = *a;
+    p.tpb = a->block_size / 16;
+    p.tpb_div = tq_make_udiv((uint32_t)p.tpb);
+    int64_t cap = (int64_t)a->max_blocks_per_seq * a->block_size;
+    cap = cap < a->max_seq_len ? cap : a->max_seq_len;
+    p.cap = (int)(cap < kKv8MaxLen ? cap : kKv8MaxLen);
+    const int64_t segs = (int64_t)a->num_seqs * a->num_kv_heads;
+    // (a launch's threads stay below 2^32)
+    if (segs > 0x3fffff) return TQ_ERR_INVALID_ARGUMENT;
+    const bool any = p.cap > a->longer_than;
+    void* args[] = {&p};
+    if (any) {
+        if (!a->workspace || (uintptr_t)a->workspace % 256 ||
+            a->workspace_bytes < tq_kv8_evict_workspace_bytes(a->num_seqs, a->num_kv_heads, a->keep, a->block_size))
+            return TQ_ERR_WORKSPACE;
+        p.units = (a->keep + kUnit - 1) / kUnit;
+        p.blocks = (a->keep + a->block_size - 1) / a->block_size;
+        if (segs * p.units > 0x3ffffff) return TQ_ERR_INVALID_ARGUMENT;
+        uint8_t* at = static_cast<uint8_t*>(a->workspace);
+        const int64_t rows = segs * p.units * kUnit;
+        p.list = reinterpret_cast<int32_t*>(at);
+        at += align256(rows * 4);
+        p.shift = reinterpret_cast<uint16_t*>(at);
+        at += align256(rows * 2);
+        p.scales = reinterpret_cast<float2*>(at);
+        at += align256(segs * p.blocks * 8);
+        p.stage_mass = reinterpret_cast<float*>(at);
+        p.stage = at + align256(rows * 4);
+    }
+    hipError_t e = hipLaunchKernel((const void*)kv8_evict_plan_kernel, dim3((unsigned)segs), dim3(kPlan), args, 0, stream);
+    if (any) {
+        const unsigned units = (unsigned)((segs * p.units + 3) / 4), blocks = (unsigned)((segs * p.blocks + 3) / 4);
+        if (e == hipSuccess) e = hipLaunchKernel((const void*)kv8_evict_scales_kernel, dim3(blocks), dim3(256), args, 0, stream);
+        const void* gather = a->encoding == TQ_E4M3 ? (const void*)kv8_evict_gather_kernel<TQ_E4M3> : (const void*)kv8_evict_gather_kernel<TQ_INT8>;
+        if (e == hipSuccess) e = hipLaunchKernel(gather, dim3(units), dim3(256), args, 0, stream);
+        if (e == hipSuccess) e = hipLaunchKernel((const void*)kv8_evict_scatter_kernel, dim3(units), dim3(256), args, 0, stream);
+    }
+    if (e == hipSuccess) e = hipGetLastError();
+    return e == hipSuccess ? TQ_OK : (int)e;
+}

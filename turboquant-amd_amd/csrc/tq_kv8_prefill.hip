@@ -63,6 +63,7 @@ struct Cut {  // a segment that several workers share
 struct Prefill {
     Kv8Attn at;
     int max_q, causal, rows, row_bits, step, grow;  // rows of a segment, their log2; tokens between row blocks; of the first
+    int reach;  // with a window: a bound of the tokens in a row block's steps, up to the set-up share
     Cut* cuts;
     int* tickets;  // one per XCD, zeroed; NULL where the call is too small to be dealt by tickets
 };
@@ -72,6 +73,9 @@ struct Seq {
     int q0, nq, L, nrb;
     int step;
     int64_t a, U;  // tokens of row block rb: a + step rb; of all row blocks
+    // with a window, from row block `flat` on: F each; flat_at: of all before it
+    int flat;
+    int64_t F, flat_at;
 };
 // A value that is the same in all lanes, in scalar registers (loads and shuffles leave it in vector registers)
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -79,7 +83,7 @@ __device__ __forceinline__ int64_t uniform(int64_t x) {
     return (int64_t)(uint32_t)uniform((int)x) | (int64_t)uniform((int)(x >> 32)) << 32;
 }
 // (whole: every segment counts the same, so that a worker's share is one of them; SAME: s is the same in all lanes)
-template <bool SAME>
+template <bool SAME, bool WINDOW>
 __device__ __forceinline__ Seq seq_of(const Prefill& p, int s, bool whole) {
     Seq q;
     q.q0 = p.at.a.cu_seqlens_q[s];
@@ -97,7 +101,24 @@ __device__ __forceinline__ Seq seq_of(const Prefill& p, int s, bool whole) {
     q.a = whole ? kMinTokens : (p.causal ? past + p.grow : q.L) + kSegTokens;
     q.step = whole || !p.causal ? 0 : p.step;
     q.U = q.nrb * q.a + (int64_t)q.step * q.nrb * (q.nrb - 1) / 2;
+    if (WINDOW && !whole) {
+        q.F = p.reach + kSegTokens;
+        const int64_t k = q.a >= q.F ? 0 : (int64_t)((uint32_t)(q.F - q.a) + (uint32_t)q.step - 1) / (uint32_t)q.step;
+        if (k < q.nrb) {
+            q.flat = (int)k;
+            q.flat_at = k * q.a + (int64_t)q.step * k * (k - 1) / 2;
+            q.U = q.flat_at + (q.nrb - k) * q.F;
+        } else {
+            q.flat = q.nrb;
+            q.flat_at = q.U;
+        }
+    }
     return q;
+}
+// tokens of row block rb
+template <bool WINDOW>
+__device__ __forceinline__ int64_t tokens_of(const Seq& q, int rb, bool whole) {
+    return WINDOW && !whole && rb >= q.flat ? q.F : q.a + (int64_t)q.step * rb;
 }
 // tokens that the last row of row block rb sees
 __device__ __forceinline__ int visible(const Prefill& p, const Seq& q, int rb) {
@@ -107,7 +128,19 @@ __device__ __forceinline__ int visible(const Prefill& p, const Seq& q, int rb) {
     const int v = q.L - q.nq + i + 1;
     return v > 0 ? v : 0;
 }
-__device__ __forceinline__ int64_t before(const Seq& q, int64_t rb) { return rb * q.a + (int64_t)q.step * rb * (rb - 1) / 2; }
+// the steps of row block rb
+__device__ __forceinline__ Kv8Span span_of(const Prefill& p, const Seq& q, int rb) {
+    const int first = q.L - q.nq + (int)tq_udiv_apply((uint32_t)(rb * p.rows), p.at.group_div) + 1;
+    return kv8_span(kv8_window_from(first, p.at.window), visible(p, q, rb), p.at.sinks);
+}
+template <bool WINDOW>
+__device__ __forceinline__ int steps_of(const Prefill& p, const Seq& q, int rb) {
+    return WINDOW ? span_of(p, q, rb).n : (visible(p, q, rb) + 31) >> 5;
+}
+template <bool WINDOW>
+__device__ __forceinline__ int64_t before(const Seq& q, int64_t rb, bool whole) {
+    return WINDOW && !whole && rb > q.flat ? q.flat_at + (rb - q.flat) * q.F : rb * q.a + (int64_t)q.step * rb * (rb - 1) / 2;
+}
 // Tokens of the whole stream, and how it is dealt to the workers:
 //   whole     the segments, at kMinTokens each, if they are no more than the workers and the longest takes no longer
 //             than a cut one's worker and the merge;
@@ -116,16 +149,18 @@ __device__ __forceinline__ int64_t before(const Seq& q, int64_t rb) { return rb 
 //             demand 64 prompts of 64 to 200 tokens 86 -> 131);
 //   shares    otherwise.
 enum { kShares, kWhole, kTickets };
+template <bool WINDOW>
 __device__ __forceinline__ int64_t stream_total(const Prefill& p, int& dealt, int& most_rb) {
     const int lane = threadIdx.x & 63;
     int64_t P = 0, segs = 0;
     int longest = 0, last = 0, nrb = 0;
     for (int s = lane; s < p.at.a.num_seqs; s += 64) {
-        const Seq q = seq_of<false>(p, s, false);
+        const Seq q = seq_of<false, WINDOW>(p, s, false);
         P += q.U * p.at.a.num_kv_heads;
         segs += (int64_t)q.nrb * p.at.a.num_kv_heads;
-        longest = q.nrb && q.L > longest ? q.L : longest;
-        last = q.nrb && q.a > last ? (int)q.a : last;
+        const int len = WINDOW && q.L > p.reach ? p.reach : q.L, of_first = (int)(WINDOW && q.a > q.F ? q.F : q.a);
+        longest = q.nrb && len > longest ? len : longest;
+        last = q.nrb && of_first > last ? of_first : last;
         nrb = nrb > q.nrb ? nrb : q.nrb;
     }
     for (int m = 32; m >= 1; m >>= 1) {
@@ -176,13 +211,14 @@ struct Place {
     int64_t seg;  // stream position of the segment's start
 };
 // The segment that holds stream position pos (below the stream's total).
+template <bool WINDOW>
 __device__ __forceinline__ Place find(const Prefill& p, int64_t pos, bool whole, Seq& q) {
     const int lane = threadIdx.x & 63;
     const int hkv = p.at.a.num_kv_heads;
     int64_t P = 0;
     Place at = {0, 0, 0, 0};
     for (int s0 = 0; s0 < p.at.a.num_seqs; s0 += 64) {
-        const int64_t u = s0 + lane < p.at.a.num_seqs ? seq_of<false>(p, s0 + lane, whole).U * hkv : 0;
+        const int64_t u = s0 + lane < p.at.a.num_seqs ? seq_of<false, WINDOW>(p, s0 + lane, whole).U * hkv : 0;
         int64_t in = u;
         for (int d = 1; d < 64; d <<= 1) {
             const int64_t x = __shfl_up(in, d, 64);
@@ -200,7 +236,7 @@ __device__ __forceinline__ Place find(const Prefill& p, int64_t pos, bool whole,
     }
     at.s = uniform(at.s);
     at.seg = uniform(at.seg);
-    q = seq_of<true>(p, at.s, whole);
+    q = seq_of<true, WINDOW>(p, at.s, whole);
     int64_t off = pos - at.seg;
     // (estimates in double, put right in whole numbers)
     int kh = (int)((double)off / (double)q.U);
@@ -211,16 +247,18 @@ __device__ __forceinline__ Place find(const Prefill& p, int64_t pos, bool whole,
     off -= kh * q.U;
     const double h = (double)q.a - 0.5 * q.step;
     int rb = q.step ? (int)((__builtin_sqrt(h * h + 2.0 * q.step * (double)off) - h) / q.step) : (int)((double)off / h);
+    if (WINDOW && !whole && off >= q.flat_at) rb = q.flat + (int)((double)(off - q.flat_at) / (double)q.F);
     rb = rb < 0 ? 0 : (rb < q.nrb ? rb : q.nrb - 1);
-    while (rb > 0 && before(q, rb) > off) --rb;
-    while (rb + 1 < q.nrb && before(q, rb + 1) <= off) ++rb;
+    while (rb > 0 && before<WINDOW>(q, rb, whole) > off) --rb;
+    while (rb + 1 < q.nrb && before<WINDOW>(q, rb + 1, whole) <= off) ++rb;
     at.kh = uniform(kh);
     at.rb = uniform(rb);
-    at.seg += at.kh * q.U + before(q, at.rb);
+    at.seg += at.kh * q.U + before<WINDOW>(q, at.rb, whole);
     return at;
 }
 
-template <int ENC, bool FINE>
+// WINDOW: a segment's steps are those that the windows of its rows and the sinks touch
+template <int ENC, bool FINE, bool WINDOW>
 __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) {
     constexpr int kRT = FINE ? 1 : 2;     // 32-row tiles of a segment
     constexpr bool kQLds = !FINE;         // query operands in LDS
@@ -233,7 +271,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
 
     // ---- this worker's part of the stream ----
     int dealt, most_rb;
-    const int64_t P = stream_total(p, dealt, most_rb);
+    const int64_t P = stream_total<WINDOW>(p, dealt, most_rb);
     if (P == 0 || dealt == kTickets) {
         if (blockIdx.x == 0 && threadIdx.x == 0) p.cuts[0].rb = 0;  // nothing to merge
         if (P == 0) return;
@@ -252,7 +290,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
     int s = 0, kh = 0, rb = 0;
     int64_t seg = 0;
     if (dealt != kTickets) {
-        const Place place = find(p, p0, whole, q);
+        const Place place = find<WINDOW>(p, p0, whole, q);
         s = place.s;
         kh = place.kh;
         rb = place.rb;
@@ -261,7 +299,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
         // start and steps are left here
         Cut cut = {0, 0, 0, (int)share.R, 0, -1, 0};
         if (w > 0 && !whole) {
-            const int nsteps = (visible(p, q, rb) + 31) >> 5;
+            const int nsteps = steps_of<WINDOW>(p, q, rb);
             const int64_t before_this = share.at(w - 1), last = seg + 32 * (int64_t)(nsteps - 1);
             if (p0 > seg && before_this <= seg && nsteps > 0 && last >= p0) {
                 int w1 = w;
@@ -279,6 +317,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
     if (lane == 0) s_nan[wave] = 0;
     // the exponent base of rows whose scores lie beyond kKv8Far: their M stays kKv8None, so that every step moves it
     __shared__ float s_base[kWaves][kRT][64];
+    // WINDOW: exponent + 127 of the largest V scale among the tokens that the lane's row sees, of the steps where the rows'
+    // windows begin
+    __shared__ int s_vrow[WINDOW ? kWaves : 1][kRT][64];
     __shared__ int s_ticket[2][2];  // pair (-1: none left), row blocks from the last
     const int pairs = a.num_seqs * hkv;
     const int turns = (most_rb + kWaves - 1) / kWaves;
@@ -309,7 +350,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
         if (threadIdx.x == 0) take_ticket(turn);
         s = pair / hkv;
         kh = pair - s * hkv;
-        q = seq_of<true>(p, s, false);
+        q = seq_of<true, WINDOW>(p, s, false);
         rb = q.nrb - 1 - (kWaves * back + wave);
         return true;
     };
@@ -323,8 +364,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
     const uint32_t k_off = 128 * (n & 15) + 16 * h, v_off = 512 * h + 16 * n;
 
     while (dealt == kTickets || seg < p1) {
-        const int64_t u = q.a + (int64_t)q.step * rb;
-        const int nsteps = rb >= 0 ? (visible(p, q, rb) + 31) >> 5 : 0;
+        const int64_t u = tokens_of<WINDOW>(q, rb, whole);
+        const Kv8Span span = WINDOW && rb >= 0 ? span_of(p, q, rb) : Kv8Span{0, 0, 0, 0};
+        const int nsteps = WINDOW ? span.n : rb >= 0 ? (visible(p, q, rb) + 31) >> 5 : 0;
         int j0 = 0, j1 = nsteps;
         bool mine = dealt == kTickets ? rb >= 0 : seg >= p0;
         if (dealt == kShares) {
@@ -347,6 +389,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
             // tokens that every row sees
             const int least = p.causal ? q.L - q.nq + (int)tq_udiv_apply((uint32_t)(rb * kRows), p.at.group_div) + 1 : q.L;
 
+            // (WINDOW: rows see from there on, the sinks apart; the last row's window begins at most at `behind_lo`)
+            int lo[WINDOW ? kRT : 1];
+            int behind_lo = 0;
+            if (WINDOW) {
+                int i = (int)tq_udiv_apply((uint32_t)(rb * kRows + kRows - 1), p.at.group_div);
+                i = i < q.nq - 1 ? i : q.nq - 1;
+                behind_lo = kv8_window_from(q.L - q.nq + i + 1, p.at.window);
+            }
+            auto step_of = [&](int j) -> int { return WINDOW ? span.step(j) : j; };
+            // some rows do not see all tokens of step js (of the sequence), by its position alone
+            auto low_edge = [&](int js) -> bool { return WINDOW && 32 * js < behind_lo && 32 * js + 32 > p.at.sinks; };
+            auto edge = [&](int js) -> bool { return 32 * js + 32 > least || low_edge(js); };
+
             // ---- the query rows ----
             int seen[kRT];
             float c1[kRT];
@@ -359,6 +414,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                 const bool real = i < computed;
                 const int sn = p.causal ? q.L - q.nq + i + 1 : q.L;  // tokens that the row sees
                 seen[rt] = real && sn > 0 ? (sn < q.L ? sn : q.L) : 0;
+                if (WINDOW) lo[WINDOW ? rt : 0] = kv8_window_from(sn, p.at.window);
                 const int64_t off = (int64_t)(q.q0 + (real ? i : 0)) * a.q_stride_token + (int64_t)(real ? head : 0) * a.q_stride_head + 16 * h;
                 float x[32], y[32], m = 0.f;
                 kv8_load32(a.q, off, 32, a.q_dtype, x);
@@ -392,7 +448,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                 int what;  // rows in use, K's exponent << 8, V's exponent << 16, both + 127
             };
             auto tiles_from = [&](int t0) -> Tiles {
-                const int ti = t0 + lane;
+                const int ti = 2 * step_of((t0 + lane) >> 1) + ((t0 + lane) & 1);
                 const int tc = ti < last_tile ? ti : last_tile;  // (behind the last: a valid address, no rows)
                 const int b = (int)tq_udiv_apply((uint32_t)tc, p.at.tpb_div);
                 int blk = bt[b];
@@ -402,6 +458,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                     blk = 0;
                     nv = 0;
                 }
+                // (no row sees any of the tile)
+                if (WINDOW && 16 * ti >= p.at.sinks && 16 * ti + 16 <= span.lo) nv = 0;
                 const uint64_t kblk = (uint64_t)kb + blk * a.k_stride_block, vblk = (uint64_t)vb + blk * a.v_stride_block;
                 const uint32_t ke = *reinterpret_cast<const uint32_t*>(kb + blk * a.k_stride_block + scale_at) >> 23;
                 const uint32_t ve = *reinterpret_cast<const uint32_t*>(vb + blk * a.v_stride_block + scale_at) >> 23;
@@ -434,6 +492,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
             float M[kRT], lsum[kRT];
             bool far = false;  // s_base holds the rows' bases
             int vref = 0;  // exponent + 127 of the largest V scale so far (0: none)
+            // WINDOW: where rows' windows begin, a row does not see tokens before it that others do.  A scale of those far from
+            // vref (kVFar) must not cost it bits: from then on (`mixed`) each row's sums have an exponent of their own, in s_vrow,
+            // and the probabilities carry the difference.
+            constexpr int kVFar = 12;
+            int vall = 0;  // the largest of the tiles that no window begins in
+            bool lows = false, mixed = false;
             f32x16 acc[kRT][4];
 #pragma unroll
             for (int rt = 0; rt < kRT; ++rt) {
@@ -503,15 +567,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                         }
                     }
                     load_keys(cur, i + 2);
-                    if (32 * j + 32 > least || nv[0] + nv[1] != 32) {
+                    const int js = step_of(j);
+                    if (edge(js) || nv[0] + nv[1] != 32) {
 #pragma unroll
                         for (int rt = 0; rt < kRT; ++rt)
 #pragma unroll
                             for (int t = 0; t < 2; ++t) {
-                                const int sn = seen[rt] - 32 * j - 16 * t, upto = (sn < nv[t] ? sn : nv[t]) - 4 * h;
+                                const int at = 32 * js + 16 * t;
+                                const int sn = seen[rt] - at, upto = (sn < nv[t] ? sn : nv[t]) - 4 * h;
+                                const int from = p.at.sinks - at - 4 * h, until = WINDOW ? lo[WINDOW ? rt : 0] - at - 4 * h : 0;
 #pragma unroll
-                                for (int v = 0; v < 8; ++v)
-                                    if (8 * (v >> 2) + (v & 3) >= upto) sc[rt][8 * t + v] = kKv8NegInf;
+                                for (int v = 0; v < 8; ++v) {
+                                    const int x = 8 * (v >> 2) + (v & 3);
+                                    if (x >= upto || (WINDOW && x >= from && x < until)) sc[rt][8 * t + v] = kKv8NegInf;
+                                }
                             }
 #pragma unroll
                         for (int t = 0; t < 2; ++t) {
@@ -524,7 +593,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                         }
                         // (a NaN among the values must not reach the rows that do not see its token, as 0 * NaN: here its code
                         // becomes 0, and the rows that do see it get theirs after the stores)
-                        if (ENC == TQ_E4M3 && 32 * j + 32 > least) {
+                        if (ENC == TQ_E4M3 && edge(js)) {
                             uint32_t nans = 0;
 #pragma unroll
                             for (int t = 0; t < 2; ++t)
@@ -608,6 +677,54 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                     }
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
+                        if (WINDOW) {
+                            const bool low = low_edge(js);
+                            const int at = 32 * js + 16 * t;
+                            auto sees = [&](int rt) -> bool {
+                                return seen[rt] > at && (lo[WINDOW ? rt : 0] < at + 16 || at < p.at.sinks);
+                            };
+                            if (low && !lows) {
+#pragma unroll
+                                for (int rt = 0; rt < kRT; ++rt) s_vrow[WINDOW ? wave : 0][rt][lane] = 0;
+                                lows = true;
+                            }
+                            if (!mixed && lows && vref && ve[t] && (ve[t] + kVFar < vref || (low && ve[t] > vref + kVFar))) {
+#pragma unroll
+                                for (int rt = 0; rt < kRT; ++rt) {
+                                    const int old = s_vrow[WINDOW ? wave : 0][rt][lane], u = old > vall ? old : vall;
+                                    // (a row that has seen nothing has sums of 0)
+                                    const float r = u ? kv8_scale(127 + vref - u < 254 ? 127 + vref - u : 254) : 0.f;
+#pragma unroll
+                                    for (int d = 0; d < 4; ++d) acc[rt][d] *= r;
+                                    s_vrow[WINDOW ? wave : 0][rt][lane] = u;
+                                }
+                                mixed = true;
+                            }
+                            if (mixed) {
+#pragma unroll
+                                for (int rt = 0; rt < kRT; ++rt) {
+                                    int u = s_vrow[WINDOW ? wave : 0][rt][lane];
+                                    const bool see = sees(rt);
+                                    const float r = see && ve[t] > u ? (u && u + 126 > ve[t] ? kv8_scale(127 + u - ve[t]) : 0.f) : 1.f;
+                                    u = see && ve[t] > u ? ve[t] : u;
+#pragma unroll
+                                    for (int d = 0; d < 4; ++d) acc[rt][d] *= r;
+                                    s_vrow[WINDOW ? wave : 0][rt][lane] = u;
+                                    const _Float16 f = (_Float16)(see ? kv8_step(ve[t] - u) : 0.f);
+                                    ph[rt][t] *= f;
+                                    if (FINE) pl[FINE ? rt : 0][t] *= f;
+                                }
+                                vref = ve[t];  // (V as it is)
+                            } else if (low) {
+#pragma unroll
+                                for (int rt = 0; rt < kRT; ++rt) {
+                                    const int old = s_vrow[WINDOW ? wave : 0][rt][lane];
+                                    if (sees(rt) && ve[t] > old) s_vrow[WINDOW ? wave : 0][rt][lane] = ve[t];
+                                }
+                            } else {
+                                vall = vall > ve[t] ? vall : ve[t];
+                            }
+                        }
                         // (tile by tile: a row that sees the first alone keeps all bits of it)
                         if (ve[t] > vref) {  // wave-uniform
                             const float r = kv8_scale(127 + vref - ve[t] > 0 ? 127 + vref - ve[t] : 0);
@@ -640,7 +757,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                 int i, head;
                 row_of(rt, i, head);
                 // (a piece is divided by its own sum: plain sums of large values pass fp32's range)
-                const float f = l == 0.f ? 0.f : kv8_scale(vref) / l;
+                const int vexp = WINDOW && mixed ? s_vrow[WINDOW ? wave : 0][rt][lane] : vref;
+                const float f = l == 0.f ? 0.f : kv8_scale(vexp) / l;
                 if (i < computed) {
                     const int64_t row = (int64_t)(2 * w + (seg > p0 ? 1 : 0)) * kRows + 32 * rt + n;
                     const int64_t at = complete ? (int64_t)(q.q0 + i) * a.out_stride_token + (int64_t)head * a.out_stride_head : row * TQ_HEAD_DIM;
@@ -664,8 +782,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
             if (ENC == TQ_E4M3 && uniform(s_nan[wave])) {
                 s_nan[wave] = 0;
                 __threadfence_block();
-                const int from = least > 32 * j0 ? least & ~31 : 32 * j0, to = 32 * j1 < q.L ? 32 * j1 : q.L;
-                for (int t = from; t < to; ++t) {
+                const int from = WINDOW || least <= 32 * j0 ? 32 * j0 : least & ~31, to = WINDOW || 32 * j1 < q.L ? 32 * j1 : q.L;
+                for (int x = from; x < to; ++x) {
+                    const int t = 32 * step_of(x >> 5) + (x & 31);
+                    if (t >= q.L) break;
                     const int b = (int)tq_udiv_apply((uint32_t)(t >> 4), p.at.tpb_div), in = t - b * a.block_size;
                     const int blk = bt[b];
                     if ((uint32_t)blk >= (uint64_t)a.num_blocks) continue;
@@ -673,10 +793,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                     for (int d = lane; d < TQ_HEAD_DIM; d += 64) {
                         if ((codes[4 * d] & 0x7f) != 0x7f) continue;
                         for (int r = 0; r < kRows; ++r) {
-                            const uint32_t x = (uint32_t)(rb * kRows + r);
-                            const int i = (int)tq_udiv_apply(x, p.at.group_div);
+                            const uint32_t row = (uint32_t)(rb * kRows + r);
+                            const int i = (int)tq_udiv_apply(row, p.at.group_div);
                             if (i >= computed || t >= (p.causal ? q.L - q.nq + i + 1 : q.L)) continue;
-                            const int head = kh * group + (int)(x - (uint32_t)i * (uint32_t)group);
+                            if (WINDOW && t >= p.at.sinks && t < kv8_window_from(q.L - q.nq + i + 1, p.at.window)) continue;
+                            const int head = kh * group + (int)(row - (uint32_t)i * (uint32_t)group);
                             if (complete) tq_store1(a.out, (int64_t)(q.q0 + i) * a.out_stride_token + (int64_t)head * a.out_stride_head + d, a.out_dtype, __builtin_nanf(""));
                             else p.at.ws_acc[((int64_t)(2 * w + (seg > p0 ? 1 : 0)) * kRows + r) * TQ_HEAD_DIM + d] = __builtin_nanf("");
                         }
@@ -697,7 +818,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_prefill_kernel(Prefill p) 
                 do {
                     ++s;
                     if (s >= a.num_seqs) return;
-                    q = seq_of<true>(p, s, whole);
+                    q = seq_of<true, WINDOW>(p, s, whole);
                 } while (q.nrb == 0);
             }
         }
@@ -771,11 +892,10 @@ extern "C" int64_t tq_kv8_prefill_workspace_bytes(int num_seqs, int max_q_len, i
     return w * (2 * 64 * (TQ_HEAD_DIM + 2) * 4 + (int64_t)sizeof(Cut)) + 8 * 4;
 }
 
-extern "C" int tq_kv8_prefill(const tq_kv8_attn_args* a, tq_stream_t stream) {
-    if (!a) return TQ_ERR_INVALID_ARGUMENT;
-    Prefill p = {};
-    const int rc = tq_kv8_attn_setup(a, &p.at);
-    if (rc != TQ_OK) return rc;
+namespace {
+
+int launch_prefill(Prefill& p, bool window, tq_stream_t stream) {
+    const tq_kv8_attn_args* a = &p.at.a;
     if (a->max_q_len < 0 || (a->flags & ~TQ_PREFILL_CAUSAL)) return TQ_ERR_INVALID_ARGUMENT;
     if (a->num_seqs == 0 || a->max_q_len == 0) return TQ_OK;
     if (!a->q || !a->out || !a->k_cache || !a->v_cache || (!a->block_tables && a->max_blocks_per_seq) || !a->seq_lens || !a->cu_seqlens_q)
@@ -797,6 +917,9 @@ extern "C" int tq_kv8_prefill(const tq_kv8_attn_args* a, tq_stream_t stream) {
     p.rows = 1 << p.row_bits;
     p.step = (p.rows + p.at.group - 1) / p.at.group;
     p.grow = (p.rows - 1) / p.at.group + 1;
+    // (its first row's window, the rows' own tokens, the sinks; a step more at most at each end, which the set-up share holds)
+    const int64_t reach = (int64_t)p.at.window + p.grow + p.at.sinks;
+    p.reach = (int)(reach < kKv8MaxLen ? reach : kKv8MaxLen);
     p.at.ws_acc = static_cast<float*>(a->workspace);
     p.at.ws_ml = p.at.ws_acc + most * 2 * 64 * TQ_HEAD_DIM;
     int* tickets = reinterpret_cast<int*>(p.at.ws_ml + most * 2 * 64 * 2);
@@ -806,8 +929,12 @@ extern "C" int tq_kv8_prefill(const tq_kv8_attn_args* a, tq_stream_t stream) {
     const int64_t blocks = ((int64_t)a->max_q_len * p.at.group + p.rows - 1) / p.rows;
     if (pairs <= 0x7fffff && blocks <= 0x7fffffff / pairs && pairs * blocks >= resident && p.at.workers == resident && resident % 8 == 0)
         p.tickets = tickets;
-    const void* kern = a->encoding == TQ_E4M3 ? (fine ? (const void*)kv8_prefill_kernel<TQ_E4M3, true> : (const void*)kv8_prefill_kernel<TQ_E4M3, false>)
-                                              : (fine ? (const void*)kv8_prefill_kernel<TQ_INT8, true> : (const void*)kv8_prefill_kernel<TQ_INT8, false>);
+    const void* kern = nullptr;
+#define TQ_PREFILL(E, F, W) \
+    if (a->encoding == E && fine == F && window == W) kern = (const void*)kv8_prefill_kernel<E, F, W>;
+    TQ_PREFILL(TQ_E4M3, false, false) TQ_PREFILL(TQ_E4M3, true, false) TQ_PREFILL(TQ_E4M3, false, true) TQ_PREFILL(TQ_E4M3, true, true)
+    TQ_PREFILL(TQ_INT8, false, false) TQ_PREFILL(TQ_INT8, true, false) TQ_PREFILL(TQ_INT8, false, true) TQ_PREFILL(TQ_INT8, true, true)
+#undef TQ_PREFILL
     const unsigned lds = fine ? 0 : kWaves * 8 * 2 * 64 * 16;  // 64 KB
     // one wave per workgroup while the workers are few: they spread over the compute units
     int64_t grid = (int64_t)cus * (kWavesPerCu / kWaves);
@@ -823,4 +950,22 @@ extern "C" int tq_kv8_prefill(const tq_kv8_attn_args* a, tq_stream_t stream) {
         e = hipLaunchKernel((const void*)kv8_prefill_merge_kernel, dim3((unsigned)p.at.workers - 1, (unsigned)p.rows / 8), dim3(256), args, 0, stream);
     if (e == hipSuccess) e = hipGetLastError();
     return e == hipSuccess ? TQ_OK : (int)e;
+}
+
+}  // namespace
+
+extern "C" int tq_kv8_prefill(const tq_kv8_attn_args* a, tq_stream_t stream) {
+    if (!a) return TQ_ERR_INVALID_ARGUMENT;
+    Prefill p = {};
+    const int rc = tq_kv8_attn_setup(a, &p.at);
+    return rc != TQ_OK ? rc : launch_prefill(p, false, stream);
+}
+
+extern "C" int tq_kv8_prefill_window(const tq_kv8_window_args* w, tq_stream_t stream) {
+    if (!w) return TQ_ERR_INVALID_ARGUMENT;
+    Prefill p = {};
+    const int rc = tq_kv8_window_setup(w, &p.at);
+    if (rc != TQ_OK) return rc;
+    if (w->mass || (w->window && !(w->attn.flags & TQ_PREFILL_CAUSAL))) return TQ_ERR_INVALID_ARGUMENT;
+    return launch_prefill(p, w->window != 0, stream);
 }

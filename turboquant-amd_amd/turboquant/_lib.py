@@ -165,6 +165,13 @@ SIGNATURES = {
     "tq_kv8_prefill": (_i32, [ctypes.c_char_p, _vp]),
     "tq_kv8_decode_workspace_bytes": (_i64, [_i32, _i32, _i32]),
     "tq_kv8_prefill_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "tq_kv8_decode_window": (_i32, [ctypes.c_char_p, _vp]),
+    "tq_kv8_prefill_window": (_i32, [ctypes.c_char_p, _vp]),
+    "tq_kv8_decode_window_workspace_bytes": (_i64, [_i32] * 7),
+    "tq_kv8_observe": (_i32, [ctypes.c_char_p, _vp]),
+    "tq_kv8_observe_workspace_bytes": (_i64, [_i32] * 5),
+    "tq_kv8_evict": (_i32, [ctypes.c_char_p, _vp]),
+    "tq_kv8_evict_workspace_bytes": (_i64, [_i32] * 4),
     "tq_rope": (_i32, [ctypes.c_char_p, _vp]),
     "tq_plan_step": (_i32, [ctypes.c_char_p, _vp]),
     "tq_plan_step_workspace_bytes": (_i64, [_i32]),

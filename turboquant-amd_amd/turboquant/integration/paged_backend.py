@@ -16,7 +16,8 @@ the hot path is here, in the shapes the reference's backends use:
   keeps its own attention for them, as the reference does), or, with `protected_bits`, get a
   4-bit (or other) packed format of their own, or with protected_bits=8 a cache of 8 bits a value.
 - TurboQuantPaged8State: the state of such a layer, or of all with k_bits=8 (kernels.paged8), with the methods that
-  TurboQuantPagedImpl calls, so that it runs on either.
+  TurboQuantPagedImpl calls, so that it runs on either; and the layer's part of a session in bounded memory:
+  observe and evict (kernels.evict8).
 - TurboQuantPagedImpl: an attention implementation in vLLM's shape
   (TurboQuantFP4Impl.do_kv_cache_update / forward and TurboQuantFP4Backend.get_kv_cache_shape,
   integration/tq_fp4_backend.py:389-735).  One uint8 tensor [num_blocks, num_kv_heads,
@@ -36,6 +37,7 @@ import torch
 
 from turboquant.core import make_codebook, make_wht_matrix
 from turboquant.kernels.paged import PagedKVFormat, compress_paged, compress_paged_kv, decode_paged, prefill_paged
+from turboquant.kernels.evict8 import allocate_mass, evict_paged8, observe_paged8
 from turboquant.kernels.paged8 import Paged8Format, decode_paged8, prefill_paged8, quantize_paged8_kv
 from turboquant.kernels.plan import StepPlan
 from turboquant.kernels.rotation import wht_rows
@@ -186,19 +188,40 @@ class TurboQuantPaged8State:
     def decode(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
                seq_lens: torch.Tensor, sm_scale: Optional[float] = None, sparse_threshold: float = 0.0,
                max_seq_len: Optional[int] = None, seq_lens_host: Optional[Sequence[int]] = None,
-               out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+               out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None,
+               window: Optional[int] = None, sinks: int = 0, mass: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Decode attention of q [S, Hq, 128].  sparse_threshold and seq_lens_host are taken for the packed state's
-        sake: every token's values are read, and the split over the keys is planned on the device."""
+        sake: every visible token's values are read, and the split over the keys is planned on the device."""
         return decode_paged8(q, k_cache, self.k_format, v_cache, self.v_format, block_tables, seq_lens, sm_scale=sm_scale,
-                             max_seq_len=max_seq_len, out=out, workspace=workspace)
+                             max_seq_len=max_seq_len, out=out, workspace=workspace, window=window, sinks=sinks, mass=mass)
 
     def prefill(self, q: torch.Tensor, cu_seqlens_q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                 block_tables: torch.Tensor, seq_lens: torch.Tensor, sm_scale: Optional[float] = None,
                 max_q_len: Optional[int] = None, out: Optional[torch.Tensor] = None,
-                causal: bool = True) -> torch.Tensor:
+                causal: bool = True, window: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
         """Prefill / extend attention of q [T, Hq, 128] (new tokens of each sequence, already in the cache)."""
         return prefill_paged8(q, cu_seqlens_q, k_cache, self.k_format, v_cache, self.v_format, block_tables, seq_lens,
-                              sm_scale=sm_scale, causal=causal, max_q_len=max_q_len, out=out)
+                              sm_scale=sm_scale, causal=causal, max_q_len=max_q_len, out=out, window=window, sinks=sinks)
+
+    # ---- accumulated weights and eviction (kernels.evict8) ----
+    def allocate_mass(self, num_blocks: int, num_kv_heads: int, device=None) -> torch.Tensor:
+        """Accumulated attention weights of a cache of num_blocks blocks."""
+        return allocate_mass(num_blocks, num_kv_heads, self.block_size, device if device is not None else self.device)
+
+    def observe(self, q: torch.Tensor, cu_seqlens_q: torch.Tensor, k_cache: torch.Tensor, block_tables: torch.Tensor,
+                seq_lens: torch.Tensor, mass: torch.Tensor, sm_scale: Optional[float] = None, last: Optional[int] = None,
+                max_q_len: Optional[int] = None, max_seq_len: Optional[int] = None, window: Optional[int] = None,
+                sinks: int = 0) -> torch.Tensor:
+        """Add the weights that the last queries of prompts give to the cached tokens to mass."""
+        return observe_paged8(q, cu_seqlens_q, k_cache, self.k_format, block_tables, seq_lens, mass, sm_scale=sm_scale, last=last,
+                              max_q_len=max_q_len, max_seq_len=max_seq_len, window=window, sinks=sinks)
+
+    def evict(self, k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor, block_tables: torch.Tensor,
+              seq_lens: torch.Tensor, keep: int, recent: int = 0, sinks: int = 0, longer_than: Optional[int] = None,
+              max_seq_len: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Cut long sequences to `keep` tokens, in place; returns the lengths' changes (plan_step's new_lens)."""
+        return evict_paged8(k_cache, self.k_format, v_cache, self.v_format, mass, block_tables, seq_lens, keep, recent=recent,
+                            sinks=sinks, longer_than=longer_than, max_seq_len=max_seq_len, out=out)
 
 
 def _check_8bit(v_bits: Optional[int], k_qjl: bool) -> None:
@@ -323,14 +346,20 @@ class PagedDecodeMetadata:
 class TurboQuantPagedImpl:
     """Attention over a packed or 8-bit paged cache, in the shape of a vLLM AttentionImpl.
 
-    sparse_threshold acts on packed caches; over an 8-bit one every token's values are read.  Decode takes up to 16
-    query heads per KV head on either, prefill any number.
+    sparse_threshold acts on packed caches; over an 8-bit one every visible token's values are read.  Decode takes up to
+    16 query heads per KV head on either, prefill any number.
+
+    Over an 8-bit cache alone: sliding_window (None: every token) and sinks, the tokens at a sequence's start that
+    stay visible; mass, accumulated attention weights (state.allocate_mass) to which forward adds those of every decode
+    query and of the last observe_last queries of every prompt, for state.evict.
     """
 
     forward_includes_kv_cache_update = False  # do_kv_cache_update is called separately
 
     def __init__(self, num_heads: int, head_size: int, scale: float, num_kv_heads: int,
-                 state: TurboQuantPagedState | TurboQuantPaged8State, sparse_threshold: float = 0.0):
+                 state: TurboQuantPagedState | TurboQuantPaged8State, sparse_threshold: float = 0.0,
+                 sliding_window: Optional[int] = None, sinks: int = 0, mass: Optional[torch.Tensor] = None,
+                 observe_last: int = 32):
         if num_heads % num_kv_heads:
             raise ValueError("num_heads must be a multiple of num_kv_heads")
         if head_size != state.head_size:
@@ -341,6 +370,15 @@ class TurboQuantPagedImpl:
         self.num_kv_heads = num_kv_heads
         self.state = state
         self.sparse_threshold = float(sparse_threshold)
+        if not isinstance(state, TurboQuantPaged8State) and (sliding_window is not None or mass is not None):
+            raise ValueError("sliding_window and mass need an 8-bit cache (TurboQuantPaged8State)")
+        if sliding_window is None and sinks:
+            raise ValueError("sinks need a sliding_window: without one every token is visible")
+        if (sliding_window is not None and sliding_window < 1) or sinks < 0 or observe_last < 1:
+            raise ValueError("sliding_window and observe_last must be positive, sinks not negative")
+        self.mass = mass
+        self.observe_last = observe_last
+        self.reach = {} if sliding_window is None else dict(window=sliding_window, sinks=sinks)
 
     @staticmethod
     def get_supported_kernel_block_sizes() -> list[int]:
@@ -394,9 +432,10 @@ class TurboQuantPagedImpl:
             q = query[:nd].view(nd, self.num_heads, self.head_size)
             out = output[:nd].view(nd, self.num_heads, self.head_size)
             lens_host = md.seq_lens_host[:nd] if md.seq_lens_host is not None else None
+            weigh = {} if self.mass is None else dict(mass=self.mass)
             self.state.decode(q, k_cache, v_cache, md.block_tables[:nd], md.seq_lens[:nd],
                               sm_scale=self.scale, sparse_threshold=self.sparse_threshold,
-                              max_seq_len=md.max_seq_len, seq_lens_host=lens_host, out=out)
+                              max_seq_len=md.max_seq_len, seq_lens_host=lens_host, out=out, **self.reach, **weigh)
         if nd < S:
             qsl = md.query_start_loc
             t0 = nd  # decode tokens come first, one per sequence
@@ -405,5 +444,8 @@ class TurboQuantPagedImpl:
             q = query[t0:].view(tp, self.num_heads, self.head_size)
             out = output[t0:].view(tp, self.num_heads, self.head_size)
             self.state.prefill(q, cu, k_cache, v_cache, md.block_tables[nd:], md.seq_lens[nd:], sm_scale=self.scale,
-                               max_q_len=md.max_query_len, out=out)
+                               max_q_len=md.max_query_len, out=out, **self.reach)
+            if self.mass is not None:
+                self.state.observe(q, cu, k_cache, md.block_tables[nd:], md.seq_lens[nd:], self.mass, sm_scale=self.scale,
+                                   last=self.observe_last, max_q_len=md.max_query_len, max_seq_len=md.max_seq_len, **self.reach)
         return output

@@ -154,11 +154,36 @@ def quantize_paged8_kv(
 
 
 _ATTN = struct.Struct("@8Q11q12ifi")
+_REACH = struct.Struct("@Q2q4i")  # what tq_kv8_window_args has behind tq_kv8_attn_args
 _SCALE = 1.0 / math.sqrt(128)
 
 
+def _check_window(window: Optional[int], sinks: int) -> tuple[int, int]:
+    """(window or 0, sinks) as the C entries take them."""
+    if window is None:
+        if sinks:
+            raise ValueError("sinks need a window: without one every token is visible")
+        return 0, 0
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window must be positive and sinks not negative, got {window} and {sinks}")
+    return min(int(window), 0x7fffffff), min(int(sinks), 0x7fffffff)
+
+
+def _check_mass(mass: torch.Tensor, num_blocks: int, heads: int, block_size: int) -> tuple[int, int]:
+    """The block and head strides of accumulated weights."""
+    if mass.dtype != torch.float32 or mass.shape != (num_blocks, heads, block_size):
+        raise ValueError(f"mass must be float32 [{num_blocks}, {heads}, {block_size}]")
+    sb, sh, s1 = mass.stride()
+    if s1 != 1 or (sb | sh) % 4 or mass.data_ptr() % 16:
+        raise ValueError("mass must have unit inner stride and 16-byte aligned rows")
+    near, far = ((sh, heads), (sb, num_blocks)) if sh <= sb else ((sb, num_blocks), (sh, heads))
+    if (near[1] > 1 and near[0] < block_size) or (far[1] > 1 and far[0] < max(block_size, near[0] * near[1])):
+        raise ValueError("rows of mass share memory")
+    return sb, sh
+
+
 def _attention(name, dev, q, caches, k_cache, v_cache, k_fmt, block_tables, seq_lens, cu_seqlens_q, sm_scale, max_seq_len,
-               max_q_len, flags, out, workspace):
+               max_q_len, flags, out, workspace, window=None, sinks=0, mass=None):
     rows, hq, _ = q.shape
     nb, hkv, kb, kh, vb, vh = caches
     S, mb = block_tables.shape if block_tables.dim() == 2 else (-1, 0)
@@ -175,6 +200,12 @@ def _attention(name, dev, q, caches, k_cache, v_cache, k_fmt, block_tables, seq_
     scale = _SCALE if sm_scale is None else float(sm_scale)
     if not math.isfinite(scale):
         raise ValueError("sm_scale must be finite")
+    window, sinks = _check_window(window, sinks)
+    reach = b""
+    if window or mass is not None:
+        ms = _check_mass(mass, nb, hkv, k_fmt.block_size) if mass is not None else (0, 0)
+        reach = _REACH.pack(0 if mass is None else mass.data_ptr(), *ms, window, sinks, 0, 0)
+        name += "_window"
     seq_lens = seq_lens.contiguous()
     q = _rows(q)
     if out is None:
@@ -191,7 +222,8 @@ def _attention(name, dev, q, caches, k_cache, v_cache, k_fmt, block_tables, seq_
         ot, oh, _ = target.stride()
     L = _lib.lib()
     if cu_seqlens_q is None:
-        need = L.tq_kv8_decode_workspace_bytes(S, hq, hkv)
+        need = (L.tq_kv8_decode_window_workspace_bytes(S, hq, hkv, max_seq_len, window, sinks, 1) if mass is not None else
+                L.tq_kv8_decode_workspace_bytes(S, hq, hkv))
     else:
         need = L.tq_kv8_prefill_workspace_bytes(S, max_q_len, hq, hkv, mb, k_fmt.block_size)
     if workspace is None:
@@ -206,7 +238,7 @@ def _attention(name, dev, q, caches, k_cache, v_cache, k_fmt, block_tables, seq_
                       qt, qh, ot, oh, kb, kh, vb, vh, nb, block_tables.stride(0) if S > 1 else mb, _lib.dtype_code(q),
                       _lib.dtype_code(target), k_fmt.encoding_code, S, hq, hkv, 128, k_fmt.block_size, mb, max_seq_len,
                       max_q_len, flags, scale, 0)
-    _lib.launch(name, dev, args)
+    _lib.launch(name, dev, args + reach)
     if target is not out:
         out.copy_(target)
     return out
@@ -224,6 +256,9 @@ def decode_paged8(
     max_seq_len: Optional[int] = None,
     out: Optional[torch.Tensor] = None,
     workspace: Optional[torch.Tensor] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
+    mass: Optional[torch.Tensor] = None,
 ) -> torch.Tensor:
     """Attention of one query token per sequence, q [S, Hq, 128], over 8-bit paged K/V caches.
 
@@ -233,10 +268,16 @@ def decode_paged8(
     to fp16 (probabilities below 2^-39 of the row's largest count as zero), with f32 on either side they are
     carried in twice the precision.  V enters relative to the largest scale so far of the sequence's blocks: exact
     down to 2^-15 of it, zero below 2^-24.  A sequence of length 0 gives zeros; a NaN in the cache reaches the
-    heads that see it.  workspace: uint8 of tq_kv8_decode_workspace_bytes(...) for callers that keep one (calls that
-    overlap must not share it).
+    heads that see it.  workspace: uint8 of tq_kv8_decode_workspace_bytes(...), with mass
+    tq_kv8_decode_window_workspace_bytes(...), for callers that keep one (calls that overlap must not share it).
+
+    window: each sequence's query sees the last `window` tokens and the first `sinks` alone, and no others are read.
+    mass: float32 [num_blocks, Hkv, block_size] (kernels.evict8.allocate_mass), accumulated weights: every token that the
+    query sees gets the softmax weights of its KV head's query heads added, in fp32 and in place; the sequence's last token, which
+    this step wrote, starts from 0.  A weight that is not a number adds nothing.  With mass, blocks must
+    belong to one sequence.
     """
-    dev = _lib.require_gpu("decode_paged8", q, k_cache, v_cache, block_tables, seq_lens, out, workspace)
+    dev = _lib.require_gpu("decode_paged8", q, k_cache, v_cache, block_tables, seq_lens, out, workspace, mass)
     if q.dim() != 3 or q.shape[2] != 128:
         raise ValueError("q must be [S, Hq, 128]")
     if seq_lens.dim() != 1 or seq_lens.shape[0] != q.shape[0]:
@@ -247,7 +288,7 @@ def decode_paged8(
     cap = min(block_tables.shape[-1] * k_fmt.block_size, 0x7fff0000) if block_tables.dim() else 0
     msl = cap if max_seq_len is None else max(0, min(int(max_seq_len), cap))
     return _attention("tq_kv8_decode", dev, q, caches, k_cache, v_cache, k_fmt, block_tables, seq_lens, None, sm_scale, msl, 1,
-                      0, out, workspace)
+                      0, out, workspace, window, sinks, mass)
 
 
 def prefill_paged8(
@@ -264,6 +305,8 @@ def prefill_paged8(
     max_q_len: Optional[int] = None,
     out: Optional[torch.Tensor] = None,
     workspace: Optional[torch.Tensor] = None,
+    window: Optional[int] = None,
+    sinks: int = 0,
 ) -> torch.Tensor:
     """Attention of several new tokens per sequence, q [T, Hq, 128], over 8-bit paged K/V caches.
 
@@ -274,6 +317,10 @@ def prefill_paged8(
     max_q_len: host-side bound of the query counts (default: T).  Rows of q that belong to no sequence are
     left as they were in out.  Types, roundings and workspace as in decode_paged8, but 16-bit calls round probabilities below
     2^-18 of the row's largest to fewer bits and those below 2^-29 to zero.
+
+    window (needs causal): the query at position p sees the tokens from p - window + 1 on and the first `sinks`
+    alone; tokens that no row sees are not read.  V's largest scale so far then counts the tokens that a row's block of
+    64 rows sees.
     """
     dev = _lib.require_gpu("prefill_paged8", q, cu_seqlens_q, k_cache, v_cache, block_tables, seq_lens, out, workspace)
     if q.dim() != 3 or q.shape[2] != 128:
@@ -282,8 +329,11 @@ def prefill_paged8(
         raise ValueError("seq_lens must be [num_seqs] and cu_seqlens_q [num_seqs + 1]")
     if cu_seqlens_q.dtype != torch.int32:
         raise TypeError("cu_seqlens_q must be int32")
+    if window is not None and not causal:
+        raise ValueError("a window needs causal=True")
     caches = _check_pair(k_cache, k_fmt, v_cache, v_fmt, "prefill_paged8")
     T = q.shape[0]
     mq = T if max_q_len is None else max(0, min(int(max_q_len), T))
     return _attention("tq_kv8_prefill", dev, q, caches, k_cache, v_cache, k_fmt, block_tables, seq_lens,
-                      cu_seqlens_q.contiguous(), sm_scale, 0, mq, PREFILL_CAUSAL if causal else 0, out, workspace)
+                      cu_seqlens_q.contiguous(), sm_scale, 0, mq, PREFILL_CAUSAL if causal else 0, out, workspace, window,
+                      sinks)
