@@ -596,7 +596,8 @@ int64_t tq_kv8_decode_window_workspace_bytes(int num_seqs, int num_q_heads, int 
  * cut there).
  */
 int tq_kv8_observe(const tq_kv8_window_args* a, tq_stream_t stream);
-int64_t tq_kv8_observe_workspace_bytes(int num_seqs, int max_q_len, int last, int num_q_heads, int num_kv_heads);
+int64_t tq_kv8_observe_workspace_bytes(int num_seqs, int max_q_len, int last, int num_q_heads, int num_kv_heads, int q_dtype,
+                                       int max_seq_len);
 
 /*
  * Cuts the sequences that hold more than longer_than tokens (at most max_seq_len and the block table's capacity of them count) to

@@ -69,8 +69,8 @@ def test_c_window_workspaces():
     # exactly what the entry asks for (the next check behind it is a device, which is not here: so only too little is shown)
     f = attn(wsb=L.tq_kv8_decode_window_workspace_bytes(2, 8, 2, 64, 20, 4, 1) - 1)
     assert L.tq_kv8_decode_window(WINDOW.pack(*(f[k] for k in ATTN + REACH)), None) == -5
-    assert L.tq_kv8_observe_workspace_bytes(2, 8, 0, 8, 2) == 0 == L.tq_kv8_observe_workspace_bytes(2, 8, 3, 8, 3)
-    assert L.tq_kv8_observe_workspace_bytes(1, 8, 3, 8, 2) > 0
+    assert L.tq_kv8_observe_workspace_bytes(2, 8, 0, 8, 2, 2, 64) == 0 == L.tq_kv8_observe_workspace_bytes(2, 8, 3, 8, 3, 2, 64)
+    assert L.tq_kv8_observe_workspace_bytes(1, 8, 3, 8, 2, 2, 64) > 0 == L.tq_kv8_observe_workspace_bytes(1, 8, 3, 8, 2, 2, 0)
     assert L.tq_kv8_evict_workspace_bytes(2, 2, 0, 16) == 0 == L.tq_kv8_evict_workspace_bytes(2, 2, 8, 24)
     assert L.tq_kv8_evict_workspace_bytes(1, 1, 1, 16) > 0
 

@@ -169,7 +169,7 @@ SIGNATURES = {
     "tq_kv8_prefill_window": (_i32, [ctypes.c_char_p, _vp]),
     "tq_kv8_decode_window_workspace_bytes": (_i64, [_i32] * 7),
     "tq_kv8_observe": (_i32, [ctypes.c_char_p, _vp]),
-    "tq_kv8_observe_workspace_bytes": (_i64, [_i32] * 5),
+    "tq_kv8_observe_workspace_bytes": (_i64, [_i32] * 7),
     "tq_kv8_evict": (_i32, [ctypes.c_char_p, _vp]),
     "tq_kv8_evict_workspace_bytes": (_i64, [_i32] * 4),
     "tq_rope": (_i32, [ctypes.c_char_p, _vp]),

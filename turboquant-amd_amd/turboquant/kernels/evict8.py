@@ -114,13 +114,13 @@ def observe_paged8(
         return mass
     last = min(last, mq)
     q, seq_lens, cu_seqlens_q = _rows(q), seq_lens.contiguous(), cu_seqlens_q.contiguous()
-    need = _lib.lib().tq_kv8_observe_workspace_bytes(S, mq, last, hq, hkv)
+    code, cap = _lib.dtype_code(q), _bound(max_seq_len, mb, k_fmt.block_size)
+    need = _lib.lib().tq_kv8_observe_workspace_bytes(S, mq, last, hq, hkv, code, cap)
     ws = _workspace(workspace, need, dev)
     qt, qh, _ = q.stride()
-    code = _lib.dtype_code(q)
     args = _ATTN.pack(q.data_ptr(), 0, k_cache.data_ptr(), 0, block_tables.data_ptr(), seq_lens.data_ptr(), cu_seqlens_q.data_ptr(),
                       ws.data_ptr(), need, qt, qh, 0, 0, kb, kh, 0, 0, nb, row, code, code, k_fmt.encoding_code, S, hq, hkv, 128,
-                      k_fmt.block_size, mb, _bound(max_seq_len, mb, k_fmt.block_size), mq, PREFILL_CAUSAL, scale, 0)
+                      k_fmt.block_size, mb, cap, mq, PREFILL_CAUSAL, scale, 0)
     _lib.launch("tq_kv8_observe", dev, args + _REACH.pack(mass.data_ptr(), *ms, window, sinks, last, 0))
     return mass
 
