@@ -163,53 +163,56 @@ __device__ __forceinline__ Step step_of(const Tiles& t, int i) {
     }
     return x;
 }
-template <int ENC, bool CLEAN>
+template <int ENC>
 __device__ __forceinline__ void convert(const Codes& x, tq_half8 (&k)[8]) {
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
-        uint32_t u = x.w[c >> 1][2 * (c & 1)], v = x.w[c >> 1][2 * (c & 1) + 1];
-        if (CLEAN && ENC == TQ_E4M3) {
-            // (NaN codes become 0: the rows that see one count for nothing)
-            const uint32_t a = kv8_nan_bytes(u), b = kv8_nan_bytes(v);
-            u &= ~((a << 1) - (a >> 7));
-            v &= ~((b << 1) - (b >> 7));
-        }
-        k[c] = kv8_half8<ENC>(u, v, 1.f, 1.f);
+        k[c] = kv8_half8<ENC>(x.w[c >> 1][2 * (c & 1)], x.w[c >> 1][2 * (c & 1) + 1], 1.f, 1.f);
     }
 }
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-// Scores in log2 units of a step's 32 tokens and row tile rt: lane n's row, token 16 t + 8 (v / 4) + 4h + v % 4 in
-// sv[8 t + v]; -inf where the row does not see the token.
+// Scores in log2 units of a step's 32 tokens and row tiles rt and rt + 1 (two chains of products): lane n's row, token
+// 16 t + 8 (v / 4) + 4h + v % 4 in sv[.][8 t + v]; -inf where the row does not see the token.
 template <bool FINE>
 __device__ __forceinline__ void scores(const Observe& p, const Block<FINE>& b, const tq_half8 (&k)[8], const Step& x, int rt, int js, bool edge,
-                                       float (&sv)[16]) {
+                                       float (&sv)[2][16]) {
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
-    f32x16 sc;
+    f32x16 sc[2];
 #pragma unroll
-    for (int v = 0; v < 16; ++v) sc[v] = 0.f;
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-        sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[c], b.hi[(rt * 8 + c) * 64 + lane], sc, 0, 0, 0);
-        if (FINE) sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[c], b.lo[(rt * 8 + c) * 64 + lane], sc, 0, 0, 0);
-    }
-    const float c1 = b.c1[32 * rt + n], f[2] = {c1 * x.ks[0], c1 * x.ks[1]};
+        for (int v = 0; v < 16; ++v) sc[i][v] = 0.f;
 #pragma unroll
-    for (int v = 0; v < 16; ++v) {
+    for (int c = 0; c < 8; ++c)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[c], b.hi[((rt + i) * 8 + c) * 64 + lane], sc[i], 0, 0, 0);
+            if (FINE) sc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[c], b.lo[((rt + i) * 8 + c) * 64 + lane], sc[i], 0, 0, 0);
+        }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const float c1 = b.c1[32 * (rt + i) + n], f[2] = {c1 * x.ks[0], c1 * x.ks[1]};
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
 #pragma clang fp contract(off)
-        sv[v] = sc[v] * f[v >> 3];  // (rounded here in both kernels: far scores then differ from M as they should)
+            sv[i][v] = sc[i][v] * f[v >> 3];  // (rounded here in both kernels: far scores then differ from M as they should)
+        }
     }
     if (edge) {
-        const int seen = b.seen[32 * rt + n], lo = kv8_window_from(seen, p.at.window);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const int at = 32 * js + 16 * t + 4 * h;
-            const int upto = seen - at < x.nv[t] - 4 * h ? seen - at : x.nv[t] - 4 * h;
+        for (int i = 0; i < 2; ++i) {
+            const int seen = b.seen[32 * (rt + i) + n], lo = kv8_window_from(seen, p.at.window);
 #pragma unroll
-            for (int v = 0; v < 8; ++v) {
-                const int i = 8 * (v >> 2) + (v & 3);
-                if (i >= upto || (i >= p.at.sinks - at && i < lo - at)) sv[8 * t + v] = kKv8NegInf;
+            for (int t = 0; t < 2; ++t) {
+                const int at = 32 * js + 16 * t + 4 * h;
+                const int upto = seen - at < x.nv[t] - 4 * h ? seen - at : x.nv[t] - 4 * h;
+#pragma unroll
+                for (int v = 0; v < 8; ++v) {
+                    const int y = 8 * (v >> 2) + (v & 3);
+                    if (y >= upto || (y >= p.at.sinks - at && y < lo - at)) sv[i][8 * t + v] = kKv8NegInf;
+                }
             }
         }
     }
@@ -244,7 +247,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_observe_stats_kernel(Obser
     const Kv8Span span = span_of(p, r, rb);
     const int j0 = chunk * p.chunk_steps, j1 = j0 + p.chunk_steps < span.n ? j0 + p.chunk_steps : span.n;
     if (j0 >= j1) return;  // (the sums read the chunks that have steps)
-    const int tiles = (last_row(p, r, rb) - rb * kRows) / 32 + 1;
+    // row tiles, in pairs: rows that do not exist are zeros
+    const int tiles = 2 * ((last_row(p, r, rb) - rb * kRows) / 64 + 1);
     float M[kTiles], l[kTiles];
 #pragma unroll
     for (int rt = 0; rt < kTiles; ++rt) {
@@ -262,23 +266,26 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_observe_stats_kernel(Obser
     for (int j = jg + wave; j < je; j += kWaves) {
         const int js = span.step(j), i = 2 * (j - jg);
         tq_half8 k[8];
-        convert<ENC, false>(next, k);
+        convert<ENC>(next, k);
         next = load_codes(now, i + 2 * kWaves < 62 ? i + 2 * kWaves : 62);  // (behind the last: a valid address)
         const Step x = step_of(now, i);
         const bool edge = at_edge(p, r, rb, js, x);
 #pragma unroll
-        for (int rt = 0; rt < kTiles; ++rt) {
+        for (int rt = 0; rt < kTiles; rt += 2) {
             if (rt >= tiles) break;
-            float sv[16];
+            float sv[2][16];
             scores<FINE>(p, b, k, x, rt, js, edge, sv);
-            float m = M[rt];
 #pragma unroll
-            for (int v = 0; v < 16; ++v) m = fmaxf(m, sv[v]);
-            float sum = 0.f;
+            for (int i = 0; i < 2; ++i) {
+                float m = M[rt + i];
 #pragma unroll
-            for (int v = 0; v < 16; ++v) sum += __builtin_amdgcn_exp2f(sv[v] - m);
-            l[rt] = l[rt] * __builtin_amdgcn_exp2f(M[rt] - m) + sum;
-            M[rt] = m;
+                for (int v = 0; v < 16; ++v) m = fmaxf(m, sv[i][v]);
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int v = 0; v < 16; ++v) sum[v & 3] += __builtin_amdgcn_exp2f(sv[i][v] - m);
+                l[rt + i] = l[rt + i] * __builtin_amdgcn_exp2f(M[rt + i] - m) + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+                M[rt + i] = m;
+            }
         }
     }
     }
@@ -328,7 +335,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_observe_sum_kernel(Observe
         const Kv8Span span = span_of(p, r, rb);
         const int hi = position(p, r, last_row(p, r, rb)) + 1;
         if (t0 >= hi || (t0 + p.tokens <= span.lo && t0 >= p.at.sinks)) continue;
-        const int tiles = (last_row(p, r, rb) - rb * kRows) / 32 + 1;
+        const int tiles = 2 * ((last_row(p, r, rb) - rb * kRows) / 64 + 1);
         const int behind = t1 < hi ? t1 : hi;
         int t = t0 + 32 * wave;
         Codes next = load_codes(now, 2 * wave);
@@ -366,7 +373,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_observe_sum_kernel(Observe
         }
         for (; t < behind; t += 32 * kWaves) {
             tq_half8 k[8];
-            convert<ENC, true>(next, k);
+            convert<ENC>(next, k);
             const int lane0 = (t - t0) >> 4;
             next = load_codes(now, lane0 + 2 * kWaves < 62 ? lane0 + 2 * kWaves : 62);
             const Step x = step_of(now, lane0);
@@ -374,13 +381,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_observe_sum_kernel(Observe
             float acc[16];
 #pragma unroll
             for (int v = 0; v < 16; ++v) acc[v] = 0.f;
-            for (int rt = 0; rt < tiles; ++rt) {
-                float sv[16];
+            for (int rt = 0; rt < tiles; rt += 2) {
+                float sv[2][16];
                 scores<FINE>(p, b, k, x, rt, t >> 5, edge, sv);
-                const float M = b.M[32 * rt + n], inv = b.inv[32 * rt + n];
 #pragma unroll
-                for (int v = 0; v < 16; ++v) acc[v] = __builtin_fmaf(__builtin_amdgcn_exp2f(sv[v] - M), inv, acc[v]);
+                for (int i = 0; i < 2; ++i) {
+                    const float M = b.M[32 * (rt + i) + n], inv = b.inv[32 * (rt + i) + n];
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) acc[v] = __builtin_fmaf(__builtin_amdgcn_exp2f(sv[i][v] - M), inv, acc[v]);
+                }
             }
+            // (NaN in a key: all rows that see its token count for nothing)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) acc[v] = fmaxf(acc[v], 0.f);
             // ---- over the half's 32 lanes: each stage halves the lane's values; lane n ends with value n / 2 ----
 #pragma unroll
             for (int m = 16; m >= 2; m >>= 1) {
