@@ -114,6 +114,17 @@ def test_evict_thresholds(dev):
     assert got is out and got.tolist() == [0, 150 - 5000]
 
 
+@pytest.mark.parametrize("code,block,hkv,seqs", [("e4m3", 16, 2, 110), ("int8", 48, 8, 25), ("e4m3", 64, 1, 200), ("int8", 64, 3, 63),
+                                                 ("e4m3", 32, 3, 64)])
+def test_evict_many_segments(dev, code, block, hkv, seqs):
+    """Around the number of (sequence, KV head) pairs from which on a workgroup takes a whole one."""
+    rng = np.random.default_rng(seqs)
+    lens = [int(x) for x in rng.integers(0, 150, seqs)]
+    compare(dev, rng, lens, hkv, code, block, 57, 11, 3, odd=True, width=11)
+    lens = [int(x) for x in rng.integers(300, 420, 4)] + [0] * (seqs - 4)
+    compare(dev, rng, lens, hkv, code, block, 290, 11, 3)
+
+
 @pytest.mark.parametrize("n,keep", [(5000, 1700), (20000, 9001), (70001, 30000)])
 def test_evict_long(dev, n, keep):
     """Rounds beyond the plan's first, against an ordering by torch; all-equal numbers keep the first tokens."""

@@ -83,9 +83,9 @@ __device__ __forceinline__ Share share_of(const Kv8Attn& p, int64_t P) {
     return h;
 }
 
-// WINDOW: each sequence's steps are those that its window and the sinks touch, and with p.scores every step leaves its
-// scores for the accumulated weights.
-template <int ENC, bool FINE, bool WINDOW>
+// WINDOW: each sequence's steps are those that its window and the sinks touch (all, where the window is 2^31 - 1); MASS: every
+// step leaves its scores for the accumulated weights.
+template <int ENC, bool FINE, bool WINDOW, bool MASS>
 __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kernel(Kv8Attn p) {
     using Code = Kv8Code<ENC>;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
         }
 
         float M = kKv8None, base = kKv8None, lsum = 0.f, vref = 0.f;  // M: largest score so far
-        float lfull = 0.f;  // WINDOW: the sum of the probabilities before their rounding
+        float lfull = 0.f;  // MASS: the sum of the probabilities before their rounding
         tq_floatx4 acc[8];
 #pragma unroll
         for (int a = 0; a < 8; ++a) acc[a] = tq_floatx4{0.f, 0.f, 0.f, 0.f};
@@ -288,12 +288,6 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
                     if (nv[h] == 0) vs[h] = 0.f;
                 }
             }
-            if (WINDOW && p.scores && n < p.group) {
-                float* dst = p.scores + (((int64_t)s * hkv + kh) * p.most_steps + j) * (32 * p.group) + 16 * n + 4 * g;
-#pragma unroll
-                for (int h = 0; h < kTiles; ++h)
-                    *reinterpret_cast<float4*>(dst + 16 * h * p.group) = make_float4(sv[4 * h], sv[4 * h + 1], sv[4 * h + 2], sv[4 * h + 3]);
-            }
             // ---- online softmax ----
             float mx = sv[0], vmax = vs[0];
 #pragma unroll
@@ -326,7 +320,7 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
                 tq_half8 ph, pl;
                 kv8_prob8<FINE>(pr, ph, pl);
                 lsum += kv8_sum8<FINE>(pr, ph);
-                if (WINDOW) lfull += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
+                if (MASS) lfull += ((pr[0] + pr[1]) + (pr[2] + pr[3])) + ((pr[4] + pr[5]) + (pr[6] + pr[7]));
                 const float va = kv8_relative(vs[h], rv), vb2 = kv8_relative(vs[h + 1], rv);
 #pragma unroll
                 for (int a = 0; a < 8; ++a) {
@@ -336,6 +330,20 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
                 }
             }
             load_values(next, kTiles * jn);
+            if (MASS) {
+                // (stores without a condition, the lanes without a head out of the buffer's range: where the compiler cannot count
+                // what is under way, it waits for all of it; 64 x 32768 tokens 1080 -> @@ us)
+                const uint32_t bytes = 128u * (uint32_t)p.group;
+                const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
+                    p.scores + (((int64_t)s * hkv + kh) * p.most_steps + j) * (32 * p.group), (short)0, (int)bytes, 0x00020000);
+#pragma unroll
+                for (int h = 0; h < kTiles; ++h) {
+                    const uint32_t at = n < p.group ? (uint32_t)(4 * h + g) * (bytes >> 3) + 16u * n : 0x40000000u;
+                    __builtin_amdgcn_raw_buffer_store_b128(
+                        tq_u32x4{__float_as_uint(sv[4 * h]), __float_as_uint(sv[4 * h + 1]), __float_as_uint(sv[4 * h + 2]), __float_as_uint(sv[4 * h + 3])},
+                        rsrc, (int)at, 0, 0);
+                }
+            }
         }
         }
 
@@ -347,7 +355,7 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
             if (j0 == 0) ends[0] = (int)w;
             if (j1 == np) ends[1] = (int)w;
         }
-        if (WINDOW && p.scores) {
+        if (MASS) {
             const float l1 = tq_sum_over_groups(lfull);
             if (g == 0 && n < p.group) {
                 const int64_t row = (w + (int64_t)s * hkv + kh) * p.group + n;
@@ -425,10 +433,10 @@ __global__ __launch_bounds__(256) void kv8_decode_mass_kernel(Kv8Attn p, int chu
     const int in = 4 * (int)(threadIdx.x & 7);  // first token within the step
     const int t = 32 * span.step(j) + in;
     if (t >= L) return;
-    const float* src = p.scores + (((int64_t)seg) * p.most_steps + j) * (32 * p.group) + (in >> 4) * (16 * p.group) + (in & 15);
+    const float* src = p.scores + (((int64_t)seg) * p.most_steps + j) * (32 * p.group) + in * p.group;
     float add[4] = {0.f, 0.f, 0.f, 0.f};
     for (int r = 0; r < p.group; ++r) {
-        const float4 x = *reinterpret_cast<const float4*>(src + 16 * r);
+        const float4 x = *reinterpret_cast<const float4*>(src + 4 * r);
         const float2 st = s_stat[r];
         const float y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -619,10 +627,11 @@ int launch_decode(Kv8Attn& p, bool window, int64_t need, tq_stream_t stream) {
     p.workers = (int)(workers < 1 ? 1 : workers);
     const bool fine = a->q_dtype == TQ_F32 || a->out_dtype == TQ_F32;
     const void* kern = nullptr;
-#define TQ_DECODE(E, F, W) \
-    if (a->encoding == E && fine == F && window == W) kern = (const void*)kv8_decode_kernel<E, F, W>;
-    TQ_DECODE(TQ_E4M3, false, false) TQ_DECODE(TQ_E4M3, true, false) TQ_DECODE(TQ_E4M3, false, true) TQ_DECODE(TQ_E4M3, true, true)
-    TQ_DECODE(TQ_INT8, false, false) TQ_DECODE(TQ_INT8, true, false) TQ_DECODE(TQ_INT8, false, true) TQ_DECODE(TQ_INT8, true, true)
+#define TQ_DECODE(E, F)                                                                      \
+    if (a->encoding == E && fine == F)                                                       \
+        kern = p.mass ? (const void*)kv8_decode_kernel<E, F, true, true>                     \
+                      : window ? (const void*)kv8_decode_kernel<E, F, true, false> : (const void*)kv8_decode_kernel<E, F, false, false>;
+    TQ_DECODE(TQ_E4M3, false) TQ_DECODE(TQ_E4M3, true) TQ_DECODE(TQ_INT8, false) TQ_DECODE(TQ_INT8, true)
 #undef TQ_DECODE
     void* args[] = {&p};
     hipError_t e = hipLaunchKernel(kern, dim3((unsigned)((p.workers + kWaves - 1) / kWaves)), dim3(64 * kWaves), args, 0, stream);
