@@ -565,7 +565,7 @@ int64_t tq_kv8_prefill_workspace_bytes(int num_seqs, int max_q_len, int num_q_he
  * The same with a window, and weights accumulated for an eviction.
  * window > 0: the query at position p of its sequence (decode: the last; prefill: seq_lens[s] - n + i) sees the tokens
  * t <= p with t > p - window or t < sinks; tokens that no row of a call sees are not read.  0: no window (sinks 0).
- * Prefill with a window needs TQ_PREFILL_CAUSAL, and V's largest scale so far counts the tokens that a block of 64 rows sees.
+ * Prefill with a window needs TQ_PREFILL_CAUSAL.
  * mass (decode and tq_kv8_observe; NULL for prefill): fp32, one number per (block, KV head, row) at
  * mass + block*stride_block + head*stride_head + row (elements; 16-byte aligned, strides multiples of 4).  A call adds to the
  * number of every token that a query sees the softmax weights that the KV head's query heads and the call's queries give

@@ -18,7 +18,12 @@
 // when a larger scale is met).
 //
 // Bound: HBM reads, 256 bytes per token and KV head: 64 x 32768 tokens of 8 heads in 762 us, 5.6 TB/s, where a large
-// copy moves 4.9.  Small calls: launches, start-up (the search for the wave's part, block table, scales) and
+// copy moves 4.9.  With a window the same per visible token: 64 sequences of 300 to 32768 tokens, window 4096, 384 MB in 82 us.
+// With accumulated weights each step's scores are kept for kv8_decode_mass_kernel, 4 bytes a head and token: at 64 x 32768 tokens
+// 402 MB more are written and the kernel takes 1078 us instead of 762; the same stores into a buffer that stays in
+// L2 cost 25 us, so it is the writes among the reads that memory takes badly (nontemporal stores, another order of the
+// scores and stores behind the next loads changed nothing).  Reading the keys again instead would move 128 bytes a token for all heads,
+// at six heads a KV head as long.  Small calls: launches, start-up (the search for the wave's part, block table, scales) and
 // the merge, about 15 us.
 #include "tq_kv8.h"
 
@@ -331,8 +336,8 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
             }
             load_values(next, kTiles * jn);
             if (MASS) {
-                // (stores without a condition, the lanes without a head out of the buffer's range: where the compiler cannot count
-                // what is under way, it waits for all of it; 64 x 32768 tokens 1080 -> @@ us)
+                // (behind the next step's loads, which would otherwise wait for them, and without a condition: lanes without a
+                // head are out of the buffer's range)
                 const uint32_t bytes = 128u * (uint32_t)p.group;
                 const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(
                     p.scores + (((int64_t)s * hkv + kh) * p.most_steps + j) * (32 * p.group), (short)0, (int)bytes, 0x00020000);
@@ -400,7 +405,8 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
 
 // Adds the weights of a segment's tokens, summed over its query heads, to what they had; the sequence's last token starts
 // from 0.  Workgroup (segment, 32 steps): first each head's base and sum over the segment's pieces, then four tokens a
-// thread.  A weight that is not a number counts as 0.
+// thread.  A weight that is not a number counts as 0.  Bound: memory, 4 bytes of score a head and 8 of weight a token: 64 x 32768
+// tokens of 48 / 8 heads, 537 MB, 113 us, 4.8 TB/s.
 __global__ __launch_bounds__(256) void kv8_decode_mass_kernel(Kv8Attn p, int chunks) {
     __shared__ float2 s_stat[16];
     const uint32_t seg = blockIdx.x / (uint32_t)chunks, chunk = blockIdx.x - seg * (uint32_t)chunks;

@@ -1,10 +1,19 @@
 // Eviction from the 8-bit paged caches by accumulated weight (tiles: tq_kv8.h).
 //
-// A segment is a (sequence, KV head).  kv8_evict_plan_kernel finds, a workgroup per segment, which tokens stay: the m-th
-// largest number between the first and the last ones by three passes over 11, 11 and 10 bits of the numbers' order
-// (counts in LDS), then the tokens above it and the first ones equal to it, in order.  kv8_evict_scales_kernel
-// gives every kept block its scale and every row its change of exponent.  The rows then move in units of 16:
-// kv8_evict_gather_kernel into the workspace, kv8_evict_scatter_kernel from there to the segment's first blocks.
+// A segment is a (sequence, KV head).  The plan, a workgroup per segment, finds which tokens stay: the m-th largest number between
+// the first and the last ones by three passes over 11, 11 and 10 bits of the numbers' order (counts in LDS; up to
+// 32768 tokens' numbers stay in registers), then the tokens above it and the first ones equal to it, in order by one
+// scan.  The kept rows move in units of 16, a wave each: their bytes, V's taken out of words of four tokens and put together
+// again, and where a block's largest scale is another's, rescaled.  Three ways:
+//   kv8_evict_segment_kernel  plan and move by one workgroup, a barrier between a round's loads and its stores: many segments
+//   kv8_evict_move_kernel     any workgroup moves any unit; units wait for those that what they overwrite goes to: few segments
+//   gather and scatter        through the workspace: blocks of more than 64 rows, whose scales take a kernel of their own
+//
+// Bound: memory, 512 bytes of codes a kept token: 32 x 4352 tokens of 8 heads cut to 4096, 546 MB in 182 us, 3.0 TB/s where a
+// copy moves 4.7.  One compute unit has some 20 GB/s of it, so the segment kernel needs most of them busy and 16 to 20 kB a round
+// under way; the move kernel pays for its flags (213 us there, 157 if nothing had to wait) and, where single tokens stay,
+// for V's words, four times the bytes of a token (16 sequences of 3001 to 32768 tokens cut to 8190: 343 MB in 28 + 130 us).  One prompt
+// of 32768: 43 us, of them 30 the plan's, one workgroup for 32768 numbers.
 #include "tq_kv8.h"
 
 namespace {
@@ -25,7 +34,7 @@ struct Evict {
     int2* list;                   // [segment][16 units]: block (-1: a bad entry) and row of the kept tokens
     int32_t* ranks;               // [segment][units + 1]: kept tokens before token 16 u
     int32_t* loaded;              // [segment][units]: 1 once the unit's rows and scales are in registers
-    int32_t* ticket;              // [segment][kPad]: one each
+    int32_t* state;               // [segment][kPad]: the next ticket; 1 where the plan cuts the sequence, for all kernels
     int items;                    // workgroups of a segment
     uint16_t* shift;              // [segment][16 units]: exponents that K's (low byte) and V's codes fall by; 63: zeros
     float2* scales;               // [segment][blocks]: K's and V's
@@ -245,9 +254,9 @@ __device__ __forceinline__ bool plan_segment(const Evict& p, PlanLds& lds, int& 
     const int L = length_of(p, s);
     const bool cut = L > p.a.longer_than;
     if (kh == 0 && threadIdx.x == 0) p.a.change[s] = cut ? p.a.keep - p.a.seq_lens[s] : 0;
+    if (p.state && threadIdx.x < 2) p.state[seg * kPad + threadIdx.x] = threadIdx.x && cut;
     if (!cut) return false;
-    if (p.ticket) {
-        if (threadIdx.x == 0) p.ticket[seg * kPad] = 0;
+    if (p.loaded) {
         for (int u = threadIdx.x; u < p.units; u += kPlan) p.loaded[(int64_t)seg * p.units + u] = 0;
         if (threadIdx.x == 0 && kUnit * p.units >= L) p.ranks[(int64_t)seg * (p.units + 1) + p.units] = p.a.keep;
     }
@@ -274,7 +283,7 @@ __global__ __launch_bounds__(256) void kv8_evict_scales_kernel(Evict p) {
     const int b = (int)(unit - seg * (uint32_t)p.blocks);
     if (seg >= (uint32_t)p.a.num_seqs * (uint32_t)p.a.num_kv_heads) return;
     const int s = (int)(seg / (uint32_t)p.a.num_kv_heads), kh = (int)seg - s * p.a.num_kv_heads;
-    if (length_of(p, s) <= p.a.longer_than) return;
+    if (!p.state[seg * kPad + 1]) return;
     const int d0 = b * p.a.block_size, d1 = d0 + p.a.block_size < p.a.keep ? d0 + p.a.block_size : p.a.keep;
     const uint8_t* kc = static_cast<const uint8_t*>(p.a.k_cache) + kh * p.a.k_stride_head;
     const uint8_t* vc = static_cast<const uint8_t*>(p.a.v_cache) + kh * p.a.v_stride_head;
@@ -430,7 +439,7 @@ __device__ __forceinline__ bool unit_of(const Evict& p, uint32_t& seg, int& s, i
     u = (int)(x - seg * (uint32_t)p.units);
     s = (int)(seg / (uint32_t)p.a.num_kv_heads);
     kh = (int)seg - s * p.a.num_kv_heads;
-    return s < p.a.num_seqs && length_of(p, s) > p.a.longer_than;
+    return s < p.a.num_seqs && p.state[seg * kPad + 1];
 }
 
 template <int ENC>
@@ -486,8 +495,8 @@ __global__ __launch_bounds__(64 * kMove, 8) void kv8_evict_move_kernel(Evict p) 
     // of 213)
     const uint32_t seg = blockIdx.x / (uint32_t)p.items;
     const int s = (int)(seg / (uint32_t)p.a.num_kv_heads), kh = (int)seg - s * p.a.num_kv_heads;
-    if (threadIdx.x == 0) s_ticket = __hip_atomic_fetch_add(p.ticket + seg * kPad, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const bool cut = length_of(p, s) > p.a.longer_than;  // (no: the ticket means nothing)
+    if (threadIdx.x == 0) s_ticket = __hip_atomic_fetch_add(p.state + seg * kPad, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const bool cut = p.state[seg * kPad + 1];
     __syncthreads();
     if (!cut) return;
     const int lane = threadIdx.x & 63;
@@ -620,8 +629,9 @@ extern "C" int64_t tq_kv8_evict_workspace_bytes(int num_seqs, int num_kv_heads, 
     if (num_seqs <= 0 || num_kv_heads <= 0 || keep <= 0 || block_size <= 0 || block_size % 16) return 0;
     const int64_t segs = (int64_t)num_seqs * num_kv_heads, units = ((int64_t)keep + kUnit - 1) / kUnit;
     const int64_t blocks = ((int64_t)keep + block_size - 1) / block_size;
-    if (block_size <= kInPlace) return align256(segs * units * kUnit * 8) + align256(segs * (units + 1) * 4) + align256(segs * units * 4) + segs * kPad * 4;
-    return align256(segs * units * kUnit * 8) + align256(segs * (units + 1) * 4) + align256(segs * units * kUnit * 2) +
+    const int64_t state = align256(segs * kPad * 4);
+    if (block_size <= kInPlace) return state + align256(segs * units * kUnit * 8) + align256(segs * (units + 1) * 4) + align256(segs * units * 4);
+    return state + align256(segs * units * kUnit * 8) + align256(segs * (units + 1) * 4) + align256(segs * units * kUnit * 2) +
            align256(segs * blocks * 8) + align256(segs * units * kUnit * 4) + segs * units * kStage;
 }
 
@@ -659,16 +669,17 @@ extern "C" int tq_kv8_evict(const tq_kv8_evict_args* a, tq_stream_t stream) {
             return TQ_ERR_WORKSPACE;
         p.units = (a->keep + kUnit - 1) / kUnit;
         p.blocks = (a->keep + a->block_size - 1) / a->block_size;
-        if (segs * p.units > 0x3ffffff) return TQ_ERR_INVALID_ARGUMENT;
+        if (segs * ((p.units + kMove - 1) / kMove) > 0xffffff || segs * p.units > 0x3fffff0) return TQ_ERR_INVALID_ARGUMENT;
         uint8_t* at = static_cast<uint8_t*>(a->workspace);
         const int64_t rows = segs * p.units * kUnit;
+        p.state = reinterpret_cast<int32_t*>(at);
+        at += align256(segs * kPad * 4);
         p.list = reinterpret_cast<int2*>(at);
         at += align256(rows * 8);
         p.ranks = reinterpret_cast<int32_t*>(at);
         at += align256(segs * (p.units + 1) * 4);
         if (a->block_size <= kInPlace) {
             p.loaded = reinterpret_cast<int32_t*>(at);
-            p.ticket = reinterpret_cast<int32_t*>(at + align256(segs * p.units * 4));
             p.items = (p.units + kMove - 1) / kMove;
         } else {
             p.shift = reinterpret_cast<uint16_t*>(at);
@@ -684,7 +695,7 @@ extern "C" int tq_kv8_evict(const tq_kv8_evict_args* a, tq_stream_t stream) {
                        : a->encoding == TQ_E4M3 ? (const void*)kv8_evict_segment_kernel<TQ_E4M3> : (const void*)kv8_evict_segment_kernel<TQ_INT8>;
     hipError_t e = hipLaunchKernel(first, dim3((unsigned)segs), dim3(kPlan), args, 0, stream);
     if (whole) {
-    } else if (any && p.ticket) {
+    } else if (any && p.loaded) {
         const void* move = a->encoding == TQ_E4M3 ? (const void*)kv8_evict_move_kernel<TQ_E4M3> : (const void*)kv8_evict_move_kernel<TQ_INT8>;
         if (e == hipSuccess) e = hipLaunchKernel(move, dim3((unsigned)(segs * p.items)), dim3(64 * kMove), args, 0, stream);
     } else if (any) {

@@ -319,8 +319,7 @@ def prefill_paged8(
     2^-18 of the row's largest to fewer bits and those below 2^-29 to zero.
 
     window (needs causal): the query at position p sees the tokens from p - window + 1 on and the first `sinks`
-    alone; tokens that no row sees are not read.  V's largest scale so far then counts the tokens that a row's block of
-    64 rows sees.
+    alone; tokens that no row sees are not read.
     """
     dev = _lib.require_gpu("prefill_paged8", q, cu_seqlens_q, k_cache, v_cache, block_tables, seq_lens, out, workspace)
     if q.dim() != 3 or q.shape[2] != 128:
