@@ -474,9 +474,8 @@ def work(case):
     if case["kind"] == "evict":
         total = [p + 1 for p in past if p + 1 > case["keep"]]
         kept = len(total) * case["keep"] * case["heads"]
-        # (each sequence's length and its change, also where none is longer than it should be)
-        return dict(bytes=8 * len(past) + sum(total) * case["heads"] * 4 + kept * (4 * D + 4)
-                    + sum(-(-t // block) for t in total) * 4, flops=len(past) + 4 * sum(total) * case["heads"])
+        return dict(bytes=sum(total) * case["heads"] * 4 + kept * (4 * D + 4) + sum(-(-t // block) for t in total) * 4,
+                    flops=4 * sum(total) * case["heads"])
     counts = []
     for p, n in zip(past, new):
         rows = min(n, case["last"]) if case["kind"] == "observe" else n
