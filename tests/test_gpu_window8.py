@@ -392,3 +392,39 @@ def test_refusals(dev):
     observe_paged8(**{**good, "q": q[:0], "cu_seqlens_q": i32([0, 0, 0], dev)})
     observe_paged8(**{**good, "max_q_len": 0})
     assert torch.equal(mass, before)
+
+
+@pytest.mark.parametrize("sm", [0.0, -0.06, 0.02])
+@pytest.mark.parametrize("qd", [torch.bfloat16, torch.float32])
+def test_score_scales(dev, sm, qd):
+    """No scale (all tokens alike), a negative one, a small one."""
+    L, new = 300, 20
+    args, (kval, vval) = caches(dev, [L], 2, "int8", 16)
+    kc, kf, vc, vf, bt = args
+    q = torch.randn(new, 4, 128, generator=torch.Generator(device=dev).manual_seed(4), device=dev).to(qd)
+    before = random_mass(kc, 16)
+    got = observe_paged8(q, i32([0, new], dev), kc, kf, bt, i32([L], dev), before.clone(), sm_scale=sm, window=120, sinks=2)
+    _, add = eref.sequence(q.cpu().double().numpy(), kval, None, bt[0].cpu(), L, 120, 2, sm)
+    check_mass(got, before, [add], bt.cpu(), [L], [new], 16, 2 * new)
+    mass = before.clone()
+    out = decode_paged8(q[-1:], *args, i32([L], dev), sm_scale=sm, window=120, sinks=2, mass=mass)
+    want, add = eref.sequence(q[-1:].cpu().double().numpy(), kval, vval, bt[0].cpu(), L, 120, 2, sm)
+    check_mass(mass, before, [add], bt.cpu(), [L], [1], 16, 2)
+    assert np.all(np.abs(out.cpu().double().numpy() - want) <= bound(np.abs(vval).max(), L, qd, qd, want))
+
+
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 14, 2.0 ** 30])
+def test_far_scores(dev, size):
+    """Scores so large that fp32's spacing passes one unit: every row's weights still are numbers and sum to one."""
+    L, new, hq = 500, 70, 4
+    g = torch.Generator(device=dev).manual_seed(11)
+    k, v = (torch.randn(L, 1, 128, generator=g, device=dev) for _ in range(2))
+    args, _ = caches(dev, [L], 1, "e4m3", 16, kv=(k * size, v))
+    kc, kf, vc, vf, bt = args
+    q = torch.randn(new, hq, 128, generator=g, device=dev) * size
+    mass = observe_paged8(q, i32([0, new], dev), kc, kf, bt, i32([L], dev), allocate_mass(kc.shape[0], 1, 16, device=dev))
+    one = allocate_mass(kc.shape[0], 1, 16, device=dev)
+    decode_paged8(q[-1:], *args, i32([L], dev), mass=one)
+    # (L weights of a row and their sum: two roundings each, an exponential of 2^-22 on either side)
+    for m, rows in ((mass, new * hq), (one, hq)):
+        assert torch.all(m >= 0) and abs(m.double().sum().item() - rows) <= rows * (2.0 ** -21 + (L + rows) * 2.0 ** -24)
