@@ -97,7 +97,7 @@ struct Kv8Attn {
     int window, sinks;    // (no window: one of 2^31 - 1 tokens)
     float* mass;
     int64_t mass_stride_block, mass_stride_head;
-    float* scores;        // decode: [segment][most_steps][8 token quads][group][4], log2 units
+    float* scores;        // decode: [segment][most_steps][2 tiles][group][16], log2 units
     float* ws_me;         // decode: [slot][row][2]: exponent base (log2) and unrounded sum of every piece
     int most_steps;
 };

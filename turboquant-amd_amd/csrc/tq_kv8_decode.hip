@@ -343,7 +343,7 @@ __global__ __launch_bounds__(64 * kWaves, kWavesPerCu / 4) void kv8_decode_kerne
                     p.scores + (((int64_t)s * hkv + kh) * p.most_steps + j) * (32 * p.group), (short)0, (int)bytes, 0x00020000);
 #pragma unroll
                 for (int h = 0; h < kTiles; ++h) {
-                    const uint32_t at = n < p.group ? (uint32_t)(4 * h + g) * (bytes >> 3) + 16u * n : 0x40000000u;
+                    const uint32_t at = n < p.group ? (uint32_t)h * (bytes >> 1) + 64u * n + 16u * g : 0x40000000u;
                     __builtin_amdgcn_raw_buffer_store_b128(
                         tq_u32x4{__float_as_uint(sv[4 * h]), __float_as_uint(sv[4 * h + 1]), __float_as_uint(sv[4 * h + 2]), __float_as_uint(sv[4 * h + 3])},
                         rsrc, (int)at, 0, 0);
@@ -439,10 +439,10 @@ __global__ __launch_bounds__(256) void kv8_decode_mass_kernel(Kv8Attn p, int chu
     const int in = 4 * (int)(threadIdx.x & 7);  // first token within the step
     const int t = 32 * span.step(j) + in;
     if (t >= L) return;
-    const float* src = p.scores + (((int64_t)seg) * p.most_steps + j) * (32 * p.group) + in * p.group;
+    const float* src = p.scores + (((int64_t)seg) * p.most_steps + j) * (32 * p.group) + (in >> 4) * (16 * p.group) + (in & 15);
     float add[4] = {0.f, 0.f, 0.f, 0.f};
     for (int r = 0; r < p.group; ++r) {
-        const float4 x = *reinterpret_cast<const float4*>(src + 4 * r);
+        const float4 x = *reinterpret_cast<const float4*>(src + 16 * r);
         const float2 st = s_stat[r];
         const float y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll

@@ -34,7 +34,8 @@ struct Evict {
     int2* list;                   // [segment][16 units]: block (-1: a bad entry) and row of the kept tokens
     int32_t* ranks;               // [segment][units + 1]: kept tokens before token 16 u
     int32_t* loaded;              // [segment][units]: 1 once the unit's rows and scales are in registers
-    int32_t* state;               // [segment][kPad]: the next ticket; 1 where the plan cuts the sequence, for all kernels
+    int32_t* cut;                 // [segment]: 1 where the plan cuts the sequence, for all kernels
+    int32_t* ticket;              // [segment][kPad]: the next one (away from what is only read)
     int items;                    // workgroups of a segment
     uint16_t* shift;              // [segment][16 units]: exponents that K's (low byte) and V's codes fall by; 63: zeros
     float2* scales;               // [segment][blocks]: K's and V's
@@ -254,9 +255,10 @@ __device__ __forceinline__ bool plan_segment(const Evict& p, PlanLds& lds, int& 
     const int L = length_of(p, s);
     const bool cut = L > p.a.longer_than;
     if (kh == 0 && threadIdx.x == 0) p.a.change[s] = cut ? p.a.keep - p.a.seq_lens[s] : 0;
-    if (p.state && threadIdx.x < 2) p.state[seg * kPad + threadIdx.x] = threadIdx.x && cut;
+    if (p.cut && threadIdx.x == 0) p.cut[seg] = cut;
     if (!cut) return false;
     if (p.loaded) {
+        if (threadIdx.x == 0) p.ticket[seg * kPad] = 0;
         for (int u = threadIdx.x; u < p.units; u += kPlan) p.loaded[(int64_t)seg * p.units + u] = 0;
         if (threadIdx.x == 0 && kUnit * p.units >= L) p.ranks[(int64_t)seg * (p.units + 1) + p.units] = p.a.keep;
     }
@@ -283,7 +285,7 @@ __global__ __launch_bounds__(256) void kv8_evict_scales_kernel(Evict p) {
     const int b = (int)(unit - seg * (uint32_t)p.blocks);
     if (seg >= (uint32_t)p.a.num_seqs * (uint32_t)p.a.num_kv_heads) return;
     const int s = (int)(seg / (uint32_t)p.a.num_kv_heads), kh = (int)seg - s * p.a.num_kv_heads;
-    if (!p.state[seg * kPad + 1]) return;
+    if (!p.cut[seg]) return;
     const int d0 = b * p.a.block_size, d1 = d0 + p.a.block_size < p.a.keep ? d0 + p.a.block_size : p.a.keep;
     const uint8_t* kc = static_cast<const uint8_t*>(p.a.k_cache) + kh * p.a.k_stride_head;
     const uint8_t* vc = static_cast<const uint8_t*>(p.a.v_cache) + kh * p.a.v_stride_head;
@@ -439,7 +441,7 @@ __device__ __forceinline__ bool unit_of(const Evict& p, uint32_t& seg, int& s, i
     u = (int)(x - seg * (uint32_t)p.units);
     s = (int)(seg / (uint32_t)p.a.num_kv_heads);
     kh = (int)seg - s * p.a.num_kv_heads;
-    return s < p.a.num_seqs && p.state[seg * kPad + 1];
+    return s < p.a.num_seqs && p.cut[seg];
 }
 
 template <int ENC>
@@ -495,10 +497,9 @@ __global__ __launch_bounds__(64 * kMove, 8) void kv8_evict_move_kernel(Evict p) 
     // of 213)
     const uint32_t seg = blockIdx.x / (uint32_t)p.items;
     const int s = (int)(seg / (uint32_t)p.a.num_kv_heads), kh = (int)seg - s * p.a.num_kv_heads;
-    if (threadIdx.x == 0) s_ticket = __hip_atomic_fetch_add(p.state + seg * kPad, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const bool cut = p.state[seg * kPad + 1];
+    if (!p.cut[seg]) return;
+    if (threadIdx.x == 0) s_ticket = __hip_atomic_fetch_add(p.ticket + seg * kPad, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    if (!cut) return;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int u = __builtin_amdgcn_readfirstlane(s_ticket) * kMove + wave;
@@ -629,9 +630,9 @@ extern "C" int64_t tq_kv8_evict_workspace_bytes(int num_seqs, int num_kv_heads, 
     if (num_seqs <= 0 || num_kv_heads <= 0 || keep <= 0 || block_size <= 0 || block_size % 16) return 0;
     const int64_t segs = (int64_t)num_seqs * num_kv_heads, units = ((int64_t)keep + kUnit - 1) / kUnit;
     const int64_t blocks = ((int64_t)keep + block_size - 1) / block_size;
-    const int64_t state = align256(segs * kPad * 4);
-    if (block_size <= kInPlace) return state + align256(segs * units * kUnit * 8) + align256(segs * (units + 1) * 4) + align256(segs * units * 4);
-    return state + align256(segs * units * kUnit * 8) + align256(segs * (units + 1) * 4) + align256(segs * units * kUnit * 2) +
+    const int64_t cut = align256(segs * 4);
+    if (block_size <= kInPlace) return cut + align256(segs * kPad * 4) + align256(segs * units * kUnit * 8) + align256(segs * (units + 1) * 4) + align256(segs * units * 4);
+    return cut + align256(segs * units * kUnit * 8) + align256(segs * (units + 1) * 4) + align256(segs * units * kUnit * 2) +
            align256(segs * blocks * 8) + align256(segs * units * kUnit * 4) + segs * units * kStage;
 }
 
@@ -672,14 +673,15 @@ extern "C" int tq_kv8_evict(const tq_kv8_evict_args* a, tq_stream_t stream) {
         if (segs * ((p.units + kMove - 1) / kMove) > 0xffffff || segs * p.units > 0x3fffff0) return TQ_ERR_INVALID_ARGUMENT;
         uint8_t* at = static_cast<uint8_t*>(a->workspace);
         const int64_t rows = segs * p.units * kUnit;
-        p.state = reinterpret_cast<int32_t*>(at);
-        at += align256(segs * kPad * 4);
+        p.cut = reinterpret_cast<int32_t*>(at);
+        at += align256(segs * 4);
         p.list = reinterpret_cast<int2*>(at);
         at += align256(rows * 8);
         p.ranks = reinterpret_cast<int32_t*>(at);
         at += align256(segs * (p.units + 1) * 4);
         if (a->block_size <= kInPlace) {
             p.loaded = reinterpret_cast<int32_t*>(at);
+            p.ticket = reinterpret_cast<int32_t*>(at + align256(segs * p.units * 4));
             p.items = (p.units + kMove - 1) / kMove;
         } else {
             p.shift = reinterpret_cast<uint16_t*>(at);
