@@ -428,3 +428,43 @@ def test_far_scores(dev, size):
     # (L weights of a row and their sum: two roundings each, an exponential of 2^-22 on either side)
     for m, rows in ((mass, new * hq), (one, hq)):
         assert torch.all(m >= 0) and abs(m.double().sum().item() - rows) <= rows * (2.0 ** -21 + (L + rows) * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("code,qd", [("e4m3", torch.float32), ("int8", torch.bfloat16), ("e4m3", torch.float16), ("int8", torch.float32)])
+@pytest.mark.parametrize("window,sinks,group", [(37, 3, 2), (20, 0, 1), (70, 17, 5)])
+def test_scales_by_block(dev, code, qd, window, sinks, group):
+    """Blocks whose values differ by 2^40: a row is as exact as the blocks that it sees allow, whatever others hold."""
+    L, new = 700, 200
+    g = torch.Generator(device=dev).manual_seed(window)
+    k, v = (torch.randn(L, 1, 128, generator=g, device=dev) for _ in range(2))
+    e = torch.randint(-1, 2, (-(-L // 16),), generator=torch.Generator().manual_seed(window)).to(dev).double() * 40
+    v = (v.double() * torch.exp2(e)[torch.arange(L, device=dev) // 16][:, None, None]).float()
+    args, (kval, vval) = caches(dev, [L], 1, code, 16, kv=(k, v))
+    q = torch.randn(new, group, 128, generator=g, device=dev).to(qd)
+    out = torch.empty(new, group, 128, device=dev, dtype=torch.float32 if qd == torch.float16 else qd)  # (2^40 is no half)
+    prefill_paged8(q, i32([0, new], dev), *args, i32([L], dev), window=window, sinks=sinks, out=out)
+    want, _ = eref.sequence(q.cpu().double().numpy(), kval, vval, args[4][0].cpu(), L, window, sinks, SM)
+    got = out.cpu().double().numpy()
+    for i in range(new):
+        seen = np.nonzero(eref.visible(L - new + i, L, window, sinks))[0]
+        # (a block's scale holds for all its rows, so what counts is the largest that its codes could be)
+        top = max(np.abs(vval[int(args[4][0, b])]).max() for b in set(seen // 16)) * 2
+        assert np.all(np.abs(got[i] - want[i]) <= bound(top, L, qd, out.dtype, want[i])), i
+
+
+@pytest.mark.parametrize("group", [17, 70, 130])
+def test_many_heads(dev, group):
+    """More query heads per KV head than a row block's share: prefill with a window, and prompts' weights."""
+    lens, new, block = [90, 200], [5, 11], 16
+    args, (kval, vval) = caches(dev, lens, 1, "e4m3", block)
+    q = torch.randn(16, group, 128, generator=torch.Generator(device=dev).manual_seed(group), device=dev).to(torch.bfloat16)
+    cu, sl = i32([0, 5, 16], dev), i32(lens, dev)
+    out = prefill_paged8(q, cu, *args, sl, window=50, sinks=3)
+    before = random_mass(args[0], block)
+    mass = observe_paged8(q, cu, args[0], args[1], args[4], sl, before.clone(), last=4, window=50, sinks=3)
+    adds = []
+    for s, (a, b) in enumerate(((0, 5), (5, 16))):
+        want, add = eref.sequence(q[a:b].cpu().double().numpy(), kval, vval, args[4][s].cpu(), lens[s], 50, 3, SM, 4)
+        adds.append(add)
+        assert np.all(np.abs(out[a:b].cpu().double().numpy() - want) <= bound(np.abs(vval).max(), lens[s], q.dtype, q.dtype, want))
+    check_mass(mass, before, adds, args[4].cpu(), lens, new, block, 4 * group)

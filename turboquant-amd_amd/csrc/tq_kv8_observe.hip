@@ -12,6 +12,13 @@
 //   kv8_observe_add_kernel    adds those up
 // Products are done twice: keeping the scores would move 4 bytes a (row, token) twice, where a token's keys
 // are 128 bytes for all rows.
+//
+// Bound: few rows by the start (lengths, block table, keys or rows, statistics: a chain of some 12 us in either kernel), many by a
+// SIMD's two waves: some 1000 cycles for 32 x 32 scores, of which the products take 256 and the vector instructions, the
+// exponentials above all, 450; the two hardly overlap.  Four prompts of 8192 tokens, last 32 queries of 48 / 8 heads: 28 + 31 us
+// (13 GFLOP); 384 to 512 queries of 32 / 8 heads after 1000 to 8000 tokens of two sequences: 52 + 69 + 5.  Tried: a row tile at a time
+// with four waves per SIMD (8 waves a workgroup): 62 -> 67 us and 120 as before; rows of 128 with 64 tokens' keys in registers:
+// 155 and 183.
 #include "tq_kv8.h"
 
 namespace {
