@@ -608,7 +608,7 @@ int64_t tq_kv8_observe_workspace_bytes(int num_seqs, int max_q_len, int last, in
  * came from, code -> code * 2^(e - f) rounded to nearest even where it is another (NaN stays).  Rows
  * from bad table entries become zeros, rows for them are dropped.
  * change[s] = keep - seq_lens[s], or 0 for a sequence that is left as it is: tq_plan_args.new_tokens for the lengths and the
- * blocks behind them.  seq_lens is not written.
+ * blocks behind them.  seq_lens is not written, and shares no memory with change.
  * 0 <= sinks + recent <= keep <= longer_than, keep > 0.  Blocks belong to one sequence.  Caches, mass and strides
  * as above.  workspace: tq_kv8_evict_workspace_bytes, 256-byte aligned, no initial contents; calls that overlap must not
  * share it.

@@ -200,6 +200,21 @@ def test_refusals(dev):
     assert empty.shape == (0,)
 
 
+def test_out_apart_from_lengths(dev):
+    """The heads of a sequence read its length while its change is written: a shared tensor is refused, a neighbour is not."""
+    (kc, vc), (kf, vf), _, _, mass, bt = tiles(dev, np.random.default_rng(0), [100, 50], 2, "e4m3", 16)
+    good = dict(k_cache=kc, k_fmt=kf, v_cache=vc, v_fmt=vf, mass=torch.from_numpy(mass).to(dev), block_tables=torch.from_numpy(bt).to(dev),
+                keep=64)
+    both = i32([100, 50, 7, 7, 7], dev)
+    before = kc.clone()
+    for at in (0, 1):
+        with pytest.raises(ValueError, match="share memory"):
+            evict_paged8(**good, seq_lens=both[:2], out=both[at:at + 2])
+    assert torch.equal(kc, before)
+    assert evict_paged8(**good, seq_lens=both[:2], out=both[2:4]).tolist() == [-36, 0]
+    assert both.tolist() == [100, 50, -36, 0, 7]
+
+
 class Session:
     """What a serving loop keeps, and its mirror in plain terms: per sequence and KV head the rows that are cached."""
 

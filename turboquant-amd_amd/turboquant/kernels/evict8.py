@@ -153,7 +153,7 @@ def evict_paged8(
     rounded to it (to nearest even; e4m3 codes that stay normal lose nothing).  Returns int32 [S]: keep - seq_lens,
     or 0 for a sequence left as it is, the new_lens of the plan_step that gives the blocks back; seq_lens and block_tables are
     not changed.  max_seq_len: host-side bound of seq_lens (default: the tables' capacity; tokens behind it do not
-    count).  Blocks must belong to one sequence.  workspace: uint8 of tq_kv8_evict_workspace_bytes(...).
+    count).  Blocks must belong to one sequence; out is memory of its own.  workspace: uint8 of tq_kv8_evict_workspace_bytes(...).
     """
     dev = _lib.require_gpu("evict_paged8", k_cache, v_cache, mass, block_tables, seq_lens, out, workspace)
     nb, heads, kb, kh, vb, vh = _check_pair(k_cache, k_fmt, v_cache, v_fmt, "evict_paged8")
@@ -173,9 +173,11 @@ def evict_paged8(
         raise ValueError("out must be int32 [num_seqs], contiguous")
     if not S:
         return out
+    seq_lens = seq_lens.contiguous()
+    if out.data_ptr() < seq_lens.data_ptr() + 4 * S and seq_lens.data_ptr() < out.data_ptr() + 4 * S:
+        raise ValueError("out and seq_lens share memory")  # (a sequence's heads read its length while its change is written)
     cap = _bound(max_seq_len, mb, k_fmt.block_size)
     keep, longer_than = min(keep, 0x7fff0000), min(longer_than, 0x7fff0000)  # (a sequence holds no more)
-    seq_lens = seq_lens.contiguous()
     need = 0 if cap <= longer_than else _lib.lib().tq_kv8_evict_workspace_bytes(S, heads, keep, k_fmt.block_size)
     ws = _workspace(workspace, need, dev)
     args = _EVICT.pack(k_cache.data_ptr(), v_cache.data_ptr(), mass.data_ptr(), block_tables.data_ptr(), seq_lens.data_ptr(),
