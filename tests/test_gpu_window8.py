@@ -307,6 +307,34 @@ def test_weights_that_are_not_numbers(dev):
     check_mass(mass, before, [np.zeros((1, L))], bt.cpu(), [L], [1], 16, 1)
 
 
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("qd,heads", [(torch.bfloat16, 2), (torch.float32, 1)])
+def test_far_query_among_ordinary_ones(dev, qd, heads, first):
+    """A query whose scores pass fp32's range adds nothing and takes nothing from the rows that share its lanes.
+
+    Its |q| of 3e38 takes a factor of 2^126 or more, and keys of some thousands a scale of 2^5 or more, 2^-3 for the softmax's own: the
+    product passes 2^128.  Ordinary queries are 2^-12 of N(0, 1), so that their scores are those of N(0, 1) rows.  first: it is the
+    call's first row, whose factor rows of padding would take over."""
+    L, new, size = 300, 150, 2.0 ** -12
+    g = torch.Generator(device=dev).manual_seed(heads)
+    k, v = (torch.randn(L, 1, 128, generator=g, device=dev) for _ in range(2))
+    args, (kval, _) = caches(dev, [L], 1, "int8", 16, kv=(k / size, v))
+    kc, kf, _, _, bt = args
+    q = (torch.randn(new, heads, 128, generator=g, device=dev) * size).to(qd)
+    at = 0 if first else 37
+    q[at, 0] = torch.where(torch.rand(128, generator=g, device=dev) < 0.5, -3e38, 3e38).to(qd)
+    assert q.isfinite().all()
+    before = random_mass(kc, 16)
+    got = observe_paged8(q, i32([0, new], dev), kc, kf, bt, i32([L], dev), before.clone())
+    keys = eref.ref.gather(kval, bt[0].cpu(), L)[0][:, 0]
+    add = np.zeros((1, L))
+    for i in range(new):
+        for h in range(heads):
+            if (i, h) != (at, 0):
+                add[0] += eref.weights(q[i, h].cpu().double().numpy(), keys, eref.visible(L - new + i, L, None, 0), SM)
+    check_mass(got, before, [add], bt.cpu(), [L], [new], 16, heads * new)
+
+
 def test_observe_short_sequences(dev):
     """More queries than tokens (rows before the sequence's start see nothing), lengths of 0 and 1, cut lengths."""
     args, (kval, _) = caches(dev, [30, 1, 64], 1, "int8", 16, width=5)

@@ -109,7 +109,8 @@ __device__ __forceinline__ void load_rows(const Observe& p, const Rows& r, int k
     }
     if (h == 0) {
         const int pos = position(p, r, row);
-        b.c1[32 * rt + n] = __builtin_fabsf(a.sm_scale) * kKv8Log2e * back;
+        // (rows that do not exist: scores of 0 * 0, whatever the row whose place they took)
+        b.c1[32 * rt + n] = real ? __builtin_fabsf(a.sm_scale) * kKv8Log2e * back : 0.f;
         b.seen[32 * rt + n] = real && pos >= 0 ? pos + 1 : 0;
     }
 }
@@ -368,7 +369,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv8_observe_sum_kernel(Observe
             b.inv[threadIdx.x] = good ? 1.f / l : 0.f;
         }
         if (__syncthreads_or(bad)) {
-            // rows whose weights are not numbers: operands of zeros, which add nothing
+            // rows whose weights are not numbers: operands and factors of zeros, which add nothing (a factor that passes fp32's range
+            // with a block's scale would make NaN of a lane's sum, and other rows' weights are in it)
+            if (threadIdx.x < kRows && !(b.inv[threadIdx.x] > 0.f)) b.c1[threadIdx.x] = 0.f;
             for (int i = threadIdx.x; i < kTiles * 8 * 64; i += 64 * kWaves) {
                 const int row = 32 * (i >> 9) + (i & 31);
                 if (rb * kRows + row < r.count && !(b.inv[row] > 0.f)) {
