@@ -152,6 +152,17 @@ def test_evict_long(dev, n, keep):
         assert torch.equal(mass[blk[:keep], 0, t[:keep] % 16], m[src])
 
 
+@pytest.mark.parametrize("code,block,hkv,seqs,n,keep", [
+    ("e4m3", 16, 1, 200, 2600, 1500), ("int8", 48, 8, 25, 1900, 1050), ("e4m3", 64, 2, 100, 2100, 1301), ("int8", 16, 1, 193, 34000, 900)])
+def test_evict_many_rounds(dev, code, block, hkv, seqs, n, keep):
+    """A workgroup per (sequence, KV head), of which two sequences are cut, over 4 to 6 rounds of 256 kept rows: blocks that reach from one
+    round into the next (48), scales that differ, numbers of one sequence that do not fit the plan's registers (34000)."""
+    rng = np.random.default_rng(n)
+    lens = [0] * seqs
+    lens[3], lens[seqs - 1] = n, keep + 77
+    compare(dev, rng, lens, hkv, code, block, keep, 200, 5, odd=True)
+
+
 def test_evict_strided(dev):
     """K and V tiles side by side in one tensor, mass with other strides, strided lengths, a stream of its own."""
     rng = np.random.default_rng(4)

@@ -614,7 +614,9 @@ __global__ __launch_bounds__(kPlan) void kv8_evict_segment_kernel(Evict p) {
         const int sk = cur.ek && mk - cur.ek < 63 ? mk - cur.ek : 63, sv = cur.ev && mv - cur.ev < 63 ? mv - cur.ev : 63;
         const int sh = __shfl(sk | sv << 8, (first_of(u) + (lane & 15)) & 63, 64);
         const Unit x = arrange<ENC>(cur.raw, cur.row, sh);
-        asm volatile("" ::"v"(x.mass));  // (all of the round's loads are back before the barrier)
+        // (all of the round's rows and scales are in registers before any wave stores; the compiler has the same wait at the top of the
+        // loop, but nothing else here asks for it)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         load(u + kRound, next, cur);
         next = place(u + 2 * kRound);
