@@ -163,6 +163,29 @@ def test_evict_many_rounds(dev, code, block, hkv, seqs, n, keep):
     compare(dev, rng, lens, hkv, code, block, keep, 200, 5, odd=True)
 
 
+@pytest.mark.parametrize("code,block,keep", [("e4m3", 16, 9001), ("int8", 48, 4000), ("e4m3", 64, 6143)])
+def test_evict_long_scales(dev, code, block, keep):
+    """Few segments over many tickets, with scales that differ: a block's scale is written when no unit needs the old one."""
+    rng = np.random.default_rng(keep)
+    compare(dev, rng, [20000, keep + 1, 9500], 1, code, block, keep, 500, 3, odd=True)
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("block", [80, 128, 160])
+def test_evict_odd_contents_of_large_blocks(dev, code, block):
+    """The path through the workspace, over several kept blocks: odd contents, bad table entries, blocks of no power of two."""
+    rng = np.random.default_rng(block)
+
+    def spoil(bt):
+        bt[0, 1], bt[1, -1], bt[2, :], bt[3, 0] = -1, 10 ** 6, -3, 1 << 30
+        bt[4, 2:] = -1
+
+    lens = [1400, 1390, 900, 1500, 1450, 700, 650]
+    compare(dev, rng, lens, 2, code, block, 650, 90, 20, odd=True)
+    compare(dev, rng, lens, 2, code, block, 650, 90, 20, odd=True, spoil=spoil)
+    compare(dev, rng, lens, 2, code, block, 641, 0, 0, odd=True, spoil=spoil)
+
+
 def test_evict_strided(dev):
     """K and V tiles side by side in one tensor, mass with other strides, strided lengths, a stream of its own."""
     rng = np.random.default_rng(4)

@@ -101,6 +101,29 @@ def test_decode(dev, code, qd, block, window, sinks):
     check_mass(mass, before, adds, bt.cpu(), lens, [min(L, 1) for L in lens], block, 1)
 
 
+@pytest.mark.parametrize("code,qd,group,window,sinks", [("e4m3", torch.bfloat16, 1, None, 0), ("int8", torch.float16, 16, None, 0),
+                                                        ("e4m3", torch.float32, 16, 8000, 40), ("int8", torch.bfloat16, 1, 6000, 0)])
+def test_mass_of_many_pieces(dev, code, qd, group, window, sinks):
+    """A segment shared by more waves than a wave has lanes (at least two steps of 32 tokens each), one and sixteen query heads to it.
+
+    (A row's sum is then at most five tokens' in a lane and nine joins of four roundings, less than the tokens / 16 that
+    weight_error counts.)"""
+    lens = [9000, 0, 700]
+    args, (kval, vval) = caches(dev, lens, 1, code, 16, seed=group)
+    kc, kf, vc, vf, bt = args
+    q = torch.randn(3, group, 128, generator=torch.Generator(device=dev).manual_seed(5), device=dev).to(qd)
+    before = random_mass(kc, 16)
+    mass = before.clone()
+    out = decode_paged8(q, *args, i32(lens, dev), window=window, sinks=sinks, mass=mass)
+    adds = []
+    for s, L in enumerate(lens):
+        want, add = eref.sequence(q[s:s + 1].cpu().double().numpy(), kval, vval, bt[s].cpu(), L, window, sinks, SM) if L else (
+            np.zeros((1, group, 128)), np.zeros((1, 0)))
+        adds.append(add)
+        assert np.all(np.abs(out[s].cpu().double().numpy() - want[0]) <= bound(np.abs(vval).max(), L, qd, qd, want[0]))
+    check_mass(mass, before, adds, bt.cpu(), lens, [1, 0, 1], 16, group)
+
+
 @pytest.mark.parametrize("code,qd,block", [("e4m3", torch.bfloat16, 16), ("int8", torch.float16, 48), ("e4m3", torch.float32, 64)])
 @pytest.mark.parametrize("window,sinks", WINDOWS)
 @pytest.mark.parametrize("group", [1, 5])
