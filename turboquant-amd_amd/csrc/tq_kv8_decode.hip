@@ -20,9 +20,9 @@
 // Bound: HBM reads, 256 bytes per token and KV head: 64 x 32768 tokens of 8 heads in 762 us, 5.6 TB/s, where a large
 // copy moves 4.9.  With a window the same per visible token: 64 sequences of 300 to 32768 tokens, window 4096, 384 MB in 82 us.
 // With accumulated weights each step's scores are kept for kv8_decode_mass_kernel, 4 bytes a head and token: at 64 x 32768 tokens
-// 402 MB more are written and the kernel takes 1078 us instead of 762; the same stores into a buffer that stays in
-// L2 cost 25 us, so it is the writes among the reads that memory takes badly (nontemporal stores, another order of the
-// scores and stores behind the next loads changed nothing).  Reading the keys again instead would move 128 bytes a token for all heads,
+// 402 MB more are written (409 by counters) and the kernel takes 1078 us instead of 762; the same stores into a buffer that stays in
+// L2 cost 25 us, so it is the writes among the reads that memory takes badly (nontemporal stores and stores behind the next
+// loads changed nothing, scores that lie by head instead of by token 1 %).  Reading the keys again instead would move 128 bytes a token for all heads,
 // at six heads a KV head as long.  Small calls: launches, start-up (the search for the wave's part, block table, scales) and
 // the merge, about 15 us.
 #include "tq_kv8.h"

@@ -9,19 +9,24 @@
 //   kv8_evict_move_kernel     any workgroup moves any unit; units wait for those that what they overwrite goes to: few segments
 //   gather and scatter        through the workspace: blocks of more than 64 rows, whose scales take a kernel of their own
 //
-// Bound: memory, 512 bytes of codes a kept token: 32 x 4352 tokens of 8 heads cut to 4096, 546 MB in 182 us, 3.0 TB/s where a
+// Bound: memory, 512 bytes of codes a kept token: 32 x 4352 tokens of 8 heads cut to 4096, 546 MB in 192 us, 2.8 TB/s where a
 // copy moves 4.7.  One compute unit has some 20 GB/s of it, so the segment kernel needs most of them busy and 16 to 20 kB a round
-// under way; the move kernel pays for its flags (213 us there, 157 if nothing had to wait) and, where single tokens stay,
-// for V's words, four times the bytes of a token (16 sequences of 3001 to 32768 tokens cut to 8190: 343 MB in 28 + 130 us).  One prompt
-// of 32768: 43 us, of them 30 the plan's, one workgroup for 32768 numbers.
+// under way; the move kernel pays for its flags (208 us there, some 50 less where nothing has to wait) and, where single tokens stay,
+// for V's words of four tokens: 16 sequences of 3001 to 32768 tokens cut to 8190 need 168 MB of codes read and as much written, and by
+// counters 279 MB are read, in 29 + 149 us.  One prompt of 32768: 31 us for the plan, one workgroup for 32768 numbers, and 11.
+// (Kernel times of a fresh cache's first cut.  Cut again, its scales have met and fewer rows are rounded: 185, 29 + 130, 31 + 11.)
 #include "tq_kv8.h"
 
 namespace {
 
 constexpr int kInPlace = 64;                      // rows of a block, at most, that move without the workspace
 constexpr int kMove = 4;                          // waves, and units, of a ticket
-// Segments from which on a workgroup takes a whole one: that keeps most compute units busy and needs no flags (256 segments, 32 x
-// 4352 tokens cut to 4096: 180 us against 228; 128 segments of up to 32768 cut to 8190: 345 against 175)
+// Segments from which on a workgroup takes a whole one: with most of them cut that keeps most compute units busy and needs no flags (kernel
+// times; 4352 tokens cut to 4096, 8 heads, all sequences: 176 segments 166 us against the plan's and the move kernel's 161, 192: 177
+// against 179, 256: 192 against 236; 128 segments, 80 of them of up to 26172 tokens cut to 8190: 350 against 177).  The lengths are on the
+// device, so those that stay as they are count too, and a call of many sequences of which few are cut pays for it: of 256 segments
+// 8 cut 135 against 41, 64: 147 against 83, 128: 166 against 135, 160: 177 against 161, 192: 181 against 186; one sequence of
+// 32768 cut to 8190 among 24: 331 against 59.
 constexpr int kSegments = 192;
 constexpr int kPad = 32;                          // words between tickets: a cache line each
 constexpr int kUnit = 16;                         // rows that a wave moves
@@ -493,8 +498,7 @@ __global__ __launch_bounds__(256) void kv8_evict_scatter_kernel(Evict p) {
 template <int ENC>
 __global__ __launch_bounds__(64 * kMove, 8) void kv8_evict_move_kernel(Evict p) {
     __shared__ int s_ticket;
-    // (the 8 XCDs have a segment's workgroups in turn: with all of them on one, 32 x 4352 tokens cut to 4096 take 284 us instead
-    // of 213)
+    // (the 8 XCDs have a segment's workgroups in turn: with all of them on one, 32 x 4352 tokens cut to 4096 took a third longer, 284 us)
     const uint32_t seg = blockIdx.x / (uint32_t)p.items;
     const int s = (int)(seg / (uint32_t)p.a.num_kv_heads), kh = (int)seg - s * p.a.num_kv_heads;
     if (!p.cut[seg]) return;

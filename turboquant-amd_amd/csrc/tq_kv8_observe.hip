@@ -14,11 +14,11 @@
 // are 128 bytes for all rows.
 //
 // Bound: few rows by the start (lengths, block table, keys or rows, statistics: a chain of some 12 us in either kernel), many by a
-// SIMD's two waves: some 1000 cycles for 32 x 32 scores, of which the products take 256 and the vector instructions, the
-// exponentials above all, 450; the two hardly overlap.  Four prompts of 8192 tokens, last 32 queries of 48 / 8 heads: 28 + 31 us
-// (13 GFLOP); 384 to 512 queries of 32 / 8 heads after 1000 to 8000 tokens of two sequences: 52 + 69 + 5.  Tried: a row tile at a time
-// with four waves per SIMD (8 waves a workgroup): 62 -> 67 us and 120 as before; rows of 128 with 64 tokens' keys in registers:
-// 155 and 183.
+// SIMD's two waves: by counters (the second call below) 990 cycles for 32 x 32 scores in the statistics and 1200 in the sums, of which the
+// products take 256 and other vector instructions, the exponentials above all, 550 and 660; the two hardly overlap.  Four prompts of
+// 8192 tokens, last 32 queries of 48 / 8 heads: 28 + 32 us (13 GFLOP); 384 to 512 queries of 32 / 8 heads after 1000 to 8000 tokens of two
+// sequences: 53 + 70 + 5.  f32 queries: twice the products, 94 and 165 us a call instead of 55 and 113.  Tried: a row tile at a time with four
+// waves per SIMD (8 waves a workgroup): 62 -> 67 us and 120 as before; rows of 128 with 64 tokens' keys in registers: 155 and 183.
 #include "tq_kv8.h"
 
 namespace {

@@ -351,7 +351,8 @@ class TurboQuantPagedImpl:
 
     Over an 8-bit cache alone: sliding_window (None: every token) and sinks, the tokens at a sequence's start that
     stay visible; mass, accumulated attention weights (state.allocate_mass) to which forward adds those of every decode
-    query and of the last observe_last queries of every prompt, for state.evict.
+    query and, of every call's prompts (or chunks of them), those of the last observe_last queries, for state.evict.  Evicting
+    takes a model all of whose layers are 8-bit ones.
     """
 
     forward_includes_kv_cache_update = False  # do_kv_cache_update is called separately

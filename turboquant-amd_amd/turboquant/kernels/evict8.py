@@ -2,7 +2,9 @@
 
 Every cached token has a number per KV head, the sum of the softmax weights it got: mass, float32 [num_blocks,
 num_kv_heads, block_size], paged like the cache.  decode_paged8(..., mass=mass) adds a step's weights,
-observe_paged8 those of a prompt's queries; new tokens start from 0 in either, so a recycled block needs no clearing.
+observe_paged8 those of a prompt's queries; new tokens start from 0 in either, so a recycled block needs no clearing, as long as
+every token is new in one of them: prompts are observed (last=1 is enough), and a request that plan_step could not serve is
+left out of the step, whose calls would take its last cached tokens for new ones.
 evict_paged8 then cuts each long sequence to its first, its last and its heaviest tokens, in place, and its result
 is what plan_step takes as new_lens to give the blocks behind them back:
 
@@ -10,8 +12,9 @@ is what plan_step takes as new_lens to give the blocks behind them back:
     plan_step(lens, change, tables, ring, pool, block_size, 0)
 
 Layers share block tables, so each of them evicts, with its own cache and mass and the same keep, before
-the one plan_step.  A cached token's index is then less than its position: a caller adds what a sequence gave up (the
-sums of -change) to the positions that plan_step returns before apply_rope.
+the one plan_step.  That takes a model all of whose layers are 8-bit ones: a packed layer has no eviction, and would be left with its
+first `keep` tokens.  A cached token's index is then less than its position: a caller adds what each sequence gave up (the
+sums of -change, once for each of its new tokens) to the positions that plan_step returns before apply_rope.
 """
 
 from __future__ import annotations
